@@ -268,6 +268,41 @@ MC_SM100_API mc_status_t mc_sm100_residual_rmsnorm_rows(uint16_t* d_res, const u
                                                         uint32_t rows, uint32_t n, float eps,
                                                         void* stream, int32_t pdl);
 
+/* ------------------------------------------- linear with a fused epilogue --- */
+
+/* Activations of mc_sm100_linear_epilogue, in fp32:
+ * relu max(z, 0) (a NaN stays one), gelu z / 2 * (1 + erf(z / sqrt 2)), gelu_tanh
+ * z / 2 * (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))), silu z / (1 + e^-z). */
+typedef enum mc_sm100_activation_t {
+    MC_SM100_ACT_NONE = 0, MC_SM100_ACT_RELU = 1, MC_SM100_ACT_GELU = 2, MC_SM100_ACT_GELU_TANH = 3, MC_SM100_ACT_SILU = 4
+} mc_sm100_activation_t;
+
+typedef struct mc_sm100_epilogue_t {
+    uint32_t struct_size;            /* caller sets sizeof(mc_sm100_epilogue_t) */
+    uint32_t activation;             /* mc_sm100_activation_t */
+    uint32_t gated;                  /* 1: W's rows are interleaved (gate_j, up_j) as mc_sm100_interleave_rows leaves them */
+    uint32_t x_stride, y_stride, residual_stride;   /* elements from row to row; 0 = compact (K, N_out, N_out) */
+    const uint16_t* d_bias;          /* [N] bf16 or NULL (gated: interleaved like the rows of W) */
+    const uint16_t* d_residual;      /* [M, N_out] bf16 or NULL; may be d_y itself, with the same stride */
+    uint32_t reserved[2];            /* must be zero */
+} mc_sm100_epilogue_t;
+
+/* A linear for any number of rows, from one token to a long prompt chunk, with what follows it:
+ *   z[m,n] = scale[n] * sum_k W[n,k] x[m,k] + bias[n]
+ *   v[m,j] = act(z[m,j])                        N_out = N
+ *          = act(z[m,2j]) * z[m,2j+1]           gated, N_out = N / 2
+ *   y[m,j] = bf16( v[m,j] + residual[m,j] )
+ * Everything between the products and y stays in fp32: one rounding.  (mc_sm100_gate_up_swiglu rounds gate and up to
+ * bf16 first, as the reference's pair of kernels does; this call does not.)  d_scale == NULL: bf16 weights (d_w read as
+ * uint16_t), otherwise e4m3 codes with one fp32 scale per row (codes 0x7F / 0xFF count as +/-480, as everywhere here).
+ * epilogue == NULL: the plain linear.  Any M, N, K >= 1 (gated: N even) and any stride >= the row; operands aligned to
+ * their elements.  16-byte aligned d_w and d_x, K * (bytes per weight) and x_stride * 2 multiples of 16 take the
+ * tensor-core kernels that stream by TMA; anything else a slower kernel with plain loads.  x and y must not overlap.
+ * Results do not depend on the launch: no atomics, a fixed order of every sum. */
+MC_SM100_API mc_status_t mc_sm100_linear_epilogue(const void* d_w, const float* d_scale, const uint16_t* d_x, uint16_t* d_y,
+                                                  uint32_t M, uint32_t N, uint32_t K, const mc_sm100_epilogue_t* epilogue,
+                                                  void* stream, int32_t pdl);
+
 /* ------------------------------------------------------- lm_head / greedy --- */
 
 /* Greedy argmax over bf16 logits compared as fp32, ties to the lowest index,
@@ -352,6 +387,62 @@ MC_SM100_API mc_status_t mc_sm100_sample_topk_topp_sharded(
     const mc_sm100_sampling_config_t* d_cfg, uint64_t* d_rng_state, int32_t* d_out_token,
     const uint64_t* d_region_peers, const void* d_my_region, uint32_t max_rows, uint32_t* d_step,
     uint32_t rank, uint32_t world, uint64_t timeout_ns, int32_t* d_status, void* stream, int32_t pdl);
+
+/* ------------------------------------------------ rules on logits, history --- */
+
+/* What a row's request asks of its logits; read by the kernel at run time from a fixed device address, so that a
+ * captured step can be replayed with other values.  All zero except history_slot = mask_row = -1 leaves a row as it is. */
+typedef struct mc_sm100_logits_config_t {
+    float    rep_penalty;            /* tokens the history has seen: l > 0 ? l / rep : l * rep; 1 (or 0) = off */
+    float    freq_penalty;           /* l -= freq * (how often the token was generated) */
+    float    pres_penalty;           /* l -= pres if the token was generated at all */
+    int32_t  history_slot;           /* row of counts / seen, < 0 = no history: the three above do nothing
+                                      * (counts are looked at where the seen bit is set) */
+    int32_t  mask_row;               /* row of masks, < 0 = every token allowed */
+    uint32_t bias_begin, bias_count; /* this row's entries of bias_token / bias_value */
+    uint32_t flags;                  /* must be zero */
+} mc_sm100_logits_config_t;
+
+/* Tables over the whole vocabulary (also when the logits are a shard of it).  A table of bits holds token t in bit t % 32
+ * of word t / 32, rows of ceil(table_vocab / 32) words. */
+typedef struct mc_sm100_logits_tables_t {
+    uint32_t struct_size;            /* caller sets sizeof(mc_sm100_logits_tables_t) */
+    uint32_t table_vocab;
+    uint32_t n_slots, n_masks, n_bias;
+    uint32_t reserved;               /* must be zero */
+    const int32_t*  d_counts;        /* [n_slots, table_vocab] how often each token was generated, kept by mc_sm100_token_history */
+    const uint32_t* d_seen;          /* [n_slots, words] tokens of the prompt or generated */
+    const uint32_t* d_mask;          /* [n_masks, words] grammar masks, bit 1 = allowed */
+    const int32_t*  d_bias_token;    /* [n_bias] */
+    const float*    d_bias_value;    /* [n_bias] */
+    int32_t* d_status;               /* optional: set to 1 when a row names a slot, a mask or entries outside the tables */
+} mc_sm100_logits_tables_t;
+
+/* Edits bf16 logits [n_rows, vocab] by the rows' rules, in this order and in fp32 with one rounding at the end:
+ * repetition penalty, frequency and presence penalty, biases (a token listed several times takes their sum, added in
+ * list order; tokens outside the logits are passed over), grammar mask (a token that is not allowed becomes -infinity,
+ * whatever it held, a NaN too).  A row whose mask leaves nothing becomes -infinity throughout.  A row that names a slot,
+ * mask or entries outside the tables goes without them, and *d_status says so.  d_out may be d_logits itself with the
+ * same stride; logits kept for their probabilities go to another buffer.  Columns from vocab to the stride are not
+ * touched.  index_base: token of column 0 (vocab shards).  Replaces rep_penalty_mark / rep_penalty_apply
+ * (native/kernels/sm120/sampling.cu:293-324) in front of mc_sm100_sample_topk_topp / mc_sm100_argmax_bf16; biases, masks
+ * and the other two penalties have no counterpart there.  n_rows <= 65535. */
+MC_SM100_API mc_status_t mc_sm100_logits_process(const uint16_t* d_logits, uint16_t* d_out, uint32_t n_rows, uint32_t vocab,
+                                                 uint32_t row_stride, uint32_t out_stride, int32_t index_base,
+                                                 const mc_sm100_logits_config_t* d_cfg, const mc_sm100_logits_tables_t* tables,
+                                                 void* stream, int32_t pdl);
+
+/* The history those penalties read.  Sequence i (of n_seqs) is d_tokens[d_offsets[i] .. d_offsets[i + 1]) -- without
+ * d_offsets the single token i, as a sampler leaves them -- and belongs to slot d_slots[i] (without d_slots: i).  Its
+ * first d_prompt_len[i] tokens (without d_prompt_len: none) are prompt: they set the seen bit only; the others also add 1
+ * to their count.  rebuild != 0: every slot named starts from nothing (a request is admitted, or comes back), otherwise
+ * the tokens are added to what is there.  Several sequences may name one slot.  Tokens outside [0, table_vocab) are passed
+ * over (a sampler's -1); a sequence whose slot is outside [0, n_slots) or whose offsets leave [0, n_tokens] is passed over
+ * and sets *d_status (optional) to 1.  Slots that no sequence names are not touched. */
+MC_SM100_API mc_status_t mc_sm100_token_history(int32_t* d_counts, uint32_t* d_seen, uint32_t n_slots, uint32_t table_vocab,
+                                                const int32_t* d_tokens, uint32_t n_tokens, const uint32_t* d_offsets,
+                                                const uint32_t* d_prompt_len, const int32_t* d_slots, uint32_t n_seqs,
+                                                int32_t rebuild, int32_t* d_status, void* stream, int32_t pdl);
 
 /* ------------------------------------------------- host-buffer convenience -- */
 

@@ -65,6 +65,9 @@ SIGNATURES = {
     "mc_sm100_sampling_exchange_bytes": (C.c_size_t, [_u32, _u32]),
     "mc_sm100_sample_topk_topp_sharded": (_i32, [_vp, _u32, _u32, _u32, _i32, _vp, _vp, _vp, _vp, _vp, _u32, _vp, _u32, _u32,
                                                  C.c_uint64, _vp, _vp, _i32]),
+    "mc_sm100_linear_epilogue": (_i32, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _i32]),
+    "mc_sm100_logits_process": (_i32, [_vp, _vp, _u32, _u32, _u32, _u32, _i32, _vp, _vp, _vp, _i32]),
+    "mc_sm100_token_history": (_i32, [_vp, _vp, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _u32, _i32, _vp, _vp, _i32]),
     "mc_sm100_linear_host": (_i32, [_i32, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp, C.c_size_t, _vp]),
     "mc_sm100_stack_sizes": (_i32, [_vp, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]),
     "mc_sm100_stack_section": (_i32, [_vp, _u32, _u32, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]),
@@ -315,6 +318,50 @@ def sample_topk_topp_sharded(logits, n_rows, vocab, row_stride, index_base, cfg,
     _check(lib().mc_sm100_sample_topk_topp_sharded(_p(logits), n_rows, vocab, row_stride, index_base, _p(cfg), _p(rng_state),
                                                    _p(out_token), _p(region_peers), _p(my_region), max_rows, _p(step), rank, world,
                                                    timeout_ns, _p(status), _stream(stream), int(pdl)))
+
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+class Epilogue(C.Structure):
+    _fields_ = [("struct_size", _u32), ("activation", _u32), ("gated", _u32), ("x_stride", _u32), ("y_stride", _u32),
+                ("residual_stride", _u32), ("d_bias", _vp), ("d_residual", _vp), ("reserved", _u32 * 2)]
+
+
+def launch_linear_epilogue(w, scale, x, y, M, N, K, bias=None, residual=None, activation="none", gated=False, x_stride=0,
+                           y_stride=0, residual_stride=0, stream=None, pdl=False):
+    """y = act(x W^T * scale + bias) [* up] + residual for any M; activation: a key of ACTIVATIONS."""
+    e = Epilogue(C.sizeof(Epilogue), ACTIVATIONS[activation], int(gated), x_stride, y_stride, residual_stride, _p(bias), _p(residual))
+    _check(lib().mc_sm100_linear_epilogue(_p(w), _p(scale), _p(x), _p(y), M, N, K, C.cast(C.byref(e), _vp), _stream(stream), int(pdl)))
+
+
+class LogitsTables(C.Structure):
+    _fields_ = [("struct_size", _u32), ("table_vocab", _u32), ("n_slots", _u32), ("n_masks", _u32), ("n_bias", _u32), ("reserved", _u32),
+                ("d_counts", _vp), ("d_seen", _vp), ("d_mask", _vp), ("d_bias_token", _vp), ("d_bias_value", _vp), ("d_status", _vp)]
+
+
+def logits_tables(table_vocab, counts=None, seen=None, masks=None, bias_token=None, bias_value=None, status=None) -> LogitsTables:
+    """Tables of logits_process out of device tensors (their sizes give the numbers of rows); the caller keeps the tensors."""
+    words = (table_vocab + 31) // 32
+    return LogitsTables(C.sizeof(LogitsTables), table_vocab, counts.numel() // table_vocab if counts is not None else 0,
+                        masks.numel() // words if masks is not None else 0, bias_token.numel() if bias_token is not None else 0, 0,
+                        _p(counts), _p(seen), _p(masks), _p(bias_token), _p(bias_value), _p(status))
+
+
+def logits_process(logits, out, n_rows, vocab, row_stride, out_stride, cfg, tables, index_base=0, stream=None, pdl=False):
+    """cfg: device tensor of n_rows x 8 words (rep, freq, pres penalty as f32 bits, history slot, mask row, bias begin, bias count, 0)."""
+    _check(lib().mc_sm100_logits_process(_p(logits), _p(out), n_rows, vocab, row_stride, out_stride, index_base, _p(cfg),
+                                         C.cast(C.byref(tables), _vp), _stream(stream), int(pdl)))
+
+
+def token_history(counts, seen, tokens, n_seqs, table_vocab, offsets=None, prompt_len=None, slots=None, n_tokens=None, n_slots=None,
+                  rebuild=False, status=None, stream=None, pdl=False):
+    if n_tokens is None:
+        n_tokens = tokens.numel()
+    if n_slots is None:
+        n_slots = counts.numel() // table_vocab
+    _check(lib().mc_sm100_token_history(_p(counts), _p(seen), n_slots, table_vocab, _p(tokens), n_tokens, _p(offsets), _p(prompt_len),
+                                        _p(slots), n_seqs, int(rebuild), _p(status), _stream(stream), int(pdl)))
 
 
 def linear_host(kind, w, scale, h_x, h_y, M, N, K, x_stage, y_stage, workspace=None, ws_size=0, stream=None):

@@ -1,0 +1,136 @@
+// linear_epilogue.cu -- mc_sm100_linear_epilogue: checks, choice of a kernel, and the kernel that takes every shape.
+#include "linear_epilogue.cuh"
+
+namespace mcl {
+
+namespace {
+
+// ---- any shape, any stride, any alignment ------------------------------------------------------
+// 64 x 64 tiles of y, K in steps of 32, mma.sync m16n8k16 with fp32 accumulators, plain element loads with bounds.
+// e4m3 codes are widened to bf16 (exact).  Each warp owns a 32 x 32 quarter.
+constexpr uint32_t kAnyTile = 64, kAnyK = 32, kAnyPitch = kAnyK + 8, kAnyThreads = 128;
+
+__device__ __forceinline__ void any_mma(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+template <int WB>
+__global__ void __launch_bounds__(kAnyThreads)
+linear_any_kernel(const void* __restrict__ w, const uint16_t* __restrict__ x, uint32_t x_stride, uint32_t M, uint32_t N, uint32_t K,
+                  uint32_t n_tiles, const EpiArgs e) {
+    __shared__ uint16_t sx[kAnyTile][kAnyPitch], sw[kAnyTile][kAnyPitch];
+    __shared__ float sz[kAnyTile][kAnyTile + 1];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
+    const uint32_t m0 = (blockIdx.x / n_tiles) * kAnyTile, n0 = (blockIdx.x % n_tiles) * kAnyTile;
+    const uint32_t wm = (warp & 1u) * 32u, wn = (warp >> 1) * 32u;
+    pdl_trigger();
+    pdl_wait();
+    float acc[2][4][4] = {};
+    for (uint32_t k0 = 0; k0 < K; k0 += kAnyK) {
+        for (uint32_t i = tid; i < kAnyTile * kAnyK; i += kAnyThreads) {
+            const uint32_t r = i / kAnyK, c = i % kAnyK, k = k0 + c;
+            sx[r][c] = (m0 + r < M && k < K) ? x[(size_t)(m0 + r) * x_stride + k] : (uint16_t)0;
+            uint16_t v = 0;
+            if (n0 + r < N && k < K) {
+                if constexpr (WB == 2) v = static_cast<const uint16_t*>(w)[(size_t)(n0 + r) * K + k];
+                else v = f32_to_bf16_bits(e4m3_to_f32(static_cast<const uint8_t*>(w)[(size_t)(n0 + r) * K + k]));
+            }
+            sw[r][c] = v;
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t kk = 0; kk < kAnyK; kk += 16) {
+            uint32_t a[2][4], b[4][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+                    a[i][h] = *reinterpret_cast<const uint32_t*>(&sx[wm + 16 * i + g + 8 * (h & 1)][kk + 2 * t + 8 * (h >> 1)]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) b[j][h] = *reinterpret_cast<const uint32_t*>(&sw[wn + 8 * j + g][kk + 2 * t + 8 * h]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) any_mma(acc[i][j], a[i], b[j]);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int h = 0; h < 4; ++h) sz[wm + 16 * i + g + 8 * (h >> 1)][wn + 8 * j + 2 * t + (h & 1)] = acc[i][j][h];
+    __syncthreads();
+    const uint32_t cols = e.gated ? kAnyTile / 2 : kAnyTile, c0 = e.gated ? n0 / 2 : n0, n_out = e.gated ? N / 2 : N;
+    auto z_of = [&](uint32_t r, uint32_t n_rel) {
+        float z = sz[r][n_rel];
+        const uint32_t n = n0 + n_rel;
+        if (e.scale != nullptr) z *= e.scale[n];
+        if (e.bias != nullptr) z += __uint_as_float((uint32_t)e.bias[n] << 16);
+        return z;
+    };
+    for (uint32_t i = tid; i < kAnyTile * cols; i += kAnyThreads) {
+        const uint32_t r = i / cols, c = i % cols, m = m0 + r, j = c0 + c;
+        if (m >= M || j >= n_out) continue;
+        float v = e.gated ? epi_act(z_of(r, 2 * c), e.act) * z_of(r, 2 * c + 1) : epi_act(z_of(r, c), e.act);
+        if (e.res != nullptr) v += __uint_as_float((uint32_t)e.res[(size_t)m * e.res_stride + j] << 16);
+        e.y[(size_t)m * e.y_stride + j] = f32_to_bf16_bits(v);
+    }
+}
+
+mc_status_t linear_any(int wb, const void* w, const uint16_t* x, uint32_t x_stride, uint32_t M, uint32_t N, uint32_t K,
+                       const EpiArgs& e, cudaStream_t stream, bool pdl) {
+    const uint64_t nt = (N + kAnyTile - 1ull) / kAnyTile, mt = (M + kAnyTile - 1ull) / kAnyTile;
+    if (nt * mt > 0x7FFFFFFFull) {
+        set_error("mc_sm100_linear_epilogue: M=%u N=%u make too many tiles", M, N);
+        return MC_E_UNSUPPORTED;
+    }
+    auto kern = wb == 2 ? linear_any_kernel<2> : linear_any_kernel<1>;
+    (void)launch(kern, dim3((uint32_t)(nt * mt)), dim3(kAnyThreads), 0, stream, pdl, w, x, x_stride, M, N, K, (uint32_t)nt, e);
+    MCL_CHECK_LAUNCH("linear_any");
+    return MC_OK;
+}
+
+bool aligned_to(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1u)) == 0u; }
+
+}  // namespace
+
+}  // namespace mcl
+
+using namespace mcl;
+
+extern "C" mc_status_t mc_sm100_linear_epilogue(const void* d_w, const float* d_scale, const uint16_t* d_x, uint16_t* d_y, uint32_t M,
+                                                uint32_t N, uint32_t K, const mc_sm100_epilogue_t* ep, void* stream, int32_t pdl) {
+    clear_error();
+    const int wb = d_scale == nullptr ? 2 : 1;
+    mc_sm100_epilogue_t d{};
+    if (ep != nullptr) {
+        if (ep->struct_size != sizeof(mc_sm100_epilogue_t) || ep->activation > MC_SM100_ACT_SILU || ep->gated > 1u ||
+            ep->reserved[0] != 0u || ep->reserved[1] != 0u) {
+            set_error("mc_sm100_linear_epilogue: invalid epilogue (struct_size=%u activation=%u gated=%u)", ep->struct_size,
+                      ep->activation, ep->gated);
+            return MC_E_INVALID_ARGUMENT;
+        }
+        d = *ep;
+    }
+    const uint32_t n_out = d.gated ? N / 2u : N;
+    const uint32_t xs = d.x_stride ? d.x_stride : K, ys = d.y_stride ? d.y_stride : n_out, rs = d.residual_stride ? d.residual_stride : n_out;
+    if (d_w == nullptr || d_x == nullptr || d_y == nullptr || M == 0 || N == 0 || K == 0 || (d.gated && (N & 1u) != 0) || xs < K ||
+        ys < n_out || (d.d_residual != nullptr && rs < n_out) || !aligned_to(d_w, (uintptr_t)wb) || !aligned_to(d_scale, 4) ||
+        !aligned_to(d_x, 2) || !aligned_to(d_y, 2) || !aligned_to(d.d_bias, 2) || !aligned_to(d.d_residual, 2)) {
+        set_error("mc_sm100_linear_epilogue: invalid args (M=%u N=%u K=%u gated=%u x_stride=%u y_stride=%u residual_stride=%u)", M, N, K,
+                  d.gated, xs, ys, rs);
+        return MC_E_INVALID_ARGUMENT;
+    }
+    if (d.d_residual == d_y && rs != ys) {
+        set_error("mc_sm100_linear_epilogue: residual and y are one buffer with strides %u and %u", rs, ys);
+        return MC_E_INVALID_ARGUMENT;
+    }
+    const EpiArgs e{d_scale, d.d_bias, d.d_residual, d_y, ys, rs, d.activation, d.gated};
+    return linear_any(wb, d_w, d_x, xs, M, N, K, e, (cudaStream_t)stream, pdl != 0);
+}

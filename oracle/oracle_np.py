@@ -297,3 +297,86 @@ def sample_topk_topp(logits_u16: np.ndarray, temperature: float, top_p: float, t
             pick = i
             break
     return int(order[pick]) + index_base, state, margin
+
+
+# ---- linear with a fused epilogue, rules on logits, token history -------------------------------------------------
+def linear_epilogue_f64(w, x, scale=None, bias=None, residual=None, act="none", gated=False, u=2.0 ** -23):
+    """The formula in 64 bits, and a bound on |kernel - formula|.  w, x: real values [N, K], [M, K]; bias [N], residual
+    [M, N_out].  Bound: K products added one after another in fp32 are off by at most u * (K + 2) * sum |w x| with
+    u = 2^-23 (an adder that cuts instead of rounding); the activations have slopes up to 1.13 and are themselves computed
+    to 2^-16 relative (erfc and e^z at arguments of size 90 pass on 90 * 2^-23 of theirs); one rounding to bf16 (2^-8)."""
+    from math import sqrt, pi
+    w, x = np.asarray(w, np.float64), np.asarray(x, np.float64)
+    s = np.ones(w.shape[0]) if scale is None else np.asarray(scale, np.float64)
+    b = np.zeros(w.shape[0]) if bias is None else np.asarray(bias, np.float64)
+    z = (x @ w.T) * s + b
+    ez = u * (w.shape[1] + 2) * ((np.abs(x) @ np.abs(w).T) * s + np.abs(b)) + u * np.abs(z)
+
+    def f(v):
+        if act == "relu":
+            return np.maximum(v, 0.0)
+        if act == "gelu":
+            from scipy.special import erfc
+            return 0.5 * v * erfc(-v / sqrt(2.0))
+        if act == "gelu_tanh":
+            return 0.5 * v * (1.0 + np.tanh(sqrt(2.0 / pi) * (v + 0.044715 * v ** 3)))
+        if act == "silu":
+            return v / (1.0 + np.exp(-v))
+        return v
+    a = f(z[:, 0::2] if gated else z)
+    ea = 1.13 * (ez[:, 0::2] if gated else ez) + (2.0 ** -16 * np.abs(a) if act not in ("none", "relu") else 0.0)
+    if gated:
+        up, eu = z[:, 1::2], ez[:, 1::2]
+        a, ea = a * up, ea * np.abs(up) + np.abs(a) * eu + ea * eu + u * np.abs(a * up)
+    if residual is not None:
+        a = a + np.asarray(residual, np.float64)
+        ea = ea + u * np.abs(a)
+    return a, ea + 2.0 ** -8 * (np.abs(a) + ea) + 2.0 ** -130
+
+
+def logits_process_f32(logits_u16, rules, counts, seen, mask, bias_token, bias_value, index_base=0):
+    """One row, the operations in fp32 and in the order that the interface states: bit-exact.  rules: (rep, freq, pres);
+    counts / seen: [table_vocab] or None; mask: truth values [table_vocab] or None; biases in list order."""
+    f = np.float32
+    l = bf16_to_f32(np.asarray(logits_u16)).astype(np.float32).copy()
+    n = l.size
+    rep, freq, pres = (f(v) for v in rules)
+    sl = slice(index_base, index_base + n)
+    with np.errstate(all="ignore"):
+        if counts is not None:
+            k, c = seen[sl], counts[sl]
+            if rep != 1 and rep != 0:
+                l = np.where(k, np.where(l > 0, l / rep, l * rep), l).astype(f)
+            l = np.where(k & (c > 0), (l - freq * c.astype(f)) - pres, l).astype(f)
+        add = {}
+        for t, v in zip(bias_token, bias_value):
+            if index_base <= t < index_base + n:
+                add[t] = f(add.get(t, f(0)) + f(v))
+        for t, v in add.items():
+            l[t - index_base] = l[t - index_base] + v
+    if mask is not None:
+        l = np.where(mask[sl], l, f(-np.inf)).astype(f)
+    return f32_to_bf16(l)
+
+
+def pack_bits(flags):
+    """Truth values [rows, vocab] as 32-bit words, token t in bit t % 32 of word t // 32."""
+    flags = np.asarray(flags, bool)
+    rows, vocab = flags.shape
+    words = (vocab + 31) // 32
+    b = np.zeros((rows, words * 32), np.uint8)
+    b[:, :vocab] = flags
+    return np.packbits(b, axis=1, bitorder="little").view(np.uint32).reshape(rows, words)
+
+
+def token_history(counts, seen, sequences, rebuild):
+    """counts [slots, vocab] int32, seen [slots, vocab] truth values, in place; sequences: (slot, tokens, prompt_len)."""
+    if rebuild:
+        for slot, _, _ in sequences:
+            counts[slot] = 0
+            seen[slot] = False
+    for slot, tokens, prompt in sequences:
+        for j, t in enumerate(tokens):
+            if 0 <= t < counts.shape[1]:
+                seen[slot, t] = True
+                counts[slot, t] += j >= prompt

@@ -1,0 +1,265 @@
+"""mc_sm100_linear_epilogue against the formula in 64 bits.  The bound on each element is the oracle's (accumulation,
+activation, one rounding), derived beside it."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import oracle_np as onp
+
+ACTS = ["none", "relu", "gelu", "gelu_tanh", "silu"]
+
+
+# ---- CPU: the formula, refusals --------------------------------------------------------------------------------------
+def test_formula_known_answers():
+    one = np.ones((1, 1))
+    for act, want in (("none", -2.0), ("relu", 0.0), ("silu", -2.0 / (1 + np.exp(2.0))), ("gelu", -2.0 * 0.022750131948179),
+                      ("gelu_tanh", -0.045402305912)):
+        y, e = onp.linear_epilogue_f64(one, -2.0 * one, act=act)
+        assert abs(y[0, 0] - want) < 1e-9 and e[0, 0] > 0
+    y, _ = onp.linear_epilogue_f64([[1.0], [3.0]], [[2.0]], scale=[1.0, 0.5], bias=[1.0, 1.0], residual=[[10.0]], act="relu", gated=True)
+    assert y[0, 0] == 3.0 * 4.0 + 10.0
+
+
+def test_refusals(pkg):
+    call = pkg.launch_linear_epilogue
+    ok = dict(stream=16)
+    for bad in ((None, 16, 16, 1, 8, 8), (16, None, 16, 1, 8, 8), (16, 16, None, 1, 8, 8), (16, 16, 16, 0, 8, 8), (16, 16, 16, 1, 0, 8),
+                (16, 16, 16, 1, 8, 0), (17, 16, 16, 1, 8, 8), (16, 17, 16, 1, 8, 8), (16, 16, 17, 1, 8, 8)):
+        w, x, y, M, N, K = bad
+        with pytest.raises(pkg.McError) as e:
+            call(w, None, x, y, M, N, K, **ok)
+        assert e.value.status == pkg.MC_E_INVALID_ARGUMENT and "invalid args" in e.value.message
+    for kw in (dict(gated=True, N=7), dict(x_stride=7), dict(y_stride=7), dict(residual=32, residual_stride=7), dict(bias=33), dict(residual=33)):
+        kw = dict(kw)
+        N = kw.pop("N", 8)
+        with pytest.raises(pkg.McError) as e:
+            call(16, None, 16, 48, 2, N, 8, **kw, **ok)
+        assert e.value.status == pkg.MC_E_INVALID_ARGUMENT, kw
+    with pytest.raises(pkg.McError) as e:                          # scales of e4m3 weights are fp32
+        call(16, 18, 16, 16, 1, 8, 8, **ok)
+    assert e.value.status == pkg.MC_E_INVALID_ARGUMENT
+    with pytest.raises(pkg.McError) as e:                          # in place needs one stride
+        call(16, None, 16, 48, 2, 8, 8, residual=48, residual_stride=8, y_stride=16, **ok)
+    assert "one buffer" in e.value.message
+    lib, ep = pkg.lib(), pkg.Epilogue(C.sizeof(pkg.Epilogue))
+    for field, value in (("struct_size", 4), ("activation", 5), ("gated", 2)):
+        bad = pkg.Epilogue.from_buffer_copy(ep)
+        setattr(bad, field, value)
+        assert lib.mc_sm100_linear_epilogue(16, None, 16, 16, 1, 8, 8, C.cast(C.byref(bad), C.c_void_p), None, 0) == pkg.MC_E_INVALID_ARGUMENT
+        assert "invalid epilogue" in pkg.last_error()
+    ep.reserved[1] = 1
+    assert lib.mc_sm100_linear_epilogue(16, None, 16, 16, 1, 8, 8, C.cast(C.byref(ep), C.c_void_p), None, 0) == pkg.MC_E_INVALID_ARGUMENT
+
+
+# ---- GPU -------------------------------------------------------------------------------------------------------------
+def _make(M, N, K, e4m3, bias, residual, gated, seed):
+    n_out = N // 2 if gated else N
+    w = onp.seeded_bf16(seed, (N, K), 0.02 if K > 64 else 0.3)
+    q, sc = onp.make_fp8_weight(w) if e4m3 else (None, None)
+    x = onp.seeded_bf16(seed + 1, (M, K), 1.0)
+    b = onp.seeded_bf16(seed + 2, (N,), 0.5) if bias else None
+    r = onp.seeded_bf16(seed + 3, (M, n_out), 1.0) if residual else None
+    return w, q, sc, x, b, r
+
+
+def _wide(a, pad, fill=0x7FC0):
+    """Rows of `a` in a wider, poisoned matrix."""
+    out = np.full((a.shape[0], a.shape[1] + pad), fill, np.uint16)
+    out[:, :a.shape[1]] = a
+    return out
+
+
+def _run(pkg, M, N, K, e4m3=False, bias=False, residual=False, act="none", gated=False, x_pad=0, y_pad=0, r_pad=0, in_place=False,
+         offset=0, seed=1, pdl=False):
+    import gpu_util as g
+    import torch
+    w, q, sc, x, b, r = _make(M, N, K, e4m3, bias, residual or in_place, gated, seed)
+    n_out = N // 2 if gated else N
+    if in_place:
+        r_pad = y_pad
+
+    def put(a):
+        """`offset` elements behind an aligned address"""
+        t = torch.zeros(a.size + offset, dtype=torch.uint8 if a.dtype == np.uint8 else torch.int16, device="cuda")
+        t[offset:] = g.dev(a).reshape(-1)
+        return t[offset:]
+    dx, dw = put(_wide(x, x_pad)), put(q if e4m3 else w)
+    dy = g.dev(_wide(r, y_pad)) if in_place else g.empty_u16(M, n_out + y_pad)
+    dr = dy if in_place else (g.dev(_wide(r, r_pad)) if residual else None)
+    pkg.launch_linear_epilogue(dw, g.dev(sc) if e4m3 else None, dx, dy, M, N, K, bias=g.dev(b) if bias else None, residual=dr,
+                               activation=act, gated=gated, x_stride=K + x_pad, y_stride=n_out + y_pad, residual_stride=n_out + r_pad, pdl=pdl)
+    g.sync()
+    got = g.host_u16(dy).reshape(M, n_out + y_pad)
+    assert np.all(got[:, n_out:] == 0x7FC0), "columns between the rows were written"
+    f = onp.bf16_to_f32
+    want, bound = onp.linear_epilogue_f64(onp.e4m3_to_f32(q) if e4m3 else f(w), f(x), sc, f(b) if bias else None,
+                                          f(r) if r is not None else None, act, gated)
+    d = np.abs(f(got[:, :n_out]).astype(np.float64) - want)
+    assert np.all(d <= bound), (float(np.max(d / bound)), np.argwhere(~(d <= bound))[:4].tolist())
+    return got
+
+
+SHAPES = [(1, 1, 1), (1, 2, 7), (2, 31, 16), (3, 130, 24), (5, 96, 72), (1, 2304, 2304), (1, 257, 5760), (4, 514, 256), (7, 65, 777), (8, 1000, 512),
+          (16, 3456, 256), (17, 258, 1040), (33, 300, 2304), (64, 128, 64), (65, 128, 64), (100, 66, 96), (127, 384, 320), (128, 256, 128),
+          (129, 514, 136), (200, 1026, 1040), (255, 30, 48), (256, 512, 512), (301, 770, 2304), (513, 258, 72), (1030, 130, 80)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_shapes(pkg, shape, e4m3):
+    M, N, K = shape
+    _run(pkg, M, N, K, e4m3, seed=sum(shape))
+    _run(pkg, M, N, K, e4m3, bias=True, residual=True, act="silu", seed=sum(shape) + 7)
+    if N % 2 == 0:
+        _run(pkg, M, N, K, e4m3, bias=True, residual=True, act="silu", gated=True, seed=sum(shape) + 14)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M", [1, 6, 20, 140])
+def test_activations(pkg, M, act, gated):
+    for e4m3 in (False, True):
+        _run(pkg, M, 196, 208, e4m3, bias=True, act=act, gated=gated, seed=M)
+        _run(pkg, M, 196, 208, e4m3, residual=True, act=act, gated=gated, seed=M + 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 3, 12, 70, 300])
+def test_strides_in_place_and_alignment(pkg, M):
+    for e4m3 in (False, True):
+        _run(pkg, M, 132, 80, e4m3, bias=True, residual=True, x_pad=8, y_pad=4, r_pad=2, seed=M)
+        _run(pkg, M, 132, 80, e4m3, residual=True, x_pad=3, y_pad=5, r_pad=1, seed=M + 1)     # rows of x not 16-byte aligned
+        _run(pkg, M, 131, 80, e4m3, bias=True, in_place=True, seed=M + 2)
+        _run(pkg, M, 132, 96, e4m3, act="gelu", gated=True, in_place=True, y_pad=7, seed=M + 3)
+        _run(pkg, M, 132, 80, e4m3, bias=True, residual=True, offset=1, seed=M + 4)           # w and x at odd addresses
+        _run(pkg, M, 132, 80, e4m3, bias=True, residual=True, seed=M + 5, pdl=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 9, 64, 200])
+def test_a_row_that_is_not_finite_stays_alone(pkg, M):
+    import gpu_util as g
+    for e4m3 in (False, True):
+        w, q, sc, x, _, _ = _make(M, 160, 192, e4m3, False, False, False, M)
+        args = (g.dev(q if e4m3 else w), g.dev(sc) if e4m3 else None)
+        bad = x.copy()
+        bad[M // 2, 5] = 0x7FC0                                                              # NaN
+        if M > 8:
+            bad[2, 7] = 0x7F80                                                               # +infinity
+        ys = []
+        for v in (x, bad):
+            y = g.empty_u16(M, 160)
+            pkg.launch_linear_epilogue(*args, g.dev(v), y, M, 160, 192, activation="relu")
+            g.sync()
+            ys.append(g.host_u16(y))
+        f = [onp.bf16_to_f32(y) for y in ys]
+        assert np.all(np.isnan(f[1][M // 2])), "max(NaN, 0) is NaN"
+        keep = [m for m in range(M) if m != M // 2 and not (M > 8 and m == 2)]
+        assert np.array_equal(ys[0][keep], ys[1][keep])
+        if M > 8:
+            assert np.all((f[1][2] == 0) | (f[1][2] == np.inf) | np.isnan(f[1][2]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 5, 40, 130])
+def test_codes_that_are_not_numbers_count_as_480(pkg, M):
+    """e4m3 codes 0x7F / 0xFF follow the library's decoder."""
+    import gpu_util as g
+    N, K = 96, 64
+    q = np.full((N, K), 0x38, np.uint8)                            # 1.0
+    q[5, 3], q[6, 4] = 0x7F, 0xFF
+    x = np.full((M, K), 0x3F80, np.uint16)
+    sc, y = np.ones(N, np.float32), g.empty_u16(M, N)
+    pkg.launch_linear_epilogue(g.dev(q), g.dev(sc), g.dev(x), y, M, N, K)
+    g.sync()
+    want = np.full((M, N), 64.0)
+    want[:, 5], want[:, 6] = 63.0 + 480.0, 63.0 - 480.0
+    got = onp.bf16_to_f32(g.host_u16(y))
+    assert np.all(np.abs(got - want) <= 2.0 ** -8 * np.abs(want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 5760, 2304), (40, 5760, 2304), (700, 1280, 2304)])
+def test_same_bits_every_time(pkg, shape):
+    a = _run(pkg, *shape, bias=True, residual=True, act="gelu_tanh", seed=3)
+    for _ in range(3):
+        assert np.array_equal(a, _run(pkg, *shape, bias=True, residual=True, act="gelu_tanh", seed=3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("shape", [(2500, 2304, 5760, False), (3001, 11520, 2304, True), (33, 122753, 2304, False), (1, 122753, 2304, False),
+                                   (9000, 200, 4096, False), (600, 3456, 2304, False), (150, 11520, 2304, True)])
+def test_large(pkg, shape, e4m3):
+    """Sizes of real work, the reference product in 64 bits on the GPU."""
+    import torch
+    M, N, K, gated = shape
+    g = torch.Generator(device="cuda")
+    g.manual_seed(M + N)
+    n_out = N // 2 if gated else N
+    w = (torch.randn(N, K, generator=g, device="cuda") * 0.02).bfloat16()
+    x, r = torch.randn(M, K, generator=g, device="cuda").bfloat16(), torch.randn(M, n_out, generator=g, device="cuda").bfloat16()
+    b = (torch.randn(N, generator=g, device="cuda") * 0.5).bfloat16()
+    sc = None
+    if e4m3:
+        sc = w.float().abs().amax(1) / 448.0
+        w = (w.float() / sc[:, None]).to(torch.float8_e4m3fn)
+    y = torch.full((M, n_out), float("nan"), dtype=torch.bfloat16, device="cuda")
+    pkg.launch_linear_epilogue(w.view(torch.uint8) if e4m3 else w, sc, x, y, M, N, K, bias=b, residual=r, activation="silu" if gated else "none", gated=gated)
+    rows = torch.randperm(M, generator=g, device="cuda")[:256]
+    wd = w.double() * sc.double()[:, None] if e4m3 else w.double()
+    z = x[rows].double() @ wd.T + b.double()
+    ez = 2.0 ** -23 * ((K + 3) * (x[rows].double().abs() @ wd.abs().T + b.double().abs()))
+    if gated:
+        a, u = z[:, 0::2] * torch.sigmoid(z[:, 0::2]), z[:, 1::2]
+        ea = 1.13 * ez[:, 0::2] + 2.0 ** -16 * a.abs()
+        z, ez = a * u, ea * u.abs() + a.abs() * ez[:, 1::2] + ea * ez[:, 1::2]
+    z = z + r[rows].double()
+    ez = ez + 2.0 ** -22 * z.abs()
+    bound = ez + 2.0 ** -8 * (z.abs() + ez)
+    assert bool(((y[rows].double() - z).abs() <= bound).all())
+    assert bool(torch.isfinite(y).all())
+    # typical error, far below the worst case: one rounding of a random value is off by 2^-9 / sqrt(3) of it on average
+    rel = float((y[rows].double() - z).norm() / z.norm())
+    assert rel <= 2.0 ** -8, rel
+
+
+@pytest.mark.gpu
+def test_streams_and_graph(pkg):
+    """Two calls at once on two streams, and both captured into one graph and replayed with other inputs."""
+    import torch
+    M, N, K = 200, 640, 512
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    w = [(torch.randn(N, K, generator=g, device="cuda") * 0.05).bfloat16() for _ in range(2)]
+    x = [torch.randn(m, K, generator=g, device="cuda").bfloat16() for m in (M, 3)]
+    y = [torch.empty(m, N, dtype=torch.bfloat16, device="cuda") for m in (M, 3)]
+    ref = [torch.empty_like(t) for t in y]
+    for i in range(2):
+        pkg.launch_linear_epilogue(w[i], None, x[i], ref[i], x[i].shape[0], N, K, activation="silu")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+
+    def both():
+        side.wait_stream(torch.cuda.current_stream())
+        pkg.launch_linear_epilogue(w[0], None, x[0], y[0], M, N, K, activation="silu")
+        with torch.cuda.stream(side):
+            pkg.launch_linear_epilogue(w[1], None, x[1], y[1], 3, N, K, activation="silu")
+        torch.cuda.current_stream().wait_stream(side)
+    both()
+    torch.cuda.synchronize()
+    assert torch.equal(y[0], ref[0]) and torch.equal(y[1], ref[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        both()
+    for t in x:
+        t.neg_()
+    for i in range(2):
+        pkg.launch_linear_epilogue(w[i], None, x[i], ref[i], x[i].shape[0], N, K, activation="silu")
+        y[i].zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y[0], ref[0]) and torch.equal(y[1], ref[1])
