@@ -67,7 +67,7 @@ inline mc_status_t launch_fast_rows(const RowsArgs& a, cudaStream_t stream, bool
 }
 
 // SwiGLU epilogue over interleaved (gate, up) rows: a warp owns a pair
-template <int WB, int PRO>
+template <int WB, int PRO, int EPI = EPI_SWIGLU>
 inline mc_status_t launch_fast_pairs(const RowsArgs& a, cudaStream_t stream, bool pdl) {
     const uint32_t per_lane = (a.K * WB / 16u + 31u) / 32u;
     if constexpr (WB == 2) {
@@ -78,27 +78,30 @@ inline mc_status_t launch_fast_pairs(const RowsArgs& a, cudaStream_t stream, boo
             const uint32_t sms = (uint32_t)sm_count();
             const uint32_t ppc = (a.N / 2u + sms - 1u) / sms, rounds = (ppc + 15u) / 16u;
             const uint32_t warps = rounds == 0u ? 16u : (ppc + rounds - 1u) / rounds + 1u;
-            if (rounds > 1u && warps <= 12u) return launch_fast_one<2, 2, 9, false, false, PRO, EPI_SWIGLU, 384>(a, stream, pdl);
-            if (rounds > 1u && warps <= 14u) return launch_fast_one<2, 2, 9, false, false, PRO, EPI_SWIGLU, 448>(a, stream, pdl);
-            return launch_fast_one<2, 2, 9, false, false, PRO, EPI_SWIGLU, 512>(a, stream, pdl);
+            if (rounds > 1u && warps <= 12u) return launch_fast_one<2, 2, 9, false, false, PRO, EPI, 384>(a, stream, pdl);
+            if (rounds > 1u && warps <= 14u) return launch_fast_one<2, 2, 9, false, false, PRO, EPI, 448>(a, stream, pdl);
+            return launch_fast_one<2, 2, 9, false, false, PRO, EPI, 512>(a, stream, pdl);
         }
-        return launch_fast_one<2, 2, 12, false, false, PRO, EPI_SWIGLU, 512>(a, stream, pdl);
+        return launch_fast_one<2, 2, 12, false, false, PRO, EPI, 512>(a, stream, pdl);
     } else {
         if (per_lane <= 5) {
             // same even-rounds rule with up to 24 warps: gate_up runs as two rounds of 20 warps
             const uint32_t sms = (uint32_t)sm_count();
             const uint32_t ppc = (a.N / 2u + sms - 1u) / sms, rounds = (ppc + 23u) / 24u;
             const uint32_t warps = rounds == 0u ? 24u : (ppc + rounds - 1u) / rounds;
-            if (warps <= 20u) return launch_fast_one<1, 2, 5, false, false, PRO, EPI_SWIGLU, 640>(a, stream, pdl);
-            return launch_fast_one<1, 2, 5, false, false, PRO, EPI_SWIGLU, 768>(a, stream, pdl);
+            if (warps <= 20u) return launch_fast_one<1, 2, 5, false, false, PRO, EPI, 640>(a, stream, pdl);
+            return launch_fast_one<1, 2, 5, false, false, PRO, EPI, 768>(a, stream, pdl);
         }
-        return launch_fast_one<1, 2, 6, false, false, PRO, EPI_SWIGLU, 512>(a, stream, pdl);
+        return launch_fast_one<1, 2, 6, false, false, PRO, EPI, 512>(a, stream, pdl);
     }
 }
 
 // Entry of one translation unit (fast_inst_w*.cu).
 template <int WB>
 mc_status_t launch_fast(int pro, int epi, const RowsArgs& a, cudaStream_t stream, bool pdl);
+
+// M = 1 with the fused epilogue (fast_inst_fused.cu): the same tile shapes.
+mc_status_t launch_fast_fused(int wb, bool gated, const RowsArgs& a, cudaStream_t stream, bool pdl);
 
 #define MCL_DEFINE_LAUNCH_FAST(WBV)                                                                  \
     template <>                                                                                      \

@@ -237,6 +237,12 @@ __global__ void __launch_bounds__(THREADS, MINB) gemv_fast_kernel(const RowsArgs
     float scA[R], scB[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) { scA[r] = 1.f; scB[r] = 1.f; }
+    // fused epilogue: the rows' biases travel the same way (no second register buffer in its tile shapes); the group's
+    // residual, which the previous kernel may write, is asked for after the wait and ahead of the arithmetic
+    constexpr bool FUSED = EPI == EPI_FUSED || EPI == EPI_FUSED_GATED;
+    static_assert(!(FUSED && DB), "one bias buffer");
+    constexpr int OUTS = EPI == EPI_FUSED_GATED ? 1 : R;
+    uint16_t bias_b[FUSED ? R : 1], res_b[FUSED ? OUTS : 1];
     auto issue = [&](auto& raw, float (&sc)[R], uint32_t g, uint32_t i0) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -244,6 +250,9 @@ __global__ void __launch_bounds__(THREADS, MINB) gemv_fast_kernel(const RowsArgs
             const uint8_t* wr = wbase + (size_t)row * row_bytes;
             if constexpr (WB == 1) {
                 if (i0 == 0u && row < a.N) sc[r] = __ldg(a.scale + row);
+            }
+            if constexpr (FUSED) {
+                if (i0 == 0u) bias_b[r] = (a.ep.bias != nullptr && row < a.N) ? __ldg(a.ep.bias + row) : (uint16_t)0;
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -352,7 +361,7 @@ __global__ void __launch_bounds__(THREADS, MINB) gemv_fast_kernel(const RowsArgs
     int32_t best_i = INT32_MAX;
     // where the outputs go: y, or (sharded) slot `rank` of every rank's gathered vector as tagged
     // words, one destination rank per lane; logits of a sharded lm_head stay local
-    const bool push = (EPI != EPI_ARGMAX) && a.sh.out_slot != 0u;
+    const bool push = (EPI != EPI_ARGMAX) && !FUSED && a.sh.out_slot != 0u;
     const uint32_t ndst = push ? a.sh.world : 1u;
     uint32_t* wdst = reinterpret_cast<uint32_t*>(a.sh.out_peer[lane & 7u]) + (size_t)a.sh.rank * a.sh.out_slot;
     const uint32_t out_tag = push ? shard_tag(a.sh, a.sh.out_seq_mul, a.sh.out_seq_add) << 16 : 0u;
@@ -430,7 +439,19 @@ __global__ void __launch_bounds__(THREADS, MINB) gemv_fast_kernel(const RowsArgs
             }
             tot[r] = s;
         }
-        if (lane < ndst) {      // the sums are the same in every lane
+        if constexpr (FUSED) {
+            if (lane == 0u) {
+                auto bf = [](uint16_t b) { return __uint_as_float((uint32_t)b << 16); };
+#pragma unroll
+                for (int o = 0; o < OUTS; ++o) {
+                    const uint32_t out = g * OUTS + o;
+                    float v;
+                    if constexpr (EPI == EPI_FUSED_GATED) v = epi_act(tot[0] + bf(bias_b[0]), a.ep.act) * (tot[R - 1] + bf(bias_b[FUSED ? R - 1 : 0]));
+                    else v = epi_act(tot[o] + bf(bias_b[FUSED ? o : 0]), a.ep.act);
+                    if (out < (EPI == EPI_FUSED_GATED ? a.N / 2u : a.N)) a.y[out] = f32_to_bf16_bits(v + bf(res_b[FUSED ? o : 0]));
+                }
+            }
+        } else if (lane < ndst) {      // the sums are the same in every lane
             if constexpr (EPI == EPI_SWIGLU) {
                 static_assert(EPI != EPI_SWIGLU || R == 2, "SwiGLU epilogue works on row pairs");
                 const uint32_t row = g * R;
@@ -489,6 +510,14 @@ __global__ void __launch_bounds__(THREADS, MINB) gemv_fast_kernel(const RowsArgs
         for (; g < groups; g += gstep) {
             float2 acc_a[R], acc_b[R];
             zero(acc_a, acc_b);
+            if constexpr (FUSED) {
+#pragma unroll
+                for (int o = 0; o < OUTS; ++o) {
+                    const uint32_t out = g * OUTS + o;
+                    // -0 leaves every sum as it is
+                    res_b[o] = (a.ep.res != nullptr && out < (EPI == EPI_FUSED_GATED ? a.N / 2u : a.N)) ? a.ep.res[out] : (uint16_t)0x8000u;
+                }
+            }
             for (uint32_t i0 = 0; i0 < per_lane; i0 += U) {
                 if (!first) issue(rawA, scA, g, i0);
                 if (!skip_mac) mac_batch(rawA, first, i0, acc_a, acc_b);

@@ -24,11 +24,12 @@
 #pragma once
 
 #include "common.cuh"
+#include "linear_epilogue.cuh"
 
 namespace mcl {
 
 enum : int { PRO_NONE = 0, PRO_RESNORM = 1, PRO_SWIGLU = 2 };
-enum : int { EPI_STORE = 0, EPI_SWIGLU = 1, EPI_ARGMAX = 2, EPI_PARTIAL = 3 };
+enum : int { EPI_STORE = 0, EPI_SWIGLU = 1, EPI_ARGMAX = 2, EPI_PARTIAL = 3, EPI_FUSED = 4, EPI_FUSED_GATED = 5 };
 enum : int { MATH_CVT = 0, MATH_MIXED = 1 };
 
 // Candidates per logits row in the argmax stage buffer ([kArgmaxCands][M]).
@@ -59,6 +60,8 @@ struct RowsArgs {
     // L2 prefetch of the next kernel's weights (all zero = off); gemv_fast_kernel also takes the
     // eviction policy of its own loads from here
     PrefetchArgs pf;
+    // EPI_FUSED, EPI_FUSED_GATED (gemv_fast_kernel only): bias, activation, residual; y and scale are the fields above
+    EpiArgs ep;
 };
 
 // ---- per-unit multiply-accumulate -------------------------------------------------

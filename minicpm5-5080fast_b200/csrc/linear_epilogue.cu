@@ -1,6 +1,9 @@
 // linear_epilogue.cu -- mc_sm100_linear_epilogue: checks, choice of a kernel, and the kernel that takes every shape.
 #include "linear_epilogue.cuh"
 
+#include "fast_dispatch.cuh"
+#include "skinny_gemm.cuh"
+
 namespace mcl {
 
 namespace {
@@ -132,5 +135,17 @@ extern "C" mc_status_t mc_sm100_linear_epilogue(const void* d_w, const float* d_
         return MC_E_INVALID_ARGUMENT;
     }
     const EpiArgs e{d_scale, d.d_bias, d.d_residual, d_y, ys, rs, d.activation, d.gated};
-    return linear_any(wb, d_w, d_x, xs, M, N, K, e, (cudaStream_t)stream, pdl != 0);
+    const cudaStream_t st = (cudaStream_t)stream;
+    // rows that a 16-byte unit divides, at aligned addresses: the kernels that stream
+    const bool unit = aligned16(d_w) && aligned16(d_x) && ((uint64_t)K * (uint32_t)wb) % 16u == 0u;
+    if (M == 1u && unit && (uint64_t)K * (wb == 1 ? 4u : 2u) <= 200u * 1024u) {       // the activation in shared memory
+        RowsArgs a{};
+        a.w = d_w; a.scale = d_scale; a.x = d_x; a.y = d_y; a.N = N; a.K = K; a.y_stride = ys; a.kseg = K; a.ep = e;
+        const NextWeights nw = take_next_weights();
+        a.pf.ptr = static_cast<const uint8_t*>(nw.ptr); a.pf.bytes = nw.bytes;
+        return launch_fast_fused(wb, d.gated != 0u, a, st, pdl != 0);
+    }
+    const bool tma = unit && (xs & 7u) == 0u;
+    if (M <= 64u && tma) return skinny_gemm_fused(wb == 2 ? SKINNY_W_BF16 : SKINNY_W_E4M3, d_w, d_x, xs, M, N, K, e, st, pdl != 0);
+    return linear_any(wb, d_w, d_x, xs, M, N, K, e, st, pdl != 0);
 }

@@ -133,6 +133,7 @@ struct SkinnyArgs {
     uint32_t swiglu;        // rows 2j / 2j+1 are gate_j / up_j: store silu(g)*u
     uint32_t op_stages, raw_stages;  // ring depths (<= 8), chosen by the launcher from the grid size
     int32_t* status;        // optional device word set to 1 when a bounded wait ran out (the caller's failure word)
+    EpiArgs ep;             // EXT: bias, activation, gate, residual, strides (scale and y are the fields above)
     PeerOut out;            // sharded step: the result goes to every rank's activation buffer as tagged words (world = 0: to y)
     PrefetchArgs pf;        // L2 prefetch of the next kernel's weights (all zero = off)
 };
@@ -152,8 +153,8 @@ template <int MODE, int NPAD> struct Ring {
 
 }  // namespace
 
-// MODE: SKINNY_W_BF16 / SKINNY_W_E4M3 / SKINNY_W8A8.  NPAD: MMA N (16, 32 or 64).
-template <int MODE, int NPAD>
+// MODE: SKINNY_W_BF16 / SKINNY_W_E4M3 / SKINNY_W8A8.  NPAD: MMA N (16, 32 or 64).  EXT: fused epilogue.
+template <int MODE, int NPAD, bool EXT>
 __global__ void __launch_bounds__(kThreads, 2)
 skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const SkinnyArgs a) {
     using G = Ring<MODE, NPAD>;
@@ -412,7 +413,28 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             const float ub = __uint_as_float((uint32_t)f32_to_bf16_bits(up) << 16);
             return f32_to_bf16_bits(swiglu_f32(gb, ub));
         };
-        if (a.out.world != 0u) {
+        if constexpr (EXT) {
+            pdl_wait();   // the residual may be the previous kernel's: every thread that reads it waits for itself
+            // one output per thread and turn, features fastest; the slice is a power of two wide
+            const uint32_t gate = a.ep.gated, outs = per_n >> gate, sh = 31u - (uint32_t)__clz((int)outs);
+            const uint32_t obase = nbase >> gate, olimit = a.N >> gate;
+            auto z_of = [&](uint32_t n_rel, uint32_t m) {
+                float z = partial_sum(n_rel, m);
+                const uint32_t n = nbase + n_rel;
+                if (a.w_scale != nullptr) z *= a.w_scale[n];
+                if (a.ep.bias != nullptr) z += __uint_as_float((uint32_t)a.ep.bias[n] << 16);
+                return z;
+            };
+            for (uint32_t idx = tid; idx < outs * a.M; idx += kThreads) {
+                const uint32_t m = idx >> sh, j_rel = idx & (outs - 1u), j = obase + j_rel;
+                if (j < olimit && !failed) {
+                    float r = -0.f;
+                    if (a.ep.res != nullptr) r = __uint_as_float((uint32_t)a.ep.res[(size_t)m * a.ep.res_stride + j] << 16);
+                    const float v = gate ? epi_act(z_of(2u * j_rel, m), a.ep.act) * z_of(2u * j_rel + 1u, m) : epi_act(z_of(j_rel, m), a.ep.act);
+                    a.y[(size_t)m * a.ep.y_stride + j] = f32_to_bf16_bits(v + r);
+                }
+            }
+        } else if (a.out.world != 0u) {
             // pairs of adjacent outputs (the slice holds an even number of them, starting at an even column)
             const uint32_t outs = a.swiglu ? per_n / 2u : per_n, obase = a.swiglu ? nbase >> 1 : nbase, olimit = a.swiglu ? a.N / 2u : a.N;
             for (uint32_t idx = tid; idx < (outs / 2u) * a.M; idx += kThreads) {
@@ -550,10 +572,10 @@ mc_status_t make_map(CUtensorMap* map, const void* ptr, uint32_t rows, uint32_t 
     return MC_OK;
 }
 
-template <int MODE, int NPAD>
+template <int MODE, int NPAD, bool EXT>
 mc_status_t launch_one(const void* w, const void* x, uint32_t x_pitch, const SkinnyArgs& a, uint32_t grid, cudaStream_t stream, bool pdl) {
     using G = Ring<MODE, NPAD>;
-    auto kern = skinny_gemm_kernel<MODE, NPAD>;
+    auto kern = skinny_gemm_kernel<MODE, NPAD, EXT>;
     constexpr size_t smem_max = 112u * 1024u;
     static SmemOptIn optin;
     const cudaError_t ae = optin.ensure(kern, smem_max);
@@ -594,11 +616,11 @@ mc_status_t launch_one(const void* w, const void* x, uint32_t x_pitch, const Ski
     return MC_OK;
 }
 
-template <int MODE>
+template <int MODE, bool EXT>
 mc_status_t launch_mode(const void* w, const void* x, uint32_t x_pitch, const SkinnyArgs& a, uint32_t grid, cudaStream_t stream, bool pdl) {
-    if (a.M <= 16) return launch_one<MODE, 16>(w, x, x_pitch, a, grid, stream, pdl);
-    if (a.M <= 32) return launch_one<MODE, 32>(w, x, x_pitch, a, grid, stream, pdl);
-    return launch_one<MODE, 64>(w, x, x_pitch, a, grid, stream, pdl);
+    if (a.M <= 16) return launch_one<MODE, 16, EXT>(w, x, x_pitch, a, grid, stream, pdl);
+    if (a.M <= 32) return launch_one<MODE, 32, EXT>(w, x, x_pitch, a, grid, stream, pdl);
+    return launch_one<MODE, 64, EXT>(w, x, x_pitch, a, grid, stream, pdl);
 }
 
 }  // namespace
@@ -611,23 +633,13 @@ bool skinny_shape_ok(uint32_t N, uint32_t K, int wb) {
 // Split-K partials travel through distributed shared memory: no global workspace.
 size_t skinny_workspace_bytes(uint32_t, uint32_t, uint32_t) { return 0; }
 
-mc_status_t skinny_gemm(int mode, const void* w, const float* w_scale, const uint16_t* x, const float* x_scale,
-                        uint16_t* y, uint32_t M, uint32_t N, uint32_t K, bool swiglu, cudaStream_t stream, bool pdl,
-                        uint32_t x_pitch, const PeerOut* out) {
-    if (x_pitch == 0u) x_pitch = K;
-    const uint32_t x_elem = mode == SKINNY_W8A8 ? 1u : 2u;
-    if (M == 0 || M > 64 || !aligned16(w) || !aligned16(x) || (swiglu && (N & 1u)) || x_pitch < K || ((x_pitch * x_elem) & 15u) != 0u) {
-        set_error("skinny_gemm: invalid args (M=%u N=%u K=%u x_pitch=%u)", M, N, K, x_pitch);
-        return MC_E_INVALID_ARGUMENT;
-    }
+// What a call needs besides its operands: K slices, ring depths, the hints of this thread.
+static uint32_t plan_args(int mode, uint32_t M, uint32_t N, uint32_t K, SkinnyArgs& a) {
     const Plan p = make_plan(N, K, mode == SKINNY_W8A8 ? 128u : 64u);
-    SkinnyArgs a{};
-    a.w_scale = w_scale; a.x_scale = x_scale; a.y = y;
-    a.M = M; a.N = N; a.K = K; a.splits = p.splits; a.swiglu = swiglu ? 1u : 0u;
+    a.M = M; a.N = N; a.K = K; a.splits = p.splits;
     const uint32_t grid = p.tiles * p.splits;
     a.pf = make_prefetch_args(take_next_weights(), grid);
     a.status = wait_status_sink();
-    if (out != nullptr) a.out = *out;
     // Ring depth: as many stages as fit in ~108 KB, i.e. half an SM's shared memory.  Measured
     // (down_proj 2304 x 5760, chain of calls): with 150 or 200 KB, one CTA per SM, a call takes 14.7 us
     // against 8.8 us at M = 8 and 19.1 against 12.9 us at M = 64, because the next kernel's CTA can then
@@ -647,9 +659,34 @@ mc_status_t skinny_gemm(int mode, const void* w, const float* w_scale, const uin
         if (a.op_stages < 2u) a.op_stages = 2u;
         a.raw_stages = 1u;
     }
-    if (mode == SKINNY_W_BF16) return launch_mode<SKINNY_W_BF16>(w, x, x_pitch, a, grid, stream, pdl);
-    if (mode == SKINNY_W_E4M3) return launch_mode<SKINNY_W_E4M3>(w, x, x_pitch, a, grid, stream, pdl);
-    return launch_mode<SKINNY_W8A8>(w, x, x_pitch, a, grid, stream, pdl);
+    return grid;
+}
+
+mc_status_t skinny_gemm(int mode, const void* w, const float* w_scale, const uint16_t* x, const float* x_scale,
+                        uint16_t* y, uint32_t M, uint32_t N, uint32_t K, bool swiglu, cudaStream_t stream, bool pdl,
+                        uint32_t x_pitch, const PeerOut* out) {
+    if (x_pitch == 0u) x_pitch = K;
+    const uint32_t x_elem = mode == SKINNY_W8A8 ? 1u : 2u;
+    if (M == 0 || M > 64 || !aligned16(w) || !aligned16(x) || (swiglu && (N & 1u)) || x_pitch < K || ((x_pitch * x_elem) & 15u) != 0u) {
+        set_error("skinny_gemm: invalid args (M=%u N=%u K=%u x_pitch=%u)", M, N, K, x_pitch);
+        return MC_E_INVALID_ARGUMENT;
+    }
+    SkinnyArgs a{};
+    a.w_scale = w_scale; a.x_scale = x_scale; a.y = y; a.swiglu = swiglu ? 1u : 0u;
+    if (out != nullptr) a.out = *out;
+    const uint32_t grid = plan_args(mode, M, N, K, a);
+    if (mode == SKINNY_W_BF16) return launch_mode<SKINNY_W_BF16, false>(w, x, x_pitch, a, grid, stream, pdl);
+    if (mode == SKINNY_W_E4M3) return launch_mode<SKINNY_W_E4M3, false>(w, x, x_pitch, a, grid, stream, pdl);
+    return launch_mode<SKINNY_W8A8, false>(w, x, x_pitch, a, grid, stream, pdl);
+}
+
+mc_status_t skinny_gemm_fused(int mode, const void* w, const uint16_t* x, uint32_t x_pitch, uint32_t M, uint32_t N, uint32_t K,
+                              const EpiArgs& ep, cudaStream_t stream, bool pdl) {
+    SkinnyArgs a{};
+    a.w_scale = ep.scale; a.y = ep.y; a.ep = ep;
+    const uint32_t grid = plan_args(mode, M, N, K, a);
+    if (mode == SKINNY_W_BF16) return launch_mode<SKINNY_W_BF16, true>(w, x, x_pitch, a, grid, stream, pdl);
+    return launch_mode<SKINNY_W_E4M3, true>(w, x, x_pitch, a, grid, stream, pdl);
 }
 
 // 1 when a bounded wait of the tensor-core kernel ran out since the last call (and clears it).

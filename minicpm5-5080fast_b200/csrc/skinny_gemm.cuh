@@ -2,6 +2,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "linear_epilogue.cuh"
 
 namespace mcl {
 
@@ -27,6 +28,10 @@ mc_status_t skinny_gemm(int mode, const void* w, const float* w_scale, const uin
                         const float* x_scale, uint16_t* y, uint32_t M, uint32_t N, uint32_t K,
                         bool swiglu, cudaStream_t stream, bool pdl, uint32_t x_pitch = 0,
                         const PeerOut* out = nullptr);
+
+// The same product for SKINNY_W_BF16 / SKINNY_W_E4M3 with the fused epilogue behind the finished sums (any parity of M, N; 1 <= M <= 64).
+mc_status_t skinny_gemm_fused(int mode, const void* w, const uint16_t* x, uint32_t x_pitch, uint32_t M, uint32_t N, uint32_t K,
+                              const EpiArgs& ep, cudaStream_t stream, bool pdl);
 
 // 1 when a bounded wait inside the tensor-core kernel ran out since the last query (clears it), -1 on a CUDA error.
 int skinny_take_error();
