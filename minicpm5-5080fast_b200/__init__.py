@@ -169,10 +169,18 @@ def _p(t) -> int | None:
     return int(t) if isinstance(t, int) else t.data_ptr()
 
 
+_current_stream = None
+
+
 def _stream(stream) -> int | None:
+    """The handle itself: a torch.cuda.Stream object per call costs 3 us of host time, more than some kernels take."""
     if stream is None:
-        import torch
-        stream = torch.cuda.current_stream()
+        global _current_stream
+        if _current_stream is None:
+            import torch
+            torch.cuda.current_stream()                       # brings CUDA up, or says why not
+            _current_stream = lambda: torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())  # noqa: E731
+        return _current_stream() or None
     s = stream if isinstance(stream, int) else stream.cuda_stream
     return s or None
 
@@ -328,11 +336,14 @@ class Epilogue(C.Structure):
                 ("residual_stride", _u32), ("d_bias", _vp), ("d_residual", _vp), ("reserved", _u32 * 2)]
 
 
+_EPILOGUE_SIZE = C.sizeof(Epilogue)
+
+
 def launch_linear_epilogue(w, scale, x, y, M, N, K, bias=None, residual=None, activation="none", gated=False, x_stride=0,
                            y_stride=0, residual_stride=0, stream=None, pdl=False):
     """y = act(x W^T * scale + bias) [* up] + residual for any M; activation: a key of ACTIVATIONS."""
-    e = Epilogue(C.sizeof(Epilogue), ACTIVATIONS[activation], int(gated), x_stride, y_stride, residual_stride, _p(bias), _p(residual))
-    _check(lib().mc_sm100_linear_epilogue(_p(w), _p(scale), _p(x), _p(y), M, N, K, C.cast(C.byref(e), _vp), _stream(stream), int(pdl)))
+    e = Epilogue(_EPILOGUE_SIZE, ACTIVATIONS[activation], gated, x_stride, y_stride, residual_stride, _p(bias), _p(residual))
+    _check((_lib or lib()).mc_sm100_linear_epilogue(_p(w), _p(scale), _p(x), _p(y), M, N, K, C.byref(e), _stream(stream), pdl))
 
 
 class LogitsTables(C.Structure):
@@ -340,18 +351,21 @@ class LogitsTables(C.Structure):
                 ("d_counts", _vp), ("d_seen", _vp), ("d_mask", _vp), ("d_bias_token", _vp), ("d_bias_value", _vp), ("d_status", _vp)]
 
 
+_TABLES_SIZE = C.sizeof(LogitsTables)
+
+
 def logits_tables(table_vocab, counts=None, seen=None, masks=None, bias_token=None, bias_value=None, status=None) -> LogitsTables:
     """Tables of logits_process out of device tensors (their sizes give the numbers of rows); the caller keeps the tensors."""
     words = (table_vocab + 31) // 32
-    return LogitsTables(C.sizeof(LogitsTables), table_vocab, counts.numel() // table_vocab if counts is not None else 0,
+    return LogitsTables(_TABLES_SIZE, table_vocab, counts.numel() // table_vocab if counts is not None else 0,
                         masks.numel() // words if masks is not None else 0, bias_token.numel() if bias_token is not None else 0, 0,
                         _p(counts), _p(seen), _p(masks), _p(bias_token), _p(bias_value), _p(status))
 
 
 def logits_process(logits, out, n_rows, vocab, row_stride, out_stride, cfg, tables, index_base=0, stream=None, pdl=False):
     """cfg: device tensor of n_rows x 8 words (rep, freq, pres penalty as f32 bits, history slot, mask row, bias begin, bias count, 0)."""
-    _check(lib().mc_sm100_logits_process(_p(logits), _p(out), n_rows, vocab, row_stride, out_stride, index_base, _p(cfg),
-                                         C.cast(C.byref(tables), _vp), _stream(stream), int(pdl)))
+    _check((_lib or lib()).mc_sm100_logits_process(_p(logits), _p(out), n_rows, vocab, row_stride, out_stride, index_base, _p(cfg),
+                                                   C.byref(tables), _stream(stream), pdl))
 
 
 def token_history(counts, seen, tokens, n_seqs, table_vocab, offsets=None, prompt_len=None, slots=None, n_tokens=None, n_slots=None,
@@ -360,8 +374,8 @@ def token_history(counts, seen, tokens, n_seqs, table_vocab, offsets=None, promp
         n_tokens = tokens.numel()
     if n_slots is None:
         n_slots = counts.numel() // table_vocab
-    _check(lib().mc_sm100_token_history(_p(counts), _p(seen), n_slots, table_vocab, _p(tokens), n_tokens, _p(offsets), _p(prompt_len),
-                                        _p(slots), n_seqs, int(rebuild), _p(status), _stream(stream), int(pdl)))
+    _check((_lib or lib()).mc_sm100_token_history(_p(counts), _p(seen), n_slots, table_vocab, _p(tokens), n_tokens, _p(offsets), _p(prompt_len),
+                                                  _p(slots), n_seqs, rebuild, _p(status), _stream(stream), pdl))
 
 
 def linear_host(kind, w, scale, h_x, h_y, M, N, K, x_stage, y_stage, workspace=None, ws_size=0, stream=None):
