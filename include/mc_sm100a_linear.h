@@ -709,6 +709,14 @@ MC_SM100_API void mc_sm100_debug_mma_rows_plan(uint32_t N, uint32_t sms, uint32_
 MC_SM100_API void mc_sm100_debug_chain_plan(int32_t fp8, uint32_t hidden, uint32_t inter, uint32_t* slot_bytes, uint32_t* rows_hidden,
                                             uint32_t* rows_gate_up, uint32_t* rows_down);
 
+/* How mc_sm100_linear_epilogue cuts a call of more than 64 rows that takes the tiled tensor-core kernel (host logic alone):
+ * CTAs per tile (1 or 2, 128 rows each), features per tile, K slices.  set_tile_plan: A/B and test hook (process-wide),
+ * every such call takes this plan (cg = 0: the rule again; as many K slices as fit the shape).  No plan changes a result
+ * beyond the order of its sums. */
+MC_SM100_API void mc_sm100_debug_tile_plan(int32_t bytes_per_weight, uint32_t M, uint32_t N, uint32_t K, uint32_t sms, uint32_t* cg,
+                                           uint32_t* bn, uint32_t* splits);
+MC_SM100_API void mc_sm100_debug_set_tile_plan(uint32_t cg, uint32_t bn, uint32_t splits);
+
 /* Host-only self-test of the per-device bookkeeping behind the kernels' shared-memory opt-in (one entry per
  * device, raised once per device and size, safe under racing host threads); makes no CUDA call.  0 = passed. */
 MC_SM100_API int32_t mc_sm100_debug_optin_selftest(void);
@@ -720,7 +728,7 @@ MC_SM100_API int32_t mc_sm100_debug_optin_selftest(void);
  * linear.  Both give the same bits.  Takes effect for steps issued (and graphs captured) afterwards. */
 MC_SM100_API void mc_sm100_debug_set_chain(int32_t on);
 
-/* Every wait inside the tensor-core kernel is bounded; a wait that runs out
+/* Every wait inside the tensor-core kernels is bounded; a wait that runs out
  * makes the kernel skip its stores and raise a device-side flag.  This reads
  * the flag (synchronising copy) and clears it: 0 = no wait ever ran out. */
 MC_SM100_API int32_t mc_sm100_debug_take_error(void);

@@ -121,6 +121,8 @@ SIGNATURES = {
     "mc_sm100_debug_optin_selftest": (_i32, []),
     "mc_sm100_debug_set_mma_rows": (None, [_i32]),
     "mc_sm100_debug_mma_rows_plan": (None, [_u32, _u32, _vp, _vp, _vp]),
+    "mc_sm100_debug_tile_plan": (None, [_i32, _u32, _u32, _u32, _u32, _vp, _vp, _vp]),
+    "mc_sm100_debug_set_tile_plan": (None, [_u32, _u32, _u32]),
     "mc_sm100_debug_chain_plan": (None, [_i32, _u32, _u32, _vp, _vp, _vp, _vp]),
     "mc_sm100_debug_set_math": (None, [_i32, _i32]),
     "mc_sm100_debug_take_error": (_i32, []),
@@ -400,6 +402,18 @@ def debug_mma_rows_plan(n: int, sms: int = 148):
     a, b, c = _u32(0), _u32(0), _u32(0)
     lib().mc_sm100_debug_mma_rows_plan(n, sms, C.byref(a), C.byref(b), C.byref(c))
     return a.value, b.value, c.value
+
+
+def debug_tile_plan(bytes_per_weight: int, M: int, N: int, K: int, sms: int = 148):
+    """(CTAs per tile, features per tile, K slices) of a fused linear of more than 64 rows -- host logic only."""
+    v = [_u32(0) for _ in range(3)]
+    lib().mc_sm100_debug_tile_plan(bytes_per_weight, M, N, K, sms, *[C.byref(x) for x in v])
+    return tuple(x.value for x in v)
+
+
+def debug_set_tile_plan(cg: int = 0, bn: int = 0, splits: int = 1) -> None:
+    """Fused linears of more than 64 rows take this plan (cg = 0: the library's rule)."""
+    lib().mc_sm100_debug_set_tile_plan(cg, bn, splits)
 
 
 def debug_chain_plan(fp8: bool, hidden: int, inter: int):

@@ -10,6 +10,7 @@
 #include "rows_dispatch.cuh"
 #include "decode_chain.cuh"
 #include "gemm_mma_rows.cuh"
+#include "linear_tile.cuh"
 #include "skinny_gemm.cuh"
 
 namespace mcl {
@@ -441,7 +442,10 @@ void mc_sm100_debug_set_math(int32_t bf16_math, int32_t fp8_math) {
     if (fp8_math >= 0 && fp8_math <= 2) g_math[1].store(fp8_math);
 }
 
-int32_t mc_sm100_debug_take_error(void) { return skinny_take_error(); }
+int32_t mc_sm100_debug_take_error(void) {
+    const int a = skinny_take_error(), b = linear_tile_take_error();
+    return a < 0 || b < 0 ? -1 : a | b;
+}
 
 void mc_sm100_debug_set_mma_rows(int32_t max_m) { mma_rows_set_max_m(max_m); }
 

@@ -2,6 +2,7 @@
 #include "linear_epilogue.cuh"
 
 #include "fast_dispatch.cuh"
+#include "linear_tile.cuh"
 #include "skinny_gemm.cuh"
 
 namespace mcl {
@@ -147,5 +148,16 @@ extern "C" mc_status_t mc_sm100_linear_epilogue(const void* d_w, const float* d_
     }
     const bool tma = unit && (xs & 7u) == 0u;
     if (M <= 64u && tma) return skinny_gemm_fused(wb == 2 ? SKINNY_W_BF16 : SKINNY_W_E4M3, d_w, d_x, xs, M, N, K, e, st, pdl != 0);
+    if (tma) return linear_tile(wb, d_w, d_x, xs, M, N, K, e, st, pdl != 0);
     return linear_any(wb, d_w, d_x, xs, M, N, K, e, st, pdl != 0);
+}
+
+extern "C" void mc_sm100_debug_set_tile_plan(uint32_t cg, uint32_t bn, uint32_t splits) { tile_force(cg, bn, splits); }
+
+extern "C" void mc_sm100_debug_tile_plan(int32_t bytes_per_weight, uint32_t M, uint32_t N, uint32_t K, uint32_t sms, uint32_t* cg,
+                                         uint32_t* bn, uint32_t* splits) {
+    const TilePlan p = tile_plan(bytes_per_weight, M, N, K, sms);
+    if (cg != nullptr) *cg = p.cg;
+    if (bn != nullptr) *bn = p.bn;
+    if (splits != nullptr) *splits = p.splits;
 }

@@ -1,0 +1,683 @@
+// linear_tile.cu -- y = epilogue(x W^T) for M > 64 on the 5th-generation tensor cores.
+//
+// The MMA's A operand is a tile of 128 activation rows per CTA, B a tile of BN weight rows, D [128 x BN] fp32 in TMEM (lane =
+// activation row, column = feature).  With CG = 2 two CTAs of a cluster work on one 256 x BN tile (cta_group::2): each loads
+// its own 128 activation rows and HALF of the weight rows, so a weight row enters shared memory once per 256 activation rows.
+//   first EPI warps: epilogue (warp w reads TMEM lanes 32 (w % 4) .. + 31; groups of four take alternate column chunks)
+//   next            : TMA producer of the ring of (A, B) stages, 64 K elements = one 128-byte swizzled row each
+//   next            : MMA issuer (of the pair's first CTA)
+//   e4m3 only, next : TMA producer of raw weight tiles; one warp idle; then eight warps that widen raw tiles to bf16 (exact)
+//                     into the B stages, two groups of four on alternate K blocks
+// Whole K per tile (splits = 1): the kernel is persistent, one CTA per SM, and D is double-buffered, so that the epilogue of a
+// tile runs under the products of the next.  K split over the CTAs of a larger cluster (few tiles): every CTA pushes the
+// column slices that others finish into their shared memory, one cluster barrier, each sums its slice in split order.
+// No atomics; every sum has a fixed order.  Every wait is bounded; one that runs out raises a flag and all roles fall through.
+#include "linear_tile.cuh"
+#include "tcgen05.cuh"
+
+#include <type_traits>
+
+namespace mcl {
+
+namespace {
+
+constexpr uint32_t kBK = 64;                                   // K elements per stage
+constexpr uint32_t kRing = 196608;                             // bytes of the rings
+constexpr unsigned long long kTileWaitNs = 200ull * 1000ull * 1000ull;
+
+__device__ int g_tile_error;
+
+template <int WB, int CG, int BN> struct TileGeom {
+    static constexpr uint32_t A = 128u * kRowBytes, BROWS = BN / CG, B = BROWS * kRowBytes, RAW = WB == 1 ? BROWS * kBK : 0u;
+    static constexpr uint32_t RAWS = WB == 1 ? (kRing / 4u / RAW < 8u ? kRing / 4u / RAW : 8u) : 0u;
+    static constexpr uint32_t FIT = (kRing - RAWS * RAW) / (A + B), STAGES = FIT < 8u ? FIT : 8u;
+    static constexpr uint32_t EPI = WB == 1 ? 4u : 8u;         // epilogue warps
+    static constexpr uint32_t THREADS = 32u * (EPI + (WB == 1 ? 12u : 2u));
+    static constexpr uint32_t COLS = BN;                       // TMEM columns of one accumulator
+    // rings, output staging (2 KB per epilogue warp), bias and scale of two tiles, alignment
+    static constexpr uint32_t SMEM = kRing + EPI * 2048u + 2u * 2u * BN * 4u + 1024u;
+};
+
+struct TileArgs {
+    EpiArgs ep;
+    uint32_t M, N, nkb, n_out;
+    uint32_t m_tiles, n_tiles, tiles, splits;
+    uint32_t y_vec, res_vec;                                   // rows of y / of the residual start on 16-byte boundaries
+    int32_t* status;
+};
+
+constexpr uint32_t kRowGroup = 16;                             // row tiles walked before the next feature tile
+
+__device__ __forceinline__ void tile_of(const TileArgs& a, uint32_t t, uint32_t& mt, uint32_t& nt) {
+    const uint32_t per = kRowGroup * a.n_tiles, g = t / per, rem = t - g * per;
+    const uint32_t rows = min(kRowGroup, a.m_tiles - g * kRowGroup);
+    nt = rem / rows;
+    mt = g * kRowGroup + (rem - nt * rows);
+}
+
+// acquire at cluster scope: arrivals come from both CTAs of a pair
+__device__ __forceinline__ bool tile_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
+    unsigned long long t0 = 0;
+    for (uint32_t spin = 0;; ++spin) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        if (done) return true;
+        if (*abort_flag) return false;
+        if ((spin & 63u) == 63u) {
+            const unsigned long long now = global_timer_ns();
+            if (t0 == 0) t0 = now;
+            else if (now - t0 > kTileWaitNs) break;
+        }
+    }
+    *abort_flag = 1;
+    g_tile_error = 1;
+    if (status != nullptr) *reinterpret_cast<volatile int32_t*>(status) = 1;
+    return false;
+}
+
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// The load lands in this CTA; with CG = 2 the bytes are counted on the barrier of the pair's first CTA (a cluster address).
+template <int CG>
+__device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y) {
+    if constexpr (CG == 1) {
+        tma_load_2d(dst, map, bar, x, y);
+    } else {
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];"
+            ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+    }
+}
+
+template <int CG>
+__device__ __forceinline__ void tile_mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (CG == 1)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// Arrives on the same barrier of every CTA of the pair once the MMAs issued so far are done.
+template <int CG>
+__device__ __forceinline__ void tile_commit(uint32_t bar, uint16_t pair_mask) {
+    if constexpr (CG == 1)
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(bar), "h"(pair_mask) : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts16(uint32_t a, const uint4& v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ float4 lds_f4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// One warp's 32 rows x 32 accumulator columns -> 32 (behind the gate 16) outputs a row.  A lane holds one row while values
+// are computed, and 16-byte pieces of consecutive columns, several rows apart, while they cross global memory; a 2 KB buffer
+// turns one into the other (pieces swizzled by row: neither side meets a bank twice).
+template <bool GATED>
+struct ChunkIO {
+    static constexpr uint32_t LG = GATED ? 1u : 2u, PIECES = 1u << LG, OUTS = 8u * PIECES, ROWS = 32u >> LG, ROW_BYTES = 2u * OUTS;
+    const TileArgs& a;
+    uint32_t buf, lane, own, own_swz, across, col;      // shared addresses of this lane's row / first piece; its first column
+    uint32_t m_base;
+    int32_t rows_left;                                  // rows from this lane's first piece's to the end of y
+    uint16_t* y;
+    const uint16_t* res;
+
+    static __device__ __forceinline__ uint32_t swizzle(uint32_t row) { return GATED ? (row >> 2) & 1u : (row >> 1) & 3u; }
+    __device__ __forceinline__ ChunkIO(const TileArgs& args, uint32_t buffer, uint32_t l, uint32_t row0) : a(args), buf(buffer), lane(l), m_base(row0) {
+        own = buf + lane * ROW_BYTES; own_swz = swizzle(lane);
+        const uint32_t row = lane >> LG, piece = lane & (PIECES - 1u);
+        across = buf + row * ROW_BYTES + ((piece ^ swizzle(row)) << 4);     // + 512 bytes per ROWS rows: the swizzle repeats
+        col = piece * 8u;
+        rows_left = (int32_t)a.M - (int32_t)(m_base + row);
+        y = a.ep.y + (size_t)(m_base + row) * a.ep.y_stride + col;
+        res = a.ep.res != nullptr ? a.ep.res + (size_t)(m_base + row) * a.ep.res_stride + col : nullptr;
+    }
+    __device__ __forceinline__ uint32_t own_piece(uint32_t k) const { return own + ((k ^ own_swz) << 4); }
+    __device__ __forceinline__ uint32_t element(uint32_t row, uint32_t c) const { return buf + row * ROW_BYTES + (((c >> 3) ^ swizzle(row)) << 4) + (c & 7u) * 2u; }
+
+    __device__ __forceinline__ void fetch_res(uint32_t j0, uint4 (&rr)[4]) const {          // aligned rows: ahead of use
+#pragma unroll
+        for (uint32_t i = 0; i < PIECES; ++i) {
+            rr[i] = make_uint4(0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u);         // -0 changes no sum
+            const uint16_t* src = res + (size_t)(i * ROWS) * a.ep.res_stride + j0;
+            if ((int32_t)(i * ROWS) < rows_left) {
+                if (j0 + col + 8u <= a.n_out) rr[i] = *reinterpret_cast<const uint4*>(src);
+                else if (j0 + col < a.n_out) {
+                    uint32_t w[4] = {rr[i].x, rr[i].y, rr[i].z, rr[i].w};
+#pragma unroll
+                    for (uint32_t e = 0; e < 7; ++e)
+                        if (j0 + col + e < a.n_out) w[e >> 1] = (e & 1) ? (w[e >> 1] & 0xFFFFu) | ((uint32_t)src[e] << 16) : (w[e >> 1] & 0xFFFF0000u) | src[e];
+                    rr[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void put_res(const uint4 (&rr)[4]) const {
+#pragma unroll
+        for (uint32_t i = 0; i < PIECES; ++i) sts16(across + i * 512u, rr[i]);
+    }
+    __device__ __forceinline__ void res_elements(uint32_t j0) const {                       // rows at any address
+        const uint32_t c = lane & (OUTS - 1u);
+        for (uint32_t r = lane / OUTS; r < 32u; r += 32u / OUTS) {
+            uint16_t v = 0x8000u;
+            if (m_base + r < a.M && j0 + c < a.n_out) v = a.ep.res[(size_t)(m_base + r) * a.ep.res_stride + j0 + c];
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(element(r, c)), "h"(v) : "memory");
+        }
+    }
+    __device__ __forceinline__ void store(uint32_t j0) const {
+        if (a.y_vec) {
+            uint4 v[PIECES];
+#pragma unroll
+            for (uint32_t i = 0; i < PIECES; ++i) v[i] = lds16(across + i * 512u);
+#pragma unroll
+            for (uint32_t i = 0; i < PIECES; ++i) {
+                uint16_t* dst = y + (size_t)(i * ROWS) * a.ep.y_stride + j0;
+                if ((int32_t)(i * ROWS) < rows_left) {
+                    if (j0 + col + 8u <= a.n_out) *reinterpret_cast<uint4*>(dst) = v[i];
+                    else if (j0 + col < a.n_out) {
+                        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                        for (uint32_t e = 0; e < 7; ++e)
+                            if (j0 + col + e < a.n_out) dst[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+                    }
+                }
+            }
+        } else {
+            const uint32_t c = lane & (OUTS - 1u);
+            for (uint32_t r = lane / OUTS; r < 32u; r += 32u / OUTS) {
+                uint16_t v;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(element(r, c)) : "memory");
+                if (m_base + r < a.M && j0 + c < a.n_out) a.ep.y[(size_t)(m_base + r) * a.ep.y_stride + j0 + c] = v;
+            }
+        }
+    }
+    // v: the 32 finished accumulators of this lane's row, columns n .. n + 31 (tile column c); col_s: staged scales, biases
+    template <uint32_t BN>
+    __device__ __forceinline__ void finish(float (&v)[32], uint32_t n, uint32_t c, uint32_t col_s, bool has_scale, bool has_bias, uint4 (&rr)[4],
+                                           uint32_t next_n) const {
+        const uint32_t j0 = GATED ? n >> 1 : n;
+        const bool has_res = a.ep.res != nullptr;
+        uint4 mine[PIECES];
+        if (has_res) {
+            if (a.res_vec) {
+                put_res(rr);
+                if (next_n != 0xFFFFFFFFu) fetch_res(GATED ? next_n >> 1 : next_n, rr);
+            } else res_elements(j0);
+            __syncwarp();
+#pragma unroll
+            for (uint32_t k = 0; k < PIECES; ++k) mine[k] = lds16(own_piece(k));
+            __syncwarp();
+        }
+        if (has_scale) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float4 f = lds_f4(col_s + (c + 4u * k) * 4u);
+                v[4 * k] *= f.x; v[4 * k + 1] *= f.y; v[4 * k + 2] *= f.z; v[4 * k + 3] *= f.w;
+            }
+        }
+        if (has_bias) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float4 f = lds_f4(col_s + (BN + c + 4u * k) * 4u);
+                v[4 * k] += f.x; v[4 * k + 1] += f.y; v[4 * k + 2] += f.z; v[4 * k + 3] += f.w;
+            }
+        }
+        const uint32_t act = a.ep.act;
+        auto apply = [&](auto f) {
+            if constexpr (GATED) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = f(v[2 * k]) * v[2 * k + 1];
+            } else {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) v[k] = f(v[k]);
+            }
+        };
+        // one loop per activation: no choice inside
+        if (act == MC_SM100_ACT_SILU) apply([](float z) { return epi_act(z, MC_SM100_ACT_SILU); });
+        else if (act == MC_SM100_ACT_GELU) apply([](float z) { return epi_act(z, MC_SM100_ACT_GELU); });
+        else if (act == MC_SM100_ACT_GELU_TANH) apply([](float z) { return epi_act(z, MC_SM100_ACT_GELU_TANH); });
+        else if (act == MC_SM100_ACT_RELU) apply([](float z) { return epi_act(z, MC_SM100_ACT_RELU); });
+        else if (GATED) apply([](float z) { return z; });
+        if (has_res) {
+#pragma unroll
+            for (uint32_t k = 0; k < PIECES; ++k) {
+                const uint32_t r[4] = {mine[k].x, mine[k].y, mine[k].z, mine[k].w};
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) { v[8 * k + 2 * e] += bf16lo(r[e]); v[8 * k + 2 * e + 1] += bf16hi(r[e]); }
+            }
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < PIECES; ++k)
+            sts16(own_piece(k), make_uint4(pack_bf16(v[8 * k], v[8 * k + 1]), pack_bf16(v[8 * k + 2], v[8 * k + 3]),
+                                           pack_bf16(v[8 * k + 4], v[8 * k + 5]), pack_bf16(v[8 * k + 6], v[8 * k + 7])));
+        __syncwarp();
+        store(j0);
+        __syncwarp();
+    }
+};
+
+}  // namespace
+
+// WB: bytes per weight element.  CG: CTAs per tile.  BN: features per tile.
+template <int WB, int CG, int BN>
+__global__ void __launch_bounds__(TileGeom<WB, CG, BN>::THREADS, 1)
+linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const TileArgs a) {
+    using G = TileGeom<WB, CG, BN>;
+    constexpr uint32_t STAGES = G::STAGES, RAWS = G::RAWS, EPI = G::EPI;
+    constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((128 * CG) >> 4) << 24);
+    constexpr uint32_t CONV_WARPS = 4;                           // warps that widen one K block
+
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[36];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sA = base, sB = base + STAGES * G::A, sRaw = sB + STAGES * G::B;
+    const uint32_t sBuf = base + kRing, sCol = sBuf + EPI * 2048u;
+    const uint32_t bar0 = smem_u32(bars);
+    auto full = [&](uint32_t s) { return bar0 + 8u * s; };
+    auto empty = [&](uint32_t s) { return bar0 + 8u * (8u + s); };
+    auto raw_full = [&](uint32_t s) { return bar0 + 8u * (16u + s); };
+    auto raw_empty = [&](uint32_t s) { return bar0 + 8u * (24u + s); };
+    auto acc_full = [&](uint32_t b) { return bar0 + 8u * (32u + b); };
+    auto acc_empty = [&](uint32_t b) { return bar0 + 8u * (34u + b); };
+
+    const uint32_t S = a.splits, csize = CG * S, crank = blockIdx.x % csize, cid = blockIdx.x / csize, clusters = gridDim.x / csize;
+    const uint32_t split = crank / CG, sub = crank % CG, lead = crank - sub;
+    const bool leader = sub == 0u;
+    const uint32_t kb0 = split * a.nkb / S, kb1 = (split + 1u) * a.nkb / S;
+    const uint32_t bufs = S == 1u ? 2u : 1u;
+    const uint32_t tmem_cols = bufs * BN < 32u ? 32u : bufs * BN;
+
+    pdl_trigger();
+    if (tid == 0) {
+        abort_flag = 0;
+        for (uint32_t s = 0; s < STAGES; ++s) { mbar_init(full(s), 1u + (WB == 1 ? CONV_WARPS * CG : 0u)); mbar_init(empty(s), 1); }
+        if constexpr (WB == 1)
+            for (uint32_t s = 0; s < RAWS; ++s) { mbar_init(raw_full(s), 1); mbar_init(raw_empty(s), CONV_WARPS); }
+        for (uint32_t b = 0; b < 2; ++b) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), EPI * CG); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+    }
+    if (warp == EPI + 1u) {
+        if constexpr (CG == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(tmem_cols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(tmem_cols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();                                              // barriers and TMEM of every CTA are there
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_slot;
+    volatile int* abortp = &abort_flag;
+    pdl_wait();
+
+    if (warp == EPI) {
+        if (lane == 0) {
+            // -------------------------------------------------- producer of A (bf16: A and B)
+            bool ok = true;
+            uint32_t it = 0;
+            for (uint32_t t = cid; t < a.tiles && ok; t += clusters) {
+                uint32_t mt, nt;
+                tile_of(a, t, mt, nt);
+                const int32_t m0 = (int32_t)((mt * CG + sub) * 128u), n0 = (int32_t)(nt * BN + sub * G::BROWS);
+                for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
+                    const uint32_t s = it % STAGES;
+                    if (it >= STAGES) ok = tile_wait(empty(s), ((it / STAGES) - 1u) & 1u, abortp, a.status);
+                    if (!ok) break;
+                    if (leader) mbar_expect_tx(full(s), CG * (G::A + (WB == 2 ? G::B : 0u)));
+                    const uint32_t bar = CG == 2 ? map_to_rank(full(s), lead) : full(s);
+                    tile_load<CG>(sA + s * G::A, &map_x, bar, (int32_t)(kb * kBK), m0);
+                    if constexpr (WB == 2) tile_load<CG>(sB + s * G::B, &map_w, bar, (int32_t)(kb * kBK), n0);
+                }
+            }
+        }
+    } else if (warp == EPI + 1u) {
+        if (lane == 0 && leader) {
+            // -------------------------------------------------- MMA issuer
+            const uint16_t pair = (uint16_t)(CG == 2 ? 3u << lead : 1u);
+            bool ok = true;
+            uint32_t it = 0, i = 0;
+            for (uint32_t t = cid; t < a.tiles && ok; t += clusters, ++i) {
+                const uint32_t b = i % bufs;
+                if (i >= bufs) ok = tile_wait(acc_empty(b), ((i / bufs) - 1u) & 1u, abortp, a.status);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
+                    const uint32_t s = it % STAGES;
+                    ok = tile_wait(full(s), (it / STAGES) & 1u, abortp, a.status);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t da = make_desc(sA + s * G::A), db = make_desc(sB + s * G::B);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        tile_mma<CG>(tmem + b * G::COLS, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), IDESC, (kb > kb0 || k > 0) ? 1u : 0u);
+                    tile_commit<CG>(empty(s), pair);
+                }
+                if (ok) tile_commit<CG>(acc_full(b), pair);
+            }
+        }
+    } else if (warp == EPI + 2u) {
+        if constexpr (WB == 1) if (lane == 0) {
+            // -------------------------------------------------- producer of raw weight tiles
+            bool ok = true;
+            uint32_t it = 0;
+            for (uint32_t t = cid; t < a.tiles && ok; t += clusters) {
+                uint32_t mt, nt;
+                tile_of(a, t, mt, nt);
+                const int32_t n0 = (int32_t)(nt * BN + sub * G::BROWS);
+                for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
+                    const uint32_t r = it % RAWS;
+                    if (it >= RAWS) ok = tile_wait(raw_empty(r), ((it / RAWS) - 1u) & 1u, abortp, a.status);
+                    if (!ok) break;
+                    mbar_expect_tx(raw_full(r), G::RAW);
+                    tma_load_2d(sRaw + r * G::RAW, &map_w, raw_full(r), (int32_t)(kb * kBK), n0);
+                }
+            }
+        }
+    } else if (warp >= EPI + 4u) {
+        // ------------------------------------------------------ e4m3 -> bf16
+        if constexpr (WB == 1) {
+        constexpr uint32_t R = RAWS;
+        const uint32_t group = (warp - (EPI + 4u)) / CONV_WARPS, ct = tid & (CONV_WARPS * 32u - 1u);
+        const uint32_t my_tiles = cid < a.tiles ? (a.tiles - cid + clusters - 1u) / clusters : 0u, total = my_tiles * (kb1 - kb0);
+        bool ok = true;
+        for (uint32_t it = group; it < total && ok; it += 2u) {
+            const uint32_t r = it % R, s = it % STAGES;
+            ok = tile_wait(raw_full(r), (it / R) & 1u, abortp, a.status);
+            if (ok && it >= STAGES) ok = tile_wait(empty(s), ((it / STAGES) - 1u) & 1u, abortp, a.status);
+            if (!ok) break;
+            // 16-byte raw chunks: 8 rows of one chunk column per quarter warp; every load ahead of the first store
+            constexpr uint32_t PER = G::BROWS * 4u / (CONV_WARPS * 32u);
+            uint4 raw[PER];
+            const uint32_t row0 = (ct & 7u) | ((ct >> 5) << 3), cc = (ct >> 3) & 3u;
+#pragma unroll
+            for (uint32_t i = 0; i < PER; ++i) raw[i] = lds16(sRaw + r * G::RAW + (row0 + 32u * i) * kBK + cc * 16u);
+#pragma unroll
+            for (uint32_t i = 0; i < PER; ++i) {
+                const uint32_t row = row0 + 32u * i;
+                const uint4 v = raw[i];
+                const uint32_t two120 = 0x7B807B80u;                      // 2^120 as bf16x2
+                uint32_t o[8];
+                o[0] = e4m3x2_to_bf16x2_scaled<0x1404u>(v.x); o[1] = e4m3x2_to_bf16x2_scaled<0x3424u>(v.x);
+                o[2] = e4m3x2_to_bf16x2_scaled<0x1404u>(v.y); o[3] = e4m3x2_to_bf16x2_scaled<0x3424u>(v.y);
+                o[4] = e4m3x2_to_bf16x2_scaled<0x1404u>(v.z); o[5] = e4m3x2_to_bf16x2_scaled<0x3424u>(v.z);
+                o[6] = e4m3x2_to_bf16x2_scaled<0x1404u>(v.w); o[7] = e4m3x2_to_bf16x2_scaled<0x3424u>(v.w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(o[j]) : "r"(two120));   // exact
+                sts16(sB + s * G::B + swz(row, 2u * cc), make_uint4(o[0], o[1], o[2], o[3]));
+                sts16(sB + s * G::B + swz(row, 2u * cc + 1u), make_uint4(o[4], o[5], o[6], o[7]));
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                if (CG == 2) arrive_remote(map_to_rank(full(s), lead));
+                else mbar_arrive(full(s));
+                mbar_arrive(raw_empty(r));
+            }
+        }
+        }
+    }
+    if (warp < EPI) {
+        // ------------------------------------------------------ epilogue
+        constexpr uint32_t GROUPS = EPI / 4u;
+        const uint32_t q = warp & 3u, group = warp >> 2;
+        const bool has_scale = a.ep.scale != nullptr, has_bias = a.ep.bias != nullptr;
+        auto run = [&](auto gated) {
+            using IO = ChunkIO<decltype(gated)::value>;
+            bool ok = true;
+            uint32_t i = 0;
+            for (uint32_t t = cid; t < a.tiles; t += clusters, ++i) {
+                uint32_t mt, nt;
+                tile_of(a, t, mt, nt);
+                const uint32_t b = i % bufs, n0 = nt * BN;
+                const IO io(a, sBuf + warp * 2048u, lane, (mt * CG + sub) * 128u + q * 32u);
+                // scale and bias of the tile's features, in the half of the staging area that the previous tile does not read
+                const uint32_t col_s = sCol + (i & 1u) * (2u * BN * 4u);
+                if (has_scale || has_bias) {
+                    for (uint32_t c = tid; c < BN; c += EPI * 32u) {
+                        const uint32_t n = n0 + c;
+                        const float sc = has_scale && n < a.N ? a.ep.scale[n] : 1.f;
+                        const float bi = has_bias && n < a.N ? __uint_as_float((uint32_t)a.ep.bias[n] << 16) : 0.f;
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(col_s + c * 4u), "f"(sc) : "memory");
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(col_s + (BN + c) * 4u), "f"(bi) : "memory");
+                    }
+                    asm volatile("bar.sync 1, %0;" ::"n"(EPI * 32u) : "memory");
+                }
+                // this CTA finishes columns [c_lo, c_hi), this warp every GROUPS-th chunk of them
+                const uint32_t per = BN / S, c_lo = split * per, c_hi = n0 + c_lo + per <= a.N ? c_lo + per : (a.N - n0 > c_lo ? a.N - n0 : c_lo);
+                const uint32_t c_first = c_lo + group * 32u;
+                uint4 rr[4];
+                if (a.ep.res != nullptr && a.res_vec && c_first < c_hi) io.fetch_res((n0 + c_first) >> a.ep.gated, rr);
+                if (ok) ok = tile_wait(acc_full(b), (i / bufs) & 1u, abortp, a.status);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t taddr = tmem + b * G::COLS + ((q * 32u) << 16);
+                const uint32_t row = q * 32u + lane;
+                auto release = [&]() {                                               // this warp has read its part of the accumulator
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) { if (CG == 2) arrive_remote(map_to_rank(acc_empty(b), lead)); else mbar_arrive(acc_empty(b)); }
+                };
+                if (S > 1u) {
+                    // the cluster's rings are idle: they become the exchange [source split][row][per] of fp32
+                    cluster_sync();
+                    uint32_t turn = 0;
+                    for (uint32_t o = 0; o < S; ++o) {
+                        if (o == split) continue;
+                        const uint32_t src = split < o ? split : split - 1u;
+                        const uint32_t dst = map_to_rank(base + (src * 128u + row) * per * 4u, o * CG + sub);
+                        for (uint32_t c = 0; c < per; c += 32u, ++turn) {
+                            if (turn % GROUPS != group) continue;
+                            float v[32];
+                            tmem_ld32(taddr + o * per + c, v);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};"
+                                             ::"r"(dst + ((((c >> 2) + k) ^ (row & 7u)) << 4)), "f"(v[4 * k]), "f"(v[4 * k + 1]), "f"(v[4 * k + 2]), "f"(v[4 * k + 3]) : "memory");
+                        }
+                    }
+                    cluster_sync();
+                } else if (c_first >= c_hi) release();
+                const bool failed = !ok || *abortp != 0;
+                for (uint32_t c = c_first; c < c_hi; c += 32u * GROUPS) {
+                    const bool last = c + 32u * GROUPS >= c_hi;
+                    float v[32];
+                    tmem_ld32(taddr + c, v);
+                    if (S == 1u && last) release();
+                    if (S > 1u) {
+                        float sum[32];
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) sum[k] = 0.f;
+                        for (uint32_t p = 0; p < S; ++p) {                           // split order
+                            if (p == split) {
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) sum[k] += v[k];
+                            } else {
+                                const uint32_t src = p < split ? p : p - 1u, at = base + (src * 128u + row) * per * 4u;
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) {
+                                    const float4 f = lds_f4(at + (((((c - c_lo) >> 2) + k) ^ (row & 7u)) << 4));
+                                    sum[4 * k] += f.x; sum[4 * k + 1] += f.y; sum[4 * k + 2] += f.z; sum[4 * k + 3] += f.w;
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) v[k] = sum[k];
+                    }
+                    if (!failed) io.template finish<BN>(v, n0 + c, c, col_s, has_scale, has_bias, rr, last ? 0xFFFFFFFFu : n0 + c + 32u * GROUPS);
+                }
+            }
+        };
+        if (a.ep.gated) run(std::true_type{});
+        else run(std::false_type{});
+    } else if (S > 1u) {
+        // the other warps pass the two barriers of the exchange
+        __syncwarp();
+        cluster_sync();
+        cluster_sync();
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (*abortp) {                                               // a wait ran out: let this CTA's copies in flight land before it leaves
+        const unsigned long long t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    }
+    cluster_sync();                                              // nobody addresses a CTA that has left
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == EPI + 1u) {
+        if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");
+    }
+}
+
+namespace {
+
+template <int WB, int CG, int BN>
+mc_status_t launch_tile(const void* w, const uint16_t* x, uint32_t x_pitch, uint32_t K, TileArgs a, cudaStream_t stream, bool pdl) {
+    using G = TileGeom<WB, CG, BN>;
+    auto kern = linear_tile_kernel<WB, CG, BN>;
+    static SmemOptIn optin;
+    const cudaError_t e = optin.ensure(kern, G::SMEM);
+    if (e != cudaSuccess) {
+        set_error("linear_tile: cannot raise shared memory to %u: %s", G::SMEM, cudaGetErrorString(e));
+        return MC_E_CUDA;
+    }
+    CUtensorMap map_w, map_x;
+    mc_status_t s = tma_encode_2d(&map_w, w, a.N, K, K, WB, kBK, G::BROWS, WB == 2);
+    if (s == MC_OK) s = tma_encode_2d(&map_x, x, a.M, K, x_pitch, 2, kBK, 128, true);
+    if (s != MC_OK) return s;
+    const uint64_t mt = (a.M + 128ull * CG - 1) / (128ull * CG), nt = (a.N + BN - 1ull) / BN;
+    if (mt * nt * CG * a.splits > 0x7FFFFFFFull) {
+        set_error("mc_sm100_linear_epilogue: M=%u N=%u make too many tiles", a.M, a.N);
+        return MC_E_UNSUPPORTED;
+    }
+    a.m_tiles = (uint32_t)mt; a.n_tiles = (uint32_t)nt; a.tiles = (uint32_t)(mt * nt);
+    uint32_t clusters = a.tiles;
+    if (a.splits == 1u) {
+        const uint32_t room = (uint32_t)sm_count() / CG;
+        if (clusters > room) clusters = room;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(clusters * CG * a.splits);
+    cfg.blockDim = dim3(G::THREADS);
+    cfg.dynamicSmemBytes = G::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = CG * a.splits;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = pdl ? 2 : 1;
+    (void)cudaLaunchKernelEx(&cfg, kern, map_w, map_x, a);
+    MCL_CHECK_LAUNCH("linear_tile");
+    return MC_OK;
+}
+
+}  // namespace
+
+TilePlan tile_plan(int, uint32_t, uint32_t, uint32_t, uint32_t) { return {2, 256, 1}; }
+
+// benchmark and test hook: every call takes this plan (cg = 0: the rule above)
+static std::atomic<uint32_t> g_forced{0};
+void tile_force(uint32_t cg, uint32_t bn, uint32_t splits) { g_forced.store(cg == 0u ? 0u : (cg << 24) | (splits << 16) | bn); }
+
+mc_status_t linear_tile(int wb, const void* w, const uint16_t* x, uint32_t x_pitch, uint32_t M, uint32_t N, uint32_t K,
+                        const EpiArgs& ep, cudaStream_t stream, bool pdl) {
+    TilePlan p = tile_plan(wb, M, N, K, (uint32_t)sm_count());
+    if (const uint32_t f = g_forced.load(); f != 0u) p = {f >> 24, f & 0xFFFFu, (f >> 16) & 0xFFu};
+    const uint32_t blocks = (K + kBK - 1) / kBK;
+    while (p.splits > 1u && (p.splits > blocks || p.bn / p.splits < 32u || p.cg * p.splits > 8u)) p.splits >>= 1;   // a slice is never empty
+    TileArgs a{};
+    a.ep = ep; a.M = M; a.N = N; a.nkb = blocks; a.n_out = ep.gated ? N / 2u : N; a.splits = p.splits;
+    a.y_vec = aligned16(ep.y) && (ep.y_stride & 7u) == 0u;
+    a.res_vec = aligned16(ep.res) && (ep.res_stride & 7u) == 0u;
+    a.status = wait_status_sink();
+    const uint32_t key = (uint32_t)wb * 10000u + p.cg * 1000u + p.bn;
+    switch (key) {
+        case 22256: return launch_tile<2, 2, 256>(w, x, x_pitch, K, a, stream, pdl);
+        case 22128: return launch_tile<2, 2, 128>(w, x, x_pitch, K, a, stream, pdl);
+        case 21256: return launch_tile<2, 1, 256>(w, x, x_pitch, K, a, stream, pdl);
+        case 21128: return launch_tile<2, 1, 128>(w, x, x_pitch, K, a, stream, pdl);
+        case 21064: return launch_tile<2, 1, 64>(w, x, x_pitch, K, a, stream, pdl);
+        case 12256: return launch_tile<1, 2, 256>(w, x, x_pitch, K, a, stream, pdl);
+        case 12128: return launch_tile<1, 2, 128>(w, x, x_pitch, K, a, stream, pdl);
+        case 11256: return launch_tile<1, 1, 256>(w, x, x_pitch, K, a, stream, pdl);
+        case 11128: return launch_tile<1, 1, 128>(w, x, x_pitch, K, a, stream, pdl);
+        case 11064: return launch_tile<1, 1, 64>(w, x, x_pitch, K, a, stream, pdl);
+        default: set_error("linear_tile: no kernel for plan %u", key); return MC_E_INTERNAL;
+    }
+}
+
+int linear_tile_take_error() {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_tile_error, sizeof(int)) != cudaSuccess) return -1;
+    if (v != 0) {
+        const int zero = 0;
+        (void)cudaMemcpyToSymbol(g_tile_error, &zero, sizeof(int));
+    }
+    return v;
+}
+
+}  // namespace mcl

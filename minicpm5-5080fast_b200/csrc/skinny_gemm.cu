@@ -25,11 +25,7 @@
 // Every wait is bounded; a wait that runs out raises a flag in global memory and all
 // roles fall through to the common exit, where TMEM is released.
 #include "skinny_gemm.cuh"
-
-#include <cuda.h>
-
-#include <mutex>
-#include <unordered_map>
+#include "tcgen05.cuh"
 
 namespace mcl {
 
@@ -39,22 +35,10 @@ constexpr int kTileN = 128;        // weight rows per CTA (MMA M)
 constexpr int kThreads = 320;      // 10 warps
 constexpr int kConvThreads = 256;  // warps 2..9
 constexpr uint32_t kConvGroup = 128;  // converter threads that share one K block (two groups; four groups of 64 ran into bounded-wait timeouts and are not used)
-constexpr int kRowBytes = 128;     // bytes per operand-tile row in shared memory (one swizzle row)
 constexpr unsigned long long kWaitLimitNs = 200ull * 1000ull * 1000ull;   // a wait gives up after 200 ms
 
 __device__ int g_skinny_error;     // set when a bounded wait ran out (read back by tests)
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
 // Bounded wait on a phase parity.  Returns false when the limit ran out or
 // another role already gave up (abort flag in shared memory).
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
@@ -81,28 +65,6 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     g_skinny_error = 1;
     if (status != nullptr) *reinterpret_cast<volatile int32_t*>(status) = 1;
     return false;
-}
-
-// 2-D tiled TMA load global -> this CTA's shared memory; x is the innermost
-// (K) coordinate in elements, y the row.  x * element size is a multiple of 16 bytes
-// at every call site (K steps of 64 bf16 / 64 or 128 e4m3).
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
-        : "memory");
-}
-
-// K-major, 128-byte swizzle: 8-row groups are 1024 bytes apart; the leading
-// offset is unused for swizzled K-major layouts (encoded as 1); version 1.
-__device__ __forceinline__ uint64_t make_desc(uint32_t saddr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr & 0x3FFFFu) >> 4);
-    d |= (uint64_t)1 << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
 }
 
 template <int KIND_F8>
@@ -137,9 +99,6 @@ struct SkinnyArgs {
     PeerOut out;            // sharded step: the result goes to every rank's activation buffer as tagged words (world = 0: to y)
     PrefetchArgs pf;        // L2 prefetch of the next kernel's weights (all zero = off)
 };
-
-// swizzled byte offset of 16-byte chunk `cc` (0..7) of tile row `row`
-__device__ __forceinline__ uint32_t swz(uint32_t row, uint32_t cc) { return row * kRowBytes + ((cc ^ (row & 7u)) << 4); }
 
 // Stage geometry per mode; the ring depth is a launch parameter (as many stages as fit in
 // half an SM's shared memory).
@@ -494,84 +453,6 @@ Plan make_plan(uint32_t N, uint32_t K, uint32_t bk) {
     return p;
 }
 
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no link against libcuda).
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    if (fn == nullptr) {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-    }
-    return fn;
-}
-
-// Row-major [rows, K] matrix of 1- or 2-byte elements, box = [box_rows x box_k]; out-of-range
-// rows / columns read as zero (ragged N, M < Mpad, K tail).
-mc_status_t encode_map(CUtensorMap* map, const void* ptr, uint32_t rows, uint32_t K, uint32_t pitch, uint32_t elem_bytes,
-                       uint32_t box_k, uint32_t box_rows, bool swizzle128) {
-    EncodeTiledFn fn = encode_fn();
-    if (fn == nullptr) {
-        set_error("skinny_gemm: cuTensorMapEncodeTiled is not available from this driver");
-        return MC_E_CUDA;
-    }
-    const cuuint64_t dims[2] = {K, rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)pitch * elem_bytes};   // row pitch in bytes (a multiple of 16)
-    const cuuint32_t box[2] = {box_k, box_rows};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
-                          const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) {
-        set_error("skinny_gemm: cuTensorMapEncodeTiled failed (%d) for rows=%u K=%u", (int)r, rows, K);
-        return MC_E_CUDA;
-    }
-    return MC_OK;
-}
-
-// An encoded tensor map depends only on (address, shape, box): a step launched eagerly would
-// otherwise pay two driver encodes per GEMM.  Small process-wide cache, cleared when full.
-struct MapKey {
-    const void* ptr; uint32_t rows, K, pitch, elem, box_k, box_rows, swz;
-    bool operator==(const MapKey& o) const {
-        return ptr == o.ptr && rows == o.rows && K == o.K && pitch == o.pitch && elem == o.elem && box_k == o.box_k && box_rows == o.box_rows && swz == o.swz;
-    }
-};
-struct MapKeyHash {
-    size_t operator()(const MapKey& k) const {
-        uint64_t h = 0xCBF29CE484222325ull;
-        const uint64_t v[5] = {(uint64_t)(uintptr_t)k.ptr, ((uint64_t)k.rows << 32) | k.K, ((uint64_t)k.box_k << 32) | k.box_rows,
-                               ((uint64_t)k.elem << 32) | k.swz, k.pitch};
-        for (uint64_t x : v) { h ^= x; h *= 0x100000001B3ull; }
-        return (size_t)h;
-    }
-};
-constexpr size_t kMapCacheMax = 4096;
-
-mc_status_t make_map(CUtensorMap* map, const void* ptr, uint32_t rows, uint32_t K, uint32_t pitch, uint32_t elem_bytes,
-                     uint32_t box_k, uint32_t box_rows, bool swizzle128) {
-    static std::mutex mu;
-    static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
-    const MapKey key{ptr, rows, K, pitch, elem_bytes, box_k, box_rows, swizzle128 ? 1u : 0u};
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        auto it = cache.find(key);
-        if (it != cache.end()) { *map = it->second; return MC_OK; }
-    }
-    const mc_status_t s = encode_map(map, ptr, rows, K, pitch, elem_bytes, box_k, box_rows, swizzle128);
-    if (s != MC_OK) return s;
-    std::lock_guard<std::mutex> lock(mu);
-    if (cache.size() >= kMapCacheMax) cache.clear();
-    cache.emplace(key, *map);
-    return MC_OK;
-}
-
 template <int MODE, int NPAD, bool EXT>
 mc_status_t launch_one(const void* w, const void* x, uint32_t x_pitch, const SkinnyArgs& a, uint32_t grid, cudaStream_t stream, bool pdl) {
     using G = Ring<MODE, NPAD>;
@@ -586,15 +467,19 @@ mc_status_t launch_one(const void* w, const void* x, uint32_t x_pitch, const Ski
     const size_t smem = (size_t)G::bytes(a.op_stages, MODE == SKINNY_W_E4M3 ? a.raw_stages : 0) + (size_t)(NPAD + 4) * kTileN * 4 + 2048;
     CUtensorMap map_w, map_x;
     mc_status_t s;
-    if (MODE == SKINNY_W_BF16) {
-        s = make_map(&map_w, w, a.N, a.K, a.K, 2, 64, kTileN, true);
-        if (s == MC_OK) s = make_map(&map_x, x, a.M, a.K, x_pitch, 2, 64, NPAD, true);
+    if (EXT) {      // nothing is kept from call to call
+        constexpr bool E4 = MODE == SKINNY_W_E4M3;
+        s = tma_encode_2d(&map_w, w, a.N, a.K, a.K, E4 ? 1 : 2, 64, kTileN, !E4);
+        if (s == MC_OK) s = tma_encode_2d(&map_x, x, a.M, a.K, x_pitch, 2, 64, NPAD, true);
+    } else if (MODE == SKINNY_W_BF16) {
+        s = tma_map_2d(&map_w, w, a.N, a.K, a.K, 2, 64, kTileN, true);
+        if (s == MC_OK) s = tma_map_2d(&map_x, x, a.M, a.K, x_pitch, 2, 64, NPAD, true);
     } else if (MODE == SKINNY_W_E4M3) {
-        s = make_map(&map_w, w, a.N, a.K, a.K, 1, 64, kTileN, false);      // raw codes, widened by warps 2-9
-        if (s == MC_OK) s = make_map(&map_x, x, a.M, a.K, x_pitch, 2, 64, NPAD, true);
+        s = tma_map_2d(&map_w, w, a.N, a.K, a.K, 1, 64, kTileN, false);      // raw codes, widened by warps 2-9
+        if (s == MC_OK) s = tma_map_2d(&map_x, x, a.M, a.K, x_pitch, 2, 64, NPAD, true);
     } else {
-        s = make_map(&map_w, w, a.N, a.K, a.K, 1, 128, kTileN, true);
-        if (s == MC_OK) s = make_map(&map_x, x, a.M, a.K, x_pitch, 1, 128, NPAD, true);
+        s = tma_map_2d(&map_w, w, a.N, a.K, a.K, 1, 128, kTileN, true);
+        if (s == MC_OK) s = tma_map_2d(&map_x, x, a.M, a.K, x_pitch, 1, 128, NPAD, true);
     }
     if (s != MC_OK) return s;
     cudaLaunchConfig_t cfg{};

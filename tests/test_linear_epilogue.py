@@ -105,6 +105,30 @@ SHAPES = [(1, 1, 1), (1, 2, 7), (2, 31, 16), (3, 130, 24), (5, 96, 72), (1, 2304
           (129, 514, 136), (200, 1026, 1040), (255, 30, 48), (256, 512, 512), (301, 770, 2304), (513, 258, 72), (1030, 130, 80)]
 
 
+PLANS = [(1, 64, 1), (1, 64, 2), (1, 128, 1), (1, 128, 2), (1, 128, 4), (1, 256, 1), (1, 256, 8), (2, 128, 1), (2, 128, 2), (2, 128, 4), (2, 256, 1), (2, 256, 4)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("plan", PLANS)
+def test_tile_plans(pkg, plan):
+    """Every way of cutting a call of more than 64 rows, at sizes around its tiles, and many more tiles than SMs."""
+    pkg.debug_set_tile_plan(*plan)
+    try:
+        for e4m3 in (False, True):
+            _run(pkg, 128, 64, 64, e4m3, seed=1)
+            assert pkg.debug_take_error() == 0
+            _run(pkg, 128, 256, 512, e4m3, seed=2)
+            _run(pkg, 65, 30, 1040, e4m3, bias=True, residual=True, act="silu", seed=3)
+            _run(pkg, 300, 514, 656, e4m3, bias=True, residual=True, act="gelu", gated=True, seed=4)
+            _run(pkg, 300, 515, 656, e4m3, bias=True, residual=True, act="relu", seed=5)
+            _run(pkg, 257, 520, 80, e4m3, bias=True, residual=True, y_pad=3, r_pad=1, x_pad=8, seed=6)
+            _run(pkg, 2600, 2000, 192, e4m3, bias=True, in_place=True, seed=7)
+            _run(pkg, 2600, 2002, 192, e4m3, act="silu", gated=True, in_place=True, y_pad=3, seed=8)
+            assert pkg.debug_take_error() == 0
+    finally:
+        pkg.debug_set_tile_plan()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("shape", SHAPES)
