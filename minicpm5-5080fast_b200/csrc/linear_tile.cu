@@ -30,8 +30,13 @@ __device__ int g_tile_error;
 template <int WB, int CG, int BN> struct TileGeom {
     static constexpr uint32_t A = 128u * kRowBytes, BROWS = BN / CG, B = BROWS * kRowBytes, RAW = WB == 1 ? BROWS * kBK : 0u;
     static constexpr uint32_t RAWS = WB == 1 ? (kRing / 4u / RAW < 8u ? kRing / 4u / RAW : 8u) : 0u;
+    // Even: a raw stage is then always the same group's.  With an odd count the groups take turns on a stage, and the one that
+    // is ahead can find the parity of the use before the last where it waits for the last: it would pass too early.
+    static_assert(RAWS % 2u == 0u, "two groups of widening warps take alternate raw stages");
     static constexpr uint32_t FIT = (kRing - RAWS * RAW) / (A + B), STAGES = FIT < 8u ? FIT : 8u;
-    static constexpr uint32_t EPI = WB == 1 ? 4u : 8u;         // epilogue warps
+    static constexpr uint32_t EPI = 8u;                        // epilogue warps
+    // e4m3: 640 threads launched with 96 registers each; the roles trade them (setmaxnreg, warpgroups of 128 threads):
+    // 2 x 128 x 136 (epilogue) + 128 x 48 (producers, MMA) + 2 x 128 x 80 (widening) = 640 x 96, what the CTA was launched with.
     static constexpr uint32_t THREADS = 32u * (EPI + (WB == 1 ? 12u : 2u));
     static constexpr uint32_t COLS = BN;                       // TMEM columns of one accumulator
     // rings, output staging (2 KB per epilogue warp), bias and scale of two tiles, alignment
@@ -84,8 +89,21 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// Nothing that the other CTA's threads read stands behind these arrivals: a widened tile is read by the tensor core out of
+// the arriving CTA's own shared memory (fence.proxy.async has run), a drained accumulator is written by it (tcgen05 fences).
+// So the release stays at CTA scope; at cluster scope it made the arrival cost more than the widening (M = 8192, 2304 x 5760:
+// 291 against 177 us).
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+// Four e4m3 codes -> four bf16 of value * 2^-120 (the 7 magnitude bits dropped at bit 4), byte-wise: 7 integer operations
+// where placing pair by pair takes 8; then * 2^120, exact.
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& p01, uint32_t& p23) {
+    const uint32_t hi = ((w >> 4) & 0x07070707u) | (w & 0x80808080u), lo = (w << 4) & 0xF0F0F0F0u;
+    p01 = __byte_perm(lo, hi, 0x5140u);
+    p23 = __byte_perm(lo, hi, 0x7362u);
+    asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(p01) : "r"(0x7B807B80u));
+    asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(p23) : "r"(0x7B807B80u));
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
@@ -208,12 +226,43 @@ struct ChunkIO {
 #pragma unroll
         for (uint32_t i = 0; i < PIECES; ++i) sts16(across + i * 512u, rr[i]);
     }
-    __device__ __forceinline__ void res_elements(uint32_t j0) const {                       // rows at any address
-        const uint32_t c = lane & (OUTS - 1u);
-        for (uint32_t r = lane / OUTS; r < 32u; r += 32u / OUTS) {
-            uint16_t v = 0x8000u;
-            if (m_base + r < a.M && j0 + c < a.n_out) v = a.ep.res[(size_t)(m_base + r) * a.ep.res_stride + j0 + c];
-            asm volatile("st.shared.u16 [%0], %1;" ::"r"(element(r, c)), "h"(v) : "memory");
+    // Rows at any address: a lane holds one column of every row (gated: of every second row); eight rows in flight.
+    __device__ __forceinline__ void res_elements(uint32_t j0) const {
+        const uint32_t c = lane & (OUTS - 1u), r0 = lane / OUTS;
+        const int32_t left = (int32_t)a.M - (int32_t)(m_base + r0);
+        const bool in = j0 + c < a.n_out;
+        const uint16_t* src = a.ep.res + (size_t)(m_base + r0) * a.ep.res_stride + j0 + c;
+        const size_t step = (size_t)(32u / OUTS) * a.ep.res_stride;
+#pragma unroll
+        for (uint32_t r = 0; r < OUTS; r += 8u) {
+            uint16_t v[8];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) {
+                v[e] = in && (int32_t)((r + e) * (32u / OUTS)) < left ? *src : (uint16_t)0x8000u;
+                src += step;
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e)
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(element(r0 + (r + e) * (32u / OUTS), c)), "h"(v[e]) : "memory");
+        }
+    }
+    __device__ __forceinline__ void store_elements(uint32_t j0) const {
+        const uint32_t c = lane & (OUTS - 1u), r0 = lane / OUTS;
+        const int32_t left = (int32_t)a.M - (int32_t)(m_base + r0);
+        const bool in = j0 + c < a.n_out;
+        uint16_t* dst = a.ep.y + (size_t)(m_base + r0) * a.ep.y_stride + j0 + c;
+        const size_t step = (size_t)(32u / OUTS) * a.ep.y_stride;
+#pragma unroll
+        for (uint32_t r = 0; r < OUTS; r += 8u) {
+            uint16_t v[8];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e)
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v[e]) : "r"(element(r0 + (r + e) * (32u / OUTS), c)) : "memory");
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) {
+                if (in && (int32_t)((r + e) * (32u / OUTS)) < left) *dst = v[e];
+                dst += step;
+            }
         }
     }
     __device__ __forceinline__ void store(uint32_t j0) const {
@@ -235,12 +284,7 @@ struct ChunkIO {
                 }
             }
         } else {
-            const uint32_t c = lane & (OUTS - 1u);
-            for (uint32_t r = lane / OUTS; r < 32u; r += 32u / OUTS) {
-                uint16_t v;
-                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(element(r, c)) : "memory");
-                if (m_base + r < a.M && j0 + c < a.n_out) a.ep.y[(size_t)(m_base + r) * a.ep.y_stride + j0 + c] = v;
-            }
+            store_elements(j0);
         }
     }
     // v: the 32 finished accumulators of this lane's row, columns n .. n + 31 (tile column c); col_s: staged scales, biases
@@ -371,113 +415,8 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     volatile int* abortp = &abort_flag;
     pdl_wait();
 
-    if (warp == EPI) {
-        if (lane == 0) {
-            // -------------------------------------------------- producer of A (bf16: A and B)
-            bool ok = true;
-            uint32_t it = 0;
-            for (uint32_t t = cid; t < a.tiles && ok; t += clusters) {
-                uint32_t mt, nt;
-                tile_of(a, t, mt, nt);
-                const int32_t m0 = (int32_t)((mt * CG + sub) * 128u), n0 = (int32_t)(nt * BN + sub * G::BROWS);
-                for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-                    const uint32_t s = it % STAGES;
-                    if (it >= STAGES) ok = tile_wait(empty(s), ((it / STAGES) - 1u) & 1u, abortp, a.status);
-                    if (!ok) break;
-                    if (leader) mbar_expect_tx(full(s), CG * (G::A + (WB == 2 ? G::B : 0u)));
-                    const uint32_t bar = CG == 2 ? map_to_rank(full(s), lead) : full(s);
-                    tile_load<CG>(sA + s * G::A, &map_x, bar, (int32_t)(kb * kBK), m0);
-                    if constexpr (WB == 2) tile_load<CG>(sB + s * G::B, &map_w, bar, (int32_t)(kb * kBK), n0);
-                }
-            }
-        }
-    } else if (warp == EPI + 1u) {
-        if (lane == 0 && leader) {
-            // -------------------------------------------------- MMA issuer
-            const uint16_t pair = (uint16_t)(CG == 2 ? 3u << lead : 1u);
-            bool ok = true;
-            uint32_t it = 0, i = 0;
-            for (uint32_t t = cid; t < a.tiles && ok; t += clusters, ++i) {
-                const uint32_t b = i % bufs;
-                if (i >= bufs) ok = tile_wait(acc_empty(b), ((i / bufs) - 1u) & 1u, abortp, a.status);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-                    const uint32_t s = it % STAGES;
-                    ok = tile_wait(full(s), (it / STAGES) & 1u, abortp, a.status);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t da = make_desc(sA + s * G::A), db = make_desc(sB + s * G::B);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        tile_mma<CG>(tmem + b * G::COLS, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), IDESC, (kb > kb0 || k > 0) ? 1u : 0u);
-                    tile_commit<CG>(empty(s), pair);
-                }
-                if (ok) tile_commit<CG>(acc_full(b), pair);
-            }
-        }
-    } else if (warp == EPI + 2u) {
-        if constexpr (WB == 1) if (lane == 0) {
-            // -------------------------------------------------- producer of raw weight tiles
-            bool ok = true;
-            uint32_t it = 0;
-            for (uint32_t t = cid; t < a.tiles && ok; t += clusters) {
-                uint32_t mt, nt;
-                tile_of(a, t, mt, nt);
-                const int32_t n0 = (int32_t)(nt * BN + sub * G::BROWS);
-                for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-                    const uint32_t r = it % RAWS;
-                    if (it >= RAWS) ok = tile_wait(raw_empty(r), ((it / RAWS) - 1u) & 1u, abortp, a.status);
-                    if (!ok) break;
-                    mbar_expect_tx(raw_full(r), G::RAW);
-                    tma_load_2d(sRaw + r * G::RAW, &map_w, raw_full(r), (int32_t)(kb * kBK), n0);
-                }
-            }
-        }
-    } else if (warp >= EPI + 4u) {
-        // ------------------------------------------------------ e4m3 -> bf16
-        if constexpr (WB == 1) {
-        constexpr uint32_t R = RAWS;
-        const uint32_t group = (warp - (EPI + 4u)) / CONV_WARPS, ct = tid & (CONV_WARPS * 32u - 1u);
-        const uint32_t my_tiles = cid < a.tiles ? (a.tiles - cid + clusters - 1u) / clusters : 0u, total = my_tiles * (kb1 - kb0);
-        bool ok = true;
-        for (uint32_t it = group; it < total && ok; it += 2u) {
-            const uint32_t r = it % R, s = it % STAGES;
-            ok = tile_wait(raw_full(r), (it / R) & 1u, abortp, a.status);
-            if (ok && it >= STAGES) ok = tile_wait(empty(s), ((it / STAGES) - 1u) & 1u, abortp, a.status);
-            if (!ok) break;
-            // 16-byte raw chunks: 8 rows of one chunk column per quarter warp; every load ahead of the first store
-            constexpr uint32_t PER = G::BROWS * 4u / (CONV_WARPS * 32u);
-            uint4 raw[PER];
-            const uint32_t row0 = (ct & 7u) | ((ct >> 5) << 3), cc = (ct >> 3) & 3u;
-#pragma unroll
-            for (uint32_t i = 0; i < PER; ++i) raw[i] = lds16(sRaw + r * G::RAW + (row0 + 32u * i) * kBK + cc * 16u);
-#pragma unroll
-            for (uint32_t i = 0; i < PER; ++i) {
-                const uint32_t row = row0 + 32u * i;
-                const uint4 v = raw[i];
-                const uint32_t two120 = 0x7B807B80u;                      // 2^120 as bf16x2
-                uint32_t o[8];
-                o[0] = e4m3x2_to_bf16x2_scaled<0x1404u>(v.x); o[1] = e4m3x2_to_bf16x2_scaled<0x3424u>(v.x);
-                o[2] = e4m3x2_to_bf16x2_scaled<0x1404u>(v.y); o[3] = e4m3x2_to_bf16x2_scaled<0x3424u>(v.y);
-                o[4] = e4m3x2_to_bf16x2_scaled<0x1404u>(v.z); o[5] = e4m3x2_to_bf16x2_scaled<0x3424u>(v.z);
-                o[6] = e4m3x2_to_bf16x2_scaled<0x1404u>(v.w); o[7] = e4m3x2_to_bf16x2_scaled<0x3424u>(v.w);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(o[j]) : "r"(two120));   // exact
-                sts16(sB + s * G::B + swz(row, 2u * cc), make_uint4(o[0], o[1], o[2], o[3]));
-                sts16(sB + s * G::B + swz(row, 2u * cc + 1u), make_uint4(o[4], o[5], o[6], o[7]));
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-                if (CG == 2) arrive_remote(map_to_rank(full(s), lead));
-                else mbar_arrive(full(s));
-                mbar_arrive(raw_empty(r));
-            }
-        }
-        }
-    }
     if (warp < EPI) {
+        if constexpr (WB == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
         // ------------------------------------------------------ epilogue
         constexpr uint32_t GROUPS = EPI / 4u;
         const uint32_t q = warp & 3u, group = warp >> 2;
@@ -569,11 +508,123 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         };
         if (a.ep.gated) run(std::true_type{});
         else run(std::false_type{});
-    } else if (S > 1u) {
-        // the other warps pass the two barriers of the exchange
-        __syncwarp();
-        cluster_sync();
-        cluster_sync();
+    } else {
+        if (warp < EPI + 4u) {
+            if constexpr (WB == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+            if (warp == EPI) {
+                if (lane == 0) {
+                    // -------------------------------------------------- producer of A (bf16: A and B)
+                    bool ok = true;
+                    uint32_t it = 0;
+                    for (uint32_t t = cid; t < a.tiles && ok; t += clusters) {
+                        uint32_t mt, nt;
+                        tile_of(a, t, mt, nt);
+                        const int32_t m0 = (int32_t)((mt * CG + sub) * 128u), n0 = (int32_t)(nt * BN + sub * G::BROWS);
+                        for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
+                            const uint32_t s = it % STAGES;
+                            if (it >= STAGES) ok = tile_wait(empty(s), ((it / STAGES) - 1u) & 1u, abortp, a.status);
+                            if (!ok) break;
+                            if (leader) mbar_expect_tx(full(s), CG * (G::A + (WB == 2 ? G::B : 0u)));
+                            const uint32_t bar = CG == 2 ? map_to_rank(full(s), lead) : full(s);
+                            tile_load<CG>(sA + s * G::A, &map_x, bar, (int32_t)(kb * kBK), m0);
+                            if constexpr (WB == 2) tile_load<CG>(sB + s * G::B, &map_w, bar, (int32_t)(kb * kBK), n0);
+                        }
+                    }
+                    // the last arrivals of the MMAs on this CTA's stages: none is under way when the CTA leaves
+                    for (uint32_t u = it < STAGES ? 0u : it - STAGES; u < it && ok; ++u) ok = tile_wait(empty(u % STAGES), (u / STAGES) & 1u, abortp, a.status);
+                }
+            } else if (warp == EPI + 1u) {
+                if (lane == 0 && leader) {
+                    // -------------------------------------------------- MMA issuer
+                    const uint16_t pair = (uint16_t)(CG == 2 ? 3u << lead : 1u);
+                    bool ok = true;
+                    uint32_t it = 0, i = 0;
+                    for (uint32_t t = cid; t < a.tiles && ok; t += clusters, ++i) {
+                        const uint32_t b = i % bufs;
+                        if (i >= bufs) ok = tile_wait(acc_empty(b), ((i / bufs) - 1u) & 1u, abortp, a.status);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
+                            const uint32_t s = it % STAGES;
+                            ok = tile_wait(full(s), (it / STAGES) & 1u, abortp, a.status);
+                            if (!ok) break;
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                            const uint64_t da = make_desc(sA + s * G::A), db = make_desc(sB + s * G::B);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                tile_mma<CG>(tmem + b * G::COLS, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), IDESC, (kb > kb0 || k > 0) ? 1u : 0u);
+                            tile_commit<CG>(empty(s), pair);
+                        }
+                        if (ok) tile_commit<CG>(acc_full(b), pair);
+                    }
+                }
+            } else if (warp == EPI + 2u) {
+                if constexpr (WB == 1) if (lane == 0) {
+                    // -------------------------------------------------- producer of raw weight tiles
+                    bool ok = true;
+                    uint32_t it = 0;
+                    for (uint32_t t = cid; t < a.tiles && ok; t += clusters) {
+                        uint32_t mt, nt;
+                        tile_of(a, t, mt, nt);
+                        const int32_t n0 = (int32_t)(nt * BN + sub * G::BROWS);
+                        for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
+                            const uint32_t r = it % RAWS;
+                            if (it >= RAWS) ok = tile_wait(raw_empty(r), ((it / RAWS) - 1u) & 1u, abortp, a.status);
+                            if (!ok) break;
+                            mbar_expect_tx(raw_full(r), G::RAW);
+                            tma_load_2d(sRaw + r * G::RAW, &map_w, raw_full(r), (int32_t)(kb * kBK), n0);
+                        }
+                    }
+                }
+            }
+        } else {
+            // -------------------------------------------------- e4m3 -> bf16
+            if constexpr (WB == 1) {
+                asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+                constexpr uint32_t R = RAWS;
+                const uint32_t group = (warp - (EPI + 4u)) / CONV_WARPS, ct = tid & (CONV_WARPS * 32u - 1u);
+                const uint32_t my_tiles = cid < a.tiles ? (a.tiles - cid + clusters - 1u) / clusters : 0u, total = my_tiles * (kb1 - kb0);
+                bool ok = true;
+                for (uint32_t it = group; it < total && ok; it += 2u) {
+                    const uint32_t r = it % R, s = it % STAGES;
+                    ok = tile_wait(raw_full(r), (it / R) & 1u, abortp, a.status);
+                    if (!ok) break;
+                    // 16-byte raw chunks, eight lanes on 128 consecutive bytes; widened in registers before the stage is free
+                    constexpr uint32_t PER = G::BROWS / 32u;
+                    const uint32_t row0 = ct >> 2, cc = ct & 3u;
+                    uint4 wide[PER][2];
+#pragma unroll
+                    for (uint32_t i = 0; i < PER; ++i) wide[i][0] = lds16(sRaw + r * G::RAW + (row0 + 32u * i) * kBK + cc * 16u);
+#pragma unroll
+                    for (uint32_t i = 0; i < PER; ++i) {
+                        const uint4 v = wide[i][0];
+                        widen4(v.x, wide[i][0].x, wide[i][0].y); widen4(v.y, wide[i][0].z, wide[i][0].w);
+                        widen4(v.z, wide[i][1].x, wide[i][1].y); widen4(v.w, wide[i][1].z, wide[i][1].w);
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(raw_empty(r));
+                    if (it >= STAGES) ok = tile_wait(empty(s), ((it / STAGES) - 1u) & 1u, abortp, a.status);
+                    if (!ok) break;
+#pragma unroll
+                    for (uint32_t i = 0; i < PER; ++i) {
+                        sts16(sB + s * G::B + swz(row0 + 32u * i, 2u * cc), wide[i][0]);
+                        sts16(sB + s * G::B + swz(row0 + 32u * i, 2u * cc + 1u), wide[i][1]);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (CG == 2) arrive_remote(map_to_rank(full(s), lead));
+                        else mbar_arrive(full(s));
+                    }
+                }
+            }
+        }
+        if (S > 1u) {
+            // these warps pass the two barriers of the exchange
+            __syncwarp();
+            cluster_sync();
+            cluster_sync();
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -647,6 +698,7 @@ mc_status_t linear_tile(int wb, const void* w, const uint16_t* x, uint32_t x_pit
                         const EpiArgs& ep, cudaStream_t stream, bool pdl) {
     TilePlan p = tile_plan(wb, M, N, K, (uint32_t)sm_count());
     if (const uint32_t f = g_forced.load(); f != 0u) p = {f >> 24, f & 0xFFFFu, (f >> 16) & 0xFFu};
+    if (wb == 1 && p.cg == 1u && p.bn == 256u) p.bn = 128u;      // one CTA cannot widen 256 rows and keep two stages of them
     const uint32_t blocks = (K + kBK - 1) / kBK;
     while (p.splits > 1u && (p.splits > blocks || p.bn / p.splits < 32u || p.cg * p.splits > 8u)) p.splits >>= 1;   // a slice is never empty
     TileArgs a{};
@@ -663,7 +715,6 @@ mc_status_t linear_tile(int wb, const void* w, const uint16_t* x, uint32_t x_pit
         case 21064: return launch_tile<2, 1, 64>(w, x, x_pitch, K, a, stream, pdl);
         case 12256: return launch_tile<1, 2, 256>(w, x, x_pitch, K, a, stream, pdl);
         case 12128: return launch_tile<1, 2, 128>(w, x, x_pitch, K, a, stream, pdl);
-        case 11256: return launch_tile<1, 1, 256>(w, x, x_pitch, K, a, stream, pdl);
         case 11128: return launch_tile<1, 1, 128>(w, x, x_pitch, K, a, stream, pdl);
         case 11064: return launch_tile<1, 1, 64>(w, x, x_pitch, K, a, stream, pdl);
         default: set_error("linear_tile: no kernel for plan %u", key); return MC_E_INTERNAL;
