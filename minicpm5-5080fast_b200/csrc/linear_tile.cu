@@ -23,6 +23,9 @@ namespace {
 
 constexpr uint32_t kBK = 64;                                   // K elements per stage
 constexpr uint32_t kRing = 196608;                             // bytes of the rings
+constexpr uint32_t kResBuf = 2048;                             // an epilogue warp's residual chunk stands behind its output chunk
+constexpr uint32_t kWarpBuf = 4096;
+constexpr uint32_t kTileNapNs = 1000000u;                      // a poll may sleep this long; spinning warps take issue slots from working ones
 constexpr unsigned long long kTileWaitNs = 200ull * 1000ull * 1000ull;
 
 __device__ int g_tile_error;
@@ -39,8 +42,8 @@ template <int WB, int CG, int BN> struct TileGeom {
     // 2 x 128 x 136 (epilogue) + 128 x 48 (producers, MMA) + 2 x 128 x 80 (widening) = 640 x 96, what the CTA was launched with.
     static constexpr uint32_t THREADS = 32u * (EPI + (WB == 1 ? 12u : 2u));
     static constexpr uint32_t COLS = BN;                       // TMEM columns of one accumulator
-    // rings, output staging (2 KB per epilogue warp), bias and scale of two tiles, alignment
-    static constexpr uint32_t SMEM = kRing + EPI * 2048u + 2u * 2u * BN * 4u + 1024u;
+    // rings, output and residual chunks of the epilogue warps, scale (fp32) and bias (bf16) of a tile, alignment
+    static constexpr uint32_t SMEM = kRing + EPI * kWarpBuf + BN * 6u + 1024u;
 };
 
 struct TileArgs {
@@ -67,12 +70,12 @@ __device__ __forceinline__ bool tile_wait(uint32_t bar, uint32_t parity, volatil
         uint32_t done;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+            : "=r"(done) : "r"(bar), "r"(parity), "r"(kTileNapNs) : "memory");
         if (done) return true;
         if (*abort_flag) return false;
-        if ((spin & 63u) == 63u) {
+        if ((spin & 15u) == 15u) {
             const unsigned long long now = global_timer_ns();
             if (t0 == 0) t0 = now;
             else if (now - t0 > kTileWaitNs) break;
@@ -181,7 +184,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 
 // One warp's 32 rows x 32 accumulator columns -> 32 (behind the gate 16) outputs a row.  A lane holds one row while values
 // are computed, and 16-byte pieces of consecutive columns, several rows apart, while they cross global memory; a 2 KB buffer
-// turns one into the other (pieces swizzled by row: neither side meets a bank twice).
+// turns one into the other (pieces swizzled by row: neither side meets a bank twice).  The residual comes the other way.
 template <bool GATED>
 struct ChunkIO {
     static constexpr uint32_t LG = GATED ? 1u : 2u, PIECES = 1u << LG, OUTS = 8u * PIECES, ROWS = 32u >> LG, ROW_BYTES = 2u * OUTS;
@@ -205,26 +208,16 @@ struct ChunkIO {
     __device__ __forceinline__ uint32_t own_piece(uint32_t k) const { return own + ((k ^ own_swz) << 4); }
     __device__ __forceinline__ uint32_t element(uint32_t row, uint32_t c) const { return buf + row * ROW_BYTES + (((c >> 3) ^ swizzle(row)) << 4) + (c & 7u) * 2u; }
 
-    __device__ __forceinline__ void fetch_res(uint32_t j0, uint4 (&rr)[4]) const {          // aligned rows: ahead of use
+    // Aligned rows, ahead of use and without registers; beyond the edges zeros, which are not stored.
+    __device__ __forceinline__ void fetch_res(uint32_t j0) const {
+        const uint32_t bytes = j0 + col + 8u <= a.n_out ? 16u : (j0 + col < a.n_out ? 2u * (a.n_out - j0 - col) : 0u);
 #pragma unroll
         for (uint32_t i = 0; i < PIECES; ++i) {
-            rr[i] = make_uint4(0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u);         // -0 changes no sum
-            const uint16_t* src = res + (size_t)(i * ROWS) * a.ep.res_stride + j0;
-            if ((int32_t)(i * ROWS) < rows_left) {
-                if (j0 + col + 8u <= a.n_out) rr[i] = *reinterpret_cast<const uint4*>(src);
-                else if (j0 + col < a.n_out) {
-                    uint32_t w[4] = {rr[i].x, rr[i].y, rr[i].z, rr[i].w};
-#pragma unroll
-                    for (uint32_t e = 0; e < 7; ++e)
-                        if (j0 + col + e < a.n_out) w[e >> 1] = (e & 1) ? (w[e >> 1] & 0xFFFFu) | ((uint32_t)src[e] << 16) : (w[e >> 1] & 0xFFFF0000u) | src[e];
-                    rr[i] = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            }
+            const bool in = (int32_t)(i * ROWS) < rows_left && bytes != 0u;
+            const uint16_t* src = in ? res + (size_t)(i * ROWS) * a.ep.res_stride + j0 : a.ep.res;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(across + kResBuf + i * 512u), "l"(src), "r"(in ? bytes : 0u) : "memory");
         }
-    }
-    __device__ __forceinline__ void put_res(const uint4 (&rr)[4]) const {
-#pragma unroll
-        for (uint32_t i = 0; i < PIECES; ++i) sts16(across + i * 512u, rr[i]);
+        asm volatile("cp.async.commit_group;" ::: "memory");
     }
     // Rows at any address: a lane holds one column of every row (gated: of every second row); eight rows in flight.
     __device__ __forceinline__ void res_elements(uint32_t j0) const {
@@ -243,7 +236,7 @@ struct ChunkIO {
             }
 #pragma unroll
             for (uint32_t e = 0; e < 8; ++e)
-                asm volatile("st.shared.u16 [%0], %1;" ::"r"(element(r0 + (r + e) * (32u / OUTS), c)), "h"(v[e]) : "memory");
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(kResBuf + element(r0 + (r + e) * (32u / OUTS), c)), "h"(v[e]) : "memory");
         }
     }
     __device__ __forceinline__ void store_elements(uint32_t j0) const {
@@ -289,21 +282,10 @@ struct ChunkIO {
     }
     // v: the 32 finished accumulators of this lane's row, columns n .. n + 31 (tile column c); col_s: staged scales, biases
     template <uint32_t BN>
-    __device__ __forceinline__ void finish(float (&v)[32], uint32_t n, uint32_t c, uint32_t col_s, bool has_scale, bool has_bias, uint4 (&rr)[4],
-                                           uint32_t next_n) const {
+    __device__ __forceinline__ void finish(float (&v)[32], uint32_t n, uint32_t c, uint32_t col_s, bool has_scale, bool has_bias, uint32_t next_n) const {
         const uint32_t j0 = GATED ? n >> 1 : n;
         const bool has_res = a.ep.res != nullptr;
-        uint4 mine[PIECES];
-        if (has_res) {
-            if (a.res_vec) {
-                put_res(rr);
-                if (next_n != 0xFFFFFFFFu) fetch_res(GATED ? next_n >> 1 : next_n, rr);
-            } else res_elements(j0);
-            __syncwarp();
-#pragma unroll
-            for (uint32_t k = 0; k < PIECES; ++k) mine[k] = lds16(own_piece(k));
-            __syncwarp();
-        }
+        if (has_res && !a.res_vec) res_elements(j0);
         if (has_scale) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
@@ -313,9 +295,11 @@ struct ChunkIO {
         }
         if (has_bias) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float4 f = lds_f4(col_s + (BN + c + 4u * k) * 4u);
-                v[4 * k] += f.x; v[4 * k + 1] += f.y; v[4 * k + 2] += f.z; v[4 * k + 3] += f.w;
+            for (int k = 0; k < 4; ++k) {
+                const uint4 f = lds16(col_s + BN * 4u + (c + 8u * k) * 2u);
+                const uint32_t p[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { v[8 * k + 2 * e] += bf16lo(p[e]); v[8 * k + 2 * e + 1] += bf16hi(p[e]); }
             }
         }
         const uint32_t act = a.ep.act;
@@ -335,9 +319,12 @@ struct ChunkIO {
         else if (act == MC_SM100_ACT_RELU) apply([](float z) { return epi_act(z, MC_SM100_ACT_RELU); });
         else if (GATED) apply([](float z) { return z; });
         if (has_res) {
+            if (a.res_vec) asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncwarp();
 #pragma unroll
             for (uint32_t k = 0; k < PIECES; ++k) {
-                const uint32_t r[4] = {mine[k].x, mine[k].y, mine[k].z, mine[k].w};
+                const uint4 m = lds16(own_piece(k) + kResBuf);
+                const uint32_t r[4] = {m.x, m.y, m.z, m.w};
 #pragma unroll
                 for (uint32_t e = 0; e < 4; ++e) { v[8 * k + 2 * e] += bf16lo(r[e]); v[8 * k + 2 * e + 1] += bf16hi(r[e]); }
             }
@@ -346,7 +333,8 @@ struct ChunkIO {
         for (uint32_t k = 0; k < PIECES; ++k)
             sts16(own_piece(k), make_uint4(pack_bf16(v[8 * k], v[8 * k + 1]), pack_bf16(v[8 * k + 2], v[8 * k + 3]),
                                            pack_bf16(v[8 * k + 4], v[8 * k + 5]), pack_bf16(v[8 * k + 6], v[8 * k + 7])));
-        __syncwarp();
+        __syncwarp();                                                  // pieces written, residual read
+        if (has_res && a.res_vec && next_n != 0xFFFFFFFFu) fetch_res(GATED ? next_n >> 1 : next_n);
         store(j0);
         __syncwarp();
     }
@@ -371,7 +359,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t sA = base, sB = base + STAGES * G::A, sRaw = sB + STAGES * G::B;
-    const uint32_t sBuf = base + kRing, sCol = sBuf + EPI * 2048u;
+    const uint32_t sBuf = base + kRing, sCol = sBuf + EPI * kWarpBuf;
     const uint32_t bar0 = smem_u32(bars);
     auto full = [&](uint32_t s) { return bar0 + 8u * s; };
     auto empty = [&](uint32_t s) { return bar0 + 8u * (8u + s); };
@@ -425,28 +413,38 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             using IO = ChunkIO<decltype(gated)::value>;
             bool ok = true;
             uint32_t i = 0;
+            // scale and bias of this thread's column of a tile
+            static_assert(BN <= (int)(EPI * 32u), "one column per epilogue thread");
+            float my_scale = 1.f;
+            uint16_t my_bias = 0;
+            auto load_column = [&](uint32_t t) {
+                if (t >= a.tiles || tid >= BN) return;
+                uint32_t mt, nt;
+                tile_of(a, t, mt, nt);
+                const uint32_t n = nt * BN + tid;
+                if (n >= a.N) return;
+                if (has_scale) my_scale = a.ep.scale[n];
+                if (has_bias) my_bias = a.ep.bias[n];
+            };
+            if (has_scale || has_bias) load_column(cid);
             for (uint32_t t = cid; t < a.tiles; t += clusters, ++i) {
                 uint32_t mt, nt;
                 tile_of(a, t, mt, nt);
                 const uint32_t b = i % bufs, n0 = nt * BN;
-                const IO io(a, sBuf + warp * 2048u, lane, (mt * CG + sub) * 128u + q * 32u);
-                // scale and bias of the tile's features, in the half of the staging area that the previous tile does not read
-                const uint32_t col_s = sCol + (i & 1u) * (2u * BN * 4u);
+                const IO io(a, sBuf + warp * kWarpBuf, lane, (mt * CG + sub) * 128u + q * 32u);
                 if (has_scale || has_bias) {
-                    for (uint32_t c = tid; c < BN; c += EPI * 32u) {
-                        const uint32_t n = n0 + c;
-                        const float sc = has_scale && n < a.N ? a.ep.scale[n] : 1.f;
-                        const float bi = has_bias && n < a.N ? __uint_as_float((uint32_t)a.ep.bias[n] << 16) : 0.f;
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(col_s + c * 4u), "f"(sc) : "memory");
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(col_s + (BN + c) * 4u), "f"(bi) : "memory");
+                    asm volatile("bar.sync 1, %0;" ::"n"(EPI * 32u) : "memory");     // the previous tile's have been read
+                    if (tid < BN) {
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(sCol + tid * 4u), "f"(my_scale) : "memory");
+                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(sCol + BN * 4u + tid * 2u), "h"(my_bias) : "memory");
                     }
+                    load_column(t + clusters);                                       // of the next tile, under this one's work
                     asm volatile("bar.sync 1, %0;" ::"n"(EPI * 32u) : "memory");
                 }
                 // this CTA finishes columns [c_lo, c_hi), this warp every GROUPS-th chunk of them
                 const uint32_t per = BN / S, c_lo = split * per, c_hi = n0 + c_lo + per <= a.N ? c_lo + per : (a.N - n0 > c_lo ? a.N - n0 : c_lo);
                 const uint32_t c_first = c_lo + group * 32u;
-                uint4 rr[4];
-                if (a.ep.res != nullptr && a.res_vec && c_first < c_hi) io.fetch_res((n0 + c_first) >> a.ep.gated, rr);
+                if (a.ep.res != nullptr && a.res_vec && c_first < c_hi) io.fetch_res((n0 + c_first) >> a.ep.gated);
                 if (ok) ok = tile_wait(acc_full(b), (i / bufs) & 1u, abortp, a.status);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t taddr = tmem + b * G::COLS + ((q * 32u) << 16);
@@ -483,26 +481,17 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     tmem_ld32(taddr + c, v);
                     if (S == 1u && last) release();
                     if (S > 1u) {
-                        float sum[32];
+                        // this CTA's own part first, then the others in split order
+                        for (uint32_t src = 0; src + 1u < S; ++src) {
+                            const uint32_t at = base + (src * 128u + row) * per * 4u;
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) sum[k] = 0.f;
-                        for (uint32_t p = 0; p < S; ++p) {                           // split order
-                            if (p == split) {
-#pragma unroll
-                                for (int k = 0; k < 32; ++k) sum[k] += v[k];
-                            } else {
-                                const uint32_t src = p < split ? p : p - 1u, at = base + (src * 128u + row) * per * 4u;
-#pragma unroll
-                                for (int k = 0; k < 8; ++k) {
-                                    const float4 f = lds_f4(at + (((((c - c_lo) >> 2) + k) ^ (row & 7u)) << 4));
-                                    sum[4 * k] += f.x; sum[4 * k + 1] += f.y; sum[4 * k + 2] += f.z; sum[4 * k + 3] += f.w;
-                                }
+                            for (int k = 0; k < 8; ++k) {
+                                const float4 f = lds_f4(at + (((((c - c_lo) >> 2) + k) ^ (row & 7u)) << 4));
+                                v[4 * k] += f.x; v[4 * k + 1] += f.y; v[4 * k + 2] += f.z; v[4 * k + 3] += f.w;
                             }
                         }
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) v[k] = sum[k];
                     }
-                    if (!failed) io.template finish<BN>(v, n0 + c, c, col_s, has_scale, has_bias, rr, last ? 0xFFFFFFFFu : n0 + c + 32u * GROUPS);
+                    if (!failed) io.template finish<BN>(v, n0 + c, c, sCol, has_scale, has_bias, last ? 0xFFFFFFFFu : n0 + c + 32u * GROUPS);
                 }
             }
         };
