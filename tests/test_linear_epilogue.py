@@ -52,6 +52,19 @@ def test_refusals(pkg):
     assert lib.mc_sm100_linear_epilogue(16, None, 16, 16, 1, 8, 8, C.cast(C.byref(ep), C.c_void_p), None, 0) == pkg.MC_E_INVALID_ARGUMENT
 
 
+def test_tile_plan(pkg):
+    """Host logic: every choice is a plan the kernel has, slices are never empty, big calls take the widest tile whole."""
+    for wb in (1, 2):
+        assert pkg.debug_tile_plan(wb, 8192, 11520, 2304) == (2, 256, 1)
+        assert pkg.debug_tile_plan(wb, 128, 2304, 5760)[2] > 1
+        for M in (65, 129, 500, 4000, 1 << 20):
+            for N in (1, 63, 2304, 122753):
+                for K in (8, 64, 65, 2304, 30000):
+                    cg, bn, s = pkg.debug_tile_plan(wb, M, N, K)
+                    assert (cg, bn) in ((1, 64), (1, 128), (2, 128), (2, 256)) and s in (1, 2, 4) and s <= -(-K // 64) and bn // s >= 32 and cg * s <= 8
+        assert pkg.debug_tile_plan(wb, 300, 300, 300, 1)[0] in (1, 2)
+
+
 # ---- GPU -------------------------------------------------------------------------------------------------------------
 def _make(M, N, K, e4m3, bias, residual, gated, seed):
     n_out = N // 2 if gated else N
@@ -105,7 +118,7 @@ SHAPES = [(1, 1, 1), (1, 2, 7), (2, 31, 16), (3, 130, 24), (5, 96, 72), (1, 2304
           (129, 514, 136), (200, 1026, 1040), (255, 30, 48), (256, 512, 512), (301, 770, 2304), (513, 258, 72), (1030, 130, 80)]
 
 
-PLANS = [(1, 64, 1), (1, 64, 2), (1, 128, 1), (1, 128, 2), (1, 128, 4), (1, 256, 1), (1, 256, 8), (2, 128, 1), (2, 128, 2), (2, 128, 4), (2, 256, 1), (2, 256, 4)]
+PLANS = [(1, 64, 1), (1, 64, 2), (1, 128, 1), (1, 128, 2), (1, 128, 4), (2, 128, 1), (2, 128, 2), (2, 128, 4), (2, 256, 1), (2, 256, 2), (2, 256, 4)]
 
 
 @pytest.mark.gpu
