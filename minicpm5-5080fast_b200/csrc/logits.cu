@@ -17,36 +17,44 @@ struct LogitsArgs {
 };
 
 // A CTA owns kSpan consecutive columns of a row (counted from a 16-byte boundary of the output, so that rows of any length
-// and stride are stored in 16-byte pieces but for their ends), a thread one piece of eight.  What costs is reading and
-// writing the logits, 4 bytes a token; seen bits and mask are 1/16 of that, and the counts are gathered for seen tokens only.
-// The bias list is read once per CTA, 256 entries at a time: those that fall into the span are kept in list order in shared
-// memory, and each thread adds up the ones of its own tokens: a fixed order, no atomics, any list length.
-constexpr uint32_t kPiece = 8, kSpan = kLogitsThreads * kPiece;
-
-struct BiasEntry { uint32_t column; float value; };
+// and stride are stored in 16-byte pieces but for their ends), a thread two pieces of eight.  Reading and writing the logits
+// is 4 bytes a token; seen bits and masks are 1/16 of that, and counts are gathered for seen tokens only.  At full batches the
+// instructions bound it, not the bytes (64 rows of 122753 with every rule: 36 us with all tokens through the fp32 path): most
+// tokens are neither seen nor listed and stay the bits that they are, a mask is a select on the packed words.
+// Biases: the entries that fall into the span are kept in list order in shared memory; the thread of a token's first entry
+// adds up the others behind it: a fixed order, no floating-point atomics, any list length (512 entries at a time).
+constexpr uint32_t kPiece = 8, kPieces = 2, kSpan = kLogitsThreads * kPiece * kPieces, kBiasBatch = 2 * kLogitsThreads;
 
 __global__ void __launch_bounds__(kLogitsThreads) logits_process_kernel(const LogitsArgs a) {
-    __shared__ BiasEntry s_bias[kLogitsThreads];
-    __shared__ uint32_t s_warp[kLogitsThreads / 32];
+    __shared__ uint32_t s_column[kBiasBatch];
+    __shared__ float s_value[kBiasBatch], s_sum[kSpan];
+    __shared__ uint32_t s_listed[kSpan / 32], s_warp[kBiasBatch / 32];
     const uint32_t row = blockIdx.y, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     pdl_trigger();
     pdl_wait();
     const mc_sm100_logits_config_t c = a.cfg[row];
     const uint16_t* in = a.in + (size_t)row * a.row_stride;
     uint16_t* out = a.out + (size_t)row * a.out_stride;
-    // columns [first, first + 8) of this thread; those below 0 or beyond the row are not there
-    const uint32_t head = (uint32_t)((reinterpret_cast<uintptr_t>(out) & 15u) >> 1);
-    const int32_t first = (int32_t)(blockIdx.x * kSpan + tid * kPiece) - (int32_t)head;
-    const int32_t lo = first < 0 ? 0 : first, hi = first + (int32_t)kPiece < (int32_t)a.vocab ? first + (int32_t)kPiece : (int32_t)a.vocab;
-    const bool whole = hi - lo == (int32_t)kPiece;
-    uint32_t raw[4] = {0u, 0u, 0u, 0u};
-    if (whole && ((reinterpret_cast<uintptr_t>(in + first)) & 15u) == 0u) {
-        const uint4 v = *reinterpret_cast<const uint4*>(in + first);
-        raw[0] = v.x; raw[1] = v.y; raw[2] = v.z; raw[3] = v.w;
-    } else {
+    // piece p: columns first[p] .. + 7; those below 0 or beyond the row are not there
+    const int32_t head = (int32_t)((reinterpret_cast<uintptr_t>(out) & 15u) >> 1), vocab = (int32_t)a.vocab;
+    const int32_t span0 = (int32_t)(blockIdx.x * kSpan) - head;
+    int32_t first[kPieces];
+    uint32_t raw[kPieces][4];
+    const bool together = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0u;
 #pragma unroll
-        for (int e = 0; e < (int)kPiece; ++e)
-            if (first + e >= lo && first + e < hi) raw[e >> 1] |= (uint32_t)in[first + e] << (16 * (e & 1));
+    for (uint32_t p = 0; p < kPieces; ++p) {
+        first[p] = span0 + (int32_t)((p * kLogitsThreads + tid) * kPiece);
+        const int32_t f = first[p];
+        if (together && f >= 0 && f + (int32_t)kPiece <= vocab) {
+            const uint4 v = *reinterpret_cast<const uint4*>(in + f);
+            raw[p][0] = v.x; raw[p][1] = v.y; raw[p][2] = v.z; raw[p][3] = v.w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) raw[p][k] = 0u;
+#pragma unroll
+            for (int e = 0; e < (int)kPiece; ++e)
+                if (f + e >= 0 && f + e < vocab) raw[p][e >> 1] |= (uint32_t)in[f + e] << (16 * (e & 1));
+        }
     }
     const uint32_t words = (a.t.table_vocab + 31u) / 32u;
     const bool history = c.history_slot >= 0 && (uint32_t)c.history_slot < a.t.n_slots;
@@ -55,69 +63,120 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_process_kernel(const Lo
     if (a.t.d_status != nullptr && blockIdx.x == 0u && tid == 0u &&
         ((c.history_slot >= 0 && !history) || (c.mask_row >= 0 && !masked) || (c.bias_count != 0u && end64 > a.t.n_bias)))
         *a.t.d_status = 1;
-    // the eight bits of a table row that belong to columns lo .. hi - 1, bit e = column first + e
-    auto bits_of = [&](const uint32_t* table_row) -> uint32_t {
+    // the bits of a table row that belong to a piece, bit e = column first + e, 0 where there is none
+    auto bits_of = [&](const uint32_t* table_row, int32_t f) -> uint32_t {
+        const int32_t lo = f < 0 ? 0 : f, hi = f + (int32_t)kPiece < vocab ? f + (int32_t)kPiece : vocab;
         if (hi <= lo) return 0u;
-        const uint32_t t0 = (uint32_t)a.index_base + (uint32_t)lo, t1 = (uint32_t)a.index_base + (uint32_t)hi - 1u;
-        const uint32_t w0 = table_row[t0 >> 5], w1 = (t1 >> 5) != (t0 >> 5) ? table_row[t1 >> 5] : 0u;
-        return (__funnelshift_r(w0, w1, t0 & 31u) & ((1u << (hi - lo)) - 1u)) << (lo - first);
+        const uint32_t t0 = (uint32_t)(a.index_base + lo), t1 = (uint32_t)(a.index_base + hi - 1);
+        const uint32_t w0 = table_row[t0 >> 5], w1 = table_row[t1 >> 5];
+        return (__funnelshift_r(w0, w1, t0 & 31u) & ((1u << (hi - lo)) - 1u)) << (lo - f);
     };
-    const uint32_t seen = history ? bits_of(a.t.d_seen + (size_t)c.history_slot * words) : 0u;
-    const uint32_t allowed = masked ? bits_of(a.t.d_mask + (size_t)c.mask_row * words) : 0xFFu;
-
-    float bias[kPiece];
-    uint32_t listed = 0u;
+    uint32_t seen[kPieces], allowed[kPieces], listed[kPieces];
+#pragma unroll
+    for (uint32_t p = 0; p < kPieces; ++p) {
+        seen[p] = history ? bits_of(a.t.d_seen + (size_t)c.history_slot * words, first[p]) : 0u;
+        allowed[p] = masked ? bits_of(a.t.d_mask + (size_t)c.mask_row * words, first[p]) : 0xFFu;
+        listed[p] = 0u;
+    }
     const uint64_t end = end64 < a.t.n_bias ? end64 : a.t.n_bias;
-    for (uint64_t j0 = c.bias_begin; j0 < end; j0 += kLogitsThreads) {               // the same for every thread
-        const int32_t span0 = (int32_t)(blockIdx.x * kSpan) - (int32_t)head;
-        uint32_t col = 0xFFFFFFFFu;
-        float value = 0.f;
-        if (j0 + tid < end) {
-            const int64_t column = (int64_t)a.t.d_bias_token[j0 + tid] - a.index_base;
-            if (column >= 0 && column < (int64_t)a.vocab && column >= span0 && column < (int64_t)span0 + kSpan) {
-                col = (uint32_t)(column - span0);
-                value = a.t.d_bias_value[j0 + tid];
-            }
-        }
-        const uint32_t hits = __ballot_sync(0xFFFFFFFFu, col != 0xFFFFFFFFu);
-        if (lane == 0) s_warp[warp] = __popc(hits);
-        __syncthreads();
-        uint32_t before = 0u, total = 0u;
+    if (c.bias_begin < end) {                                                        // the same for every thread
+        const int32_t lo = span0 < 0 ? 0 : span0, hi = span0 + (int32_t)kSpan < vocab ? span0 + (int32_t)kSpan : vocab;
+        if (tid < kSpan / 32) s_listed[tid] = 0u;
+        for (uint64_t j0 = c.bias_begin; j0 < end; j0 += kBiasBatch) {
+            uint32_t col[2], hits[2];
+            float value[2];
 #pragma unroll
-        for (uint32_t w = 0; w < kLogitsThreads / 32; ++w) { const uint32_t n = s_warp[w]; before += w < warp ? n : 0u; total += n; }
-        if (col != 0xFFFFFFFFu) s_bias[before + __popc(hits & ((1u << lane) - 1u))] = BiasEntry{col, value};
-        __syncthreads();
-        for (uint32_t k = 0; k < total; ++k) {
-            const BiasEntry b = s_bias[k];
-            if ((b.column / kPiece) == tid) {
-#pragma unroll
-                for (uint32_t e = 0; e < kPiece; ++e)
-                    if ((b.column & (kPiece - 1u)) == e) { bias[e] = (listed >> e) & 1u ? __fadd_rn(bias[e], b.value) : __fadd_rn(0.f, b.value); listed |= 1u << e; }
+            for (int h = 0; h < 2; ++h) {
+                const uint64_t j = j0 + h * kLogitsThreads + tid;
+                int32_t column = -1;
+                value[h] = 0.f;
+                // tokens and index_base are not negative, or the difference is: no overflow
+                if (j < end) { const int32_t tok = a.t.d_bias_token[j]; column = tok < 0 ? -1 : tok - a.index_base; value[h] = a.t.d_bias_value[j]; }
+                col[h] = column >= lo && column < hi ? (uint32_t)(column - span0) : 0xFFFFFFFFu;
             }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                hits[h] = __ballot_sync(0xFFFFFFFFu, col[h] != 0xFFFFFFFFu);
+                if (lane == 0) s_warp[h * (kLogitsThreads / 32) + warp] = __popc(hits[h]);
+            }
+            __syncthreads();
+            constexpr uint32_t kCounts = kBiasBatch / 32;
+            uint32_t upto = lane < kCounts ? s_warp[lane] : 0u;
+#pragma unroll
+            for (uint32_t d = 1; d < kCounts; d <<= 1) {
+                const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+                if (lane >= d) upto += v;
+            }
+            const uint32_t total = __shfl_sync(0xFFFFFFFFu, upto, kCounts - 1u);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t at = h * (kLogitsThreads / 32) + warp, before = __shfl_sync(0xFFFFFFFFu, upto, at) - __popc(hits[h]);
+                if (col[h] != 0xFFFFFFFFu) {
+                    const uint32_t k = before + __popc(hits[h] & ((1u << lane) - 1u));
+                    s_column[k] = col[h]; s_value[k] = value[h];
+                }
+            }
+            __syncthreads();
+            for (uint32_t k = tid; k < total; k += kLogitsThreads) {
+                const uint32_t mine = s_column[k];
+                bool earlier = false;
+                for (uint32_t o = 0; o < k && !earlier; ++o) earlier = s_column[o] == mine;
+                if (earlier) continue;                                               // the thread of that entry adds this one
+                const bool known = (s_listed[mine >> 5] >> (mine & 31u)) & 1u;       // from an earlier batch
+                float sum = __fadd_rn(known ? s_sum[mine] : 0.f, s_value[k]);
+                for (uint32_t o = k + 1u; o < total; ++o)
+                    if (s_column[o] == mine) sum = __fadd_rn(sum, s_value[o]);
+                s_sum[mine] = sum;
+                atomicOr(&s_listed[mine >> 5], 1u << (mine & 31u));
+            }
+            __syncthreads();
         }
-        __syncthreads();
+#pragma unroll
+        for (uint32_t p = 0; p < kPieces; ++p) {
+            const uint32_t at = (p * kLogitsThreads + tid) * kPiece;
+            listed[p] = (s_listed[at >> 5] >> (at & 31u)) & 0xFFu;
+        }
     }
     const bool repeat = c.rep_penalty != 1.f && c.rep_penalty != 0.f;
     const int32_t* counts = history ? a.t.d_counts + (size_t)c.history_slot * a.t.table_vocab + a.index_base : nullptr;
-    uint32_t res[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int e = 0; e < (int)kPiece; ++e) {
-        float l = (e & 1) ? bf16hi(raw[e >> 1]) : bf16lo(raw[e >> 1]);
-        if ((seen >> e) & 1u) {
-            if (repeat) l = l > 0.f ? __fdiv_rn(l, c.rep_penalty) : __fmul_rn(l, c.rep_penalty);
-            const int32_t n = counts[first + e];
-            if (n > 0) l = __fsub_rn(__fsub_rn(l, __fmul_rn(c.freq_penalty, (float)n)), c.pres_penalty);
+    for (uint32_t p = 0; p < kPieces; ++p) {
+        const int32_t f = first[p];
+        uint32_t res[4] = {raw[p][0], raw[p][1], raw[p][2], raw[p][3]};
+        // a banned token's value does not matter any more
+        const uint32_t s = seen[p] & allowed[p], b = listed[p] & allowed[p];
+        if ((s | b) != 0u) {
+            int32_t n_of[kPiece];
+#pragma unroll
+            for (int e = 0; e < (int)kPiece; ++e) n_of[e] = (s >> e) & 1u ? counts[f + e] : 0;
+#pragma unroll
+            for (int e = 0; e < (int)kPiece; ++e) {
+                if (((s | b) >> e) & 1u) {
+                    float l = (e & 1) ? bf16hi(res[e >> 1]) : bf16lo(res[e >> 1]);
+                    if (repeat && ((s >> e) & 1u)) l = l > 0.f ? __fdiv_rn(l, c.rep_penalty) : __fmul_rn(l, c.rep_penalty);
+                    if (n_of[e] > 0) l = __fsub_rn(__fsub_rn(l, __fmul_rn(c.freq_penalty, (float)n_of[e])), c.pres_penalty);
+                    if ((b >> e) & 1u) l = __fadd_rn(l, s_sum[(p * kLogitsThreads + tid) * kPiece + e]);
+                    const uint32_t bits = f32_to_bf16_bits(l);
+                    res[e >> 1] = (e & 1) ? (res[e >> 1] & 0xFFFFu) | (bits << 16) : (res[e >> 1] & 0xFFFF0000u) | bits;
+                }
+            }
         }
-        if ((listed >> e) & 1u) l = __fadd_rn(l, bias[e]);
-        if (!((allowed >> e) & 1u)) l = -INFINITY;
-        res[e >> 1] |= (uint32_t)f32_to_bf16_bits(l) << (16 * (e & 1));
-    }
-    if (in == out && res[0] == raw[0] && res[1] == raw[1] && res[2] == raw[2] && res[3] == raw[3]) return;   // in place, nothing to say
-    if (whole) *reinterpret_cast<uint4*>(out + first) = make_uint4(res[0], res[1], res[2], res[3]);
-    else {
+        if (masked) {
 #pragma unroll
-        for (int e = 0; e < (int)kPiece; ++e)
-            if (first + e >= lo && first + e < hi) out[first + e] = (uint16_t)(res[e >> 1] >> (16 * (e & 1)));
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t keep = ((allowed[p] >> (2 * k)) & 1u) * 0xFFFFu + ((allowed[p] >> (2 * k + 1)) & 1u) * 0xFFFF0000u;
+                res[k] = (res[k] & keep) | (0xFF80FF80u & ~keep);                    // -infinity
+            }
+        }
+        if (f >= 0 && f + (int32_t)kPiece <= vocab) {
+            // in place, a piece that stays as it was is not written
+            if (in != out || res[0] != raw[p][0] || res[1] != raw[p][1] || res[2] != raw[p][2] || res[3] != raw[p][3])
+                *reinterpret_cast<uint4*>(out + f) = make_uint4(res[0], res[1], res[2], res[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < (int)kPiece; ++e)
+                if (f + e >= 0 && f + e < vocab) out[f + e] = (uint16_t)(res[e >> 1] >> (16 * (e & 1)));
+        }
     }
 }
 
@@ -159,37 +218,42 @@ __global__ void __launch_bounds__(kHistThreads) history_rebuild_kernel(const His
     uint32_t slot, lo, hi;
     if (!history_seq(a, seq, slot, lo, hi)) return;
     for (uint32_t i = tid; i < span; i += kHistThreads) s_count[i] = 0u;
-    auto same_slot = [&](uint32_t other) {
-        uint32_t s, l, h;
-        return other < n_seqs && history_seq(a, other, s, l, h) && s == slot;
-    };
-    if (a.slots != nullptr) {
-        bool taken = false;
-        for (uint32_t j = tid; j < seq; j += kHistThreads) taken = taken || same_slot(j);
-        if (__syncthreads_or(taken ? 1 : 0)) return;
-    } else {
-        __syncthreads();
-    }
     const uint32_t t0 = blockIdx.y * span, t1 = min(a.vocab, t0 + span);
-    auto add = [&](uint32_t which) {
-        uint32_t s, l, h;
-        (void)history_seq(a, which, s, l, h);
+    auto add = [&](uint32_t which, uint32_t l, uint32_t h) {
         const uint32_t n = h - l, prompt = a.prompt_len != nullptr ? a.prompt_len[which] : 0u;
-        for (uint32_t k = tid; k < n; k += kHistThreads) {
-            const uint32_t tok = (uint32_t)a.tokens[l + k];
-            if (tok < t0 || tok >= t1) continue;
-            if (k < prompt) atomicOr(s_count + (tok - t0), 0x80000000u);
-            else atomicAdd(s_count + (tok - t0), 1u);
+        const int32_t* src = a.tokens + l;
+        for (uint32_t k0 = tid; k0 < n; k0 += kHistThreads * 8u) {
+            uint32_t tok[8];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) tok[e] = k0 + e * kHistThreads < n ? (uint32_t)src[k0 + e * kHistThreads] : 0xFFFFFFFFu;
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) {
+                if (tok[e] < t0 || tok[e] >= t1) continue;
+                if (k0 + e * kHistThreads < prompt) atomicOr(s_count + (tok[e] - t0), 0x80000000u);
+                else atomicAdd(s_count + (tok[e] - t0), 1u);
+            }
         }
     };
-    add(seq);
-    if (a.slots != nullptr) {
-        for (uint32_t j0 = seq + 1u; j0 < n_seqs; j0 += kHistThreads) {
-            const uint32_t hits = __ballot_sync(0xFFFFFFFFu, same_slot(j0 + tid));
+    if (a.slots == nullptr) {
+        __syncthreads();
+        add(seq, lo, hi);
+    } else {
+        // one look over the sequences: does an earlier one own the slot, which later ones join
+        bool counted = false;
+        for (uint32_t j0 = 0; j0 < n_seqs; j0 += kHistThreads) {
+            const uint32_t j = j0 + tid;
+            uint32_t s, l, h;
+            const bool same = j != seq && j < n_seqs && history_seq(a, j, s, l, h) && s == slot;
+            const uint32_t hits = __ballot_sync(0xFFFFFFFFu, same);
             if (lane == 0) s_same[warp] = hits;
-            __syncthreads();
+            if (__syncthreads_or(same && j < seq ? 1 : 0)) return;
+            if (!counted && j0 + kHistThreads > seq) { add(seq, lo, hi); counted = true; }
             for (uint32_t w = 0; w < kHistThreads / 32u; ++w)
-                for (uint32_t m = s_same[w]; m != 0u; m &= m - 1u) add(j0 + w * 32u + (uint32_t)__ffs((int)m) - 1u);
+                for (uint32_t m = s_same[w]; m != 0u; m &= m - 1u) {
+                    const uint32_t other = j0 + w * 32u + (uint32_t)__ffs((int)m) - 1u;
+                    (void)history_seq(a, other, s, l, h);
+                    add(other, l, h);
+                }
             __syncthreads();
         }
     }
