@@ -393,7 +393,7 @@ MC_SM100_API mc_status_t mc_sm100_sample_topk_topp_sharded(
 /* What a row's request asks of its logits; read by the kernel at run time from a fixed device address, so that a
  * captured step can be replayed with other values.  All zero except history_slot = mask_row = -1 leaves a row as it is. */
 typedef struct mc_sm100_logits_config_t {
-    float    rep_penalty;            /* tokens the history has seen: l > 0 ? l / rep : l * rep; 1 (or 0) = off */
+    float    rep_penalty;            /* tokens the history has seen: l > 0 ? l * (1 / rep) : l * rep; 1 (or 0) = off */
     float    freq_penalty;           /* l -= freq * (how often the token was generated) */
     float    pres_penalty;           /* l -= pres if the token was generated at all */
     int32_t  history_slot;           /* row of counts / seen, < 0 = no history: the three above do nothing

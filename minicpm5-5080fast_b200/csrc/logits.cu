@@ -26,9 +26,10 @@ struct LogitsArgs {
 constexpr uint32_t kPiece = 8, kPieces = 2, kSpan = kLogitsThreads * kPiece * kPieces, kBiasBatch = 2 * kLogitsThreads;
 
 __global__ void __launch_bounds__(kLogitsThreads) logits_process_kernel(const LogitsArgs a) {
-    __shared__ uint32_t s_column[kBiasBatch];
-    __shared__ float s_value[kBiasBatch], s_sum[kSpan];
-    __shared__ uint32_t s_listed[kSpan / 32], s_warp[kBiasBatch / 32];
+    __shared__ __align__(16) uint32_t s_column[kBiasBatch + 4];
+    __shared__ __align__(16) float s_sum[kSpan];
+    __shared__ float s_value[kBiasBatch];
+    __shared__ uint32_t s_listed[kSpan / 32], s_once[kSpan / 32], s_again[kSpan / 32], s_warp[kBiasBatch / 32];
     const uint32_t row = blockIdx.y, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     pdl_trigger();
     pdl_wait();
@@ -81,7 +82,7 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_process_kernel(const Lo
     const uint64_t end = end64 < a.t.n_bias ? end64 : a.t.n_bias;
     if (c.bias_begin < end) {                                                        // the same for every thread
         const int32_t lo = span0 < 0 ? 0 : span0, hi = span0 + (int32_t)kSpan < vocab ? span0 + (int32_t)kSpan : vocab;
-        if (tid < kSpan / 32) s_listed[tid] = 0u;
+        for (uint32_t w = tid; w < kSpan / 32; w += kLogitsThreads) s_listed[w] = 0u;
         for (uint64_t j0 = c.bias_begin; j0 < end; j0 += kBiasBatch) {
             uint32_t col[2], hits[2];
             float value[2];
@@ -117,17 +118,32 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_process_kernel(const Lo
                 }
             }
             __syncthreads();
-            for (uint32_t k = tid; k < total; k += kLogitsThreads) {
-                const uint32_t mine = s_column[k];
-                bool earlier = false;
-                for (uint32_t o = 0; o < k && !earlier; ++o) earlier = s_column[o] == mine;
-                if (earlier) continue;                                               // the thread of that entry adds this one
-                const bool known = (s_listed[mine >> 5] >> (mine & 31u)) & 1u;       // from an earlier batch
-                float sum = __fadd_rn(known ? s_sum[mine] : 0.f, s_value[k]);
-                for (uint32_t o = k + 1u; o < total; ++o)
-                    if (s_column[o] == mine) sum = __fadd_rn(sum, s_value[o]);
-                s_sum[mine] = sum;
-                atomicOr(&s_listed[mine >> 5], 1u << (mine & 31u));
+            if (total != 0u) {                                                       // the same for every thread
+                for (uint32_t w = tid; w < kSpan / 32; w += kLogitsThreads) s_once[w] = s_again[w] = 0u;
+                if (tid < 4u) s_column[total + tid] = 0xFFFFFFFFu;                   // the walk reads four at a time
+                __syncthreads();
+                for (uint32_t k = tid; k < total; k += kLogitsThreads) {
+                    const uint32_t mine = s_column[k], bit = 1u << (mine & 31u);
+                    if (atomicOr(&s_once[mine >> 5], bit) & bit) atomicOr(&s_again[mine >> 5], bit);
+                }
+                __syncthreads();
+                for (uint32_t k = tid; k < total; k += kLogitsThreads) {
+                    const uint32_t mine = s_column[k], bit = 1u << (mine & 31u);
+                    float sum = s_listed[mine >> 5] & bit ? s_sum[mine] : 0.f;       // from the batches before
+                    bool owner = true;
+                    if (s_again[mine >> 5] & bit) {                                  // the first of its entries adds them up in order
+                        for (uint32_t o = 0; o < total; o += 4u) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(s_column + o);
+                            const uint32_t cols[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; ++e)
+                                if (cols[e] == mine) { if (o + e < k) owner = false; sum = __fadd_rn(sum, s_value[o + e]); }
+                        }
+                    } else sum = __fadd_rn(sum, s_value[k]);
+                    if (owner) s_sum[mine] = sum;
+                }
+                __syncthreads();
+                for (uint32_t w = tid; w < kSpan / 32; w += kLogitsThreads) s_listed[w] |= s_once[w];
             }
             __syncthreads();
         }
@@ -137,7 +153,8 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_process_kernel(const Lo
             listed[p] = (s_listed[at >> 5] >> (at & 31u)) & 0xFFu;
         }
     }
-    const bool repeat = c.rep_penalty != 1.f && c.rep_penalty != 0.f;
+    // one reciprocal a row instead of a division a token: off by 2^-24 of the value, in front of a rounding of 2^-9
+    const float grow = c.rep_penalty != 0.f ? c.rep_penalty : 1.f, shrink = __frcp_rn(grow);
     const int32_t* counts = history ? a.t.d_counts + (size_t)c.history_slot * a.t.table_vocab + a.index_base : nullptr;
 #pragma unroll
     for (uint32_t p = 0; p < kPieces; ++p) {
@@ -146,19 +163,23 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_process_kernel(const Lo
         // a banned token's value does not matter any more
         const uint32_t s = seen[p] & allowed[p], b = listed[p] & allowed[p];
         if ((s | b) != 0u) {
+            // no branch per token: the eight chains run side by side
             int32_t n_of[kPiece];
+            float add[kPiece];
 #pragma unroll
             for (int e = 0; e < (int)kPiece; ++e) n_of[e] = (s >> e) & 1u ? counts[f + e] : 0;
+            const float4 b0 = *reinterpret_cast<const float4*>(s_sum + (p * kLogitsThreads + tid) * kPiece);
+            const float4 b1 = *reinterpret_cast<const float4*>(s_sum + (p * kLogitsThreads + tid) * kPiece + 4);
+            add[0] = b0.x; add[1] = b0.y; add[2] = b0.z; add[3] = b0.w; add[4] = b1.x; add[5] = b1.y; add[6] = b1.z; add[7] = b1.w;
 #pragma unroll
             for (int e = 0; e < (int)kPiece; ++e) {
-                if (((s | b) >> e) & 1u) {
-                    float l = (e & 1) ? bf16hi(res[e >> 1]) : bf16lo(res[e >> 1]);
-                    if (repeat && ((s >> e) & 1u)) l = l > 0.f ? __fdiv_rn(l, c.rep_penalty) : __fmul_rn(l, c.rep_penalty);
-                    if (n_of[e] > 0) l = __fsub_rn(__fsub_rn(l, __fmul_rn(c.freq_penalty, (float)n_of[e])), c.pres_penalty);
-                    if ((b >> e) & 1u) l = __fadd_rn(l, s_sum[(p * kLogitsThreads + tid) * kPiece + e]);
-                    const uint32_t bits = f32_to_bf16_bits(l);
-                    res[e >> 1] = (e & 1) ? (res[e >> 1] & 0xFFFFu) | (bits << 16) : (res[e >> 1] & 0xFFFF0000u) | bits;
-                }
+                const uint32_t old = (e & 1) ? res[e >> 1] >> 16 : res[e >> 1] & 0xFFFFu;
+                float l = __uint_as_float(old << 16);
+                l = (s >> e) & 1u ? __fmul_rn(l, l > 0.f ? shrink : grow) : l;
+                l = n_of[e] > 0 ? __fsub_rn(__fsub_rn(l, __fmul_rn(c.freq_penalty, (float)n_of[e])), c.pres_penalty) : l;
+                l = (b >> e) & 1u ? __fadd_rn(l, add[e]) : l;
+                const uint32_t bits = ((s | b) >> e) & 1u ? f32_to_bf16_bits(l) : old;
+                res[e >> 1] = (e & 1) ? (res[e >> 1] & 0xFFFFu) | (bits << 16) : (res[e >> 1] & 0xFFFF0000u) | bits;
             }
         }
         if (masked) {
@@ -203,22 +224,27 @@ __device__ __forceinline__ bool history_seq(const HistoryArgs& a, uint32_t seq, 
     return ok;
 }
 
-// Rebuild: a CTA owns `span` tokens of the vocabulary of one slot.  It counts in shared memory (bit 31: seen in the prompt)
-// over the slot's tokens and writes each count and seen bit once: no clearing pass, no global atomics, one launch; the token
+// Rebuild: a CTA owns `span` tokens of the vocabulary of one slot.  It counts in shared memory over the slot's tokens and
+// writes each count and seen bit once: no clearing pass, no global atomics, one launch; the token
 // list is read once per span (from L2 after the first).  Of several sequences that name a slot the first owns it and the
 // others add to its counts.
 constexpr uint32_t kHistThreads = 512;
 
 __global__ void __launch_bounds__(kHistThreads) history_rebuild_kernel(const HistoryArgs a, uint32_t n_seqs, uint32_t span) {
-    extern __shared__ uint32_t s_count[];
+    extern __shared__ __align__(16) int32_t s_hist[];            // [span + 4] counts, [span / 32] seen bits
     __shared__ uint32_t s_same[kHistThreads / 32];
     pdl_trigger();
     pdl_wait();
     const uint32_t seq = blockIdx.x, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     uint32_t slot, lo, hi;
     if (!history_seq(a, seq, slot, lo, hi)) return;
-    for (uint32_t i = tid; i < span; i += kHistThreads) s_count[i] = 0u;
     const uint32_t t0 = blockIdx.y * span, t1 = min(a.vocab, t0 + span);
+    // counts stand in shared memory as far from a 16-byte boundary as in the table: rows of any length go out 16 bytes at a time
+    int32_t* row = a.counts + (size_t)slot * a.vocab + t0;
+    const uint32_t shift = (uint32_t)((reinterpret_cast<uintptr_t>(row) & 15u) >> 2);
+    int32_t* s_count = s_hist + shift;
+    uint32_t* s_seen = reinterpret_cast<uint32_t*>(s_hist + span + 4u);
+    for (uint32_t i = tid; i < (span + 4u + span / 32u + 3u) / 4u; i += kHistThreads) reinterpret_cast<uint4*>(s_hist)[i] = make_uint4(0u, 0u, 0u, 0u);
     auto add = [&](uint32_t which, uint32_t l, uint32_t h) {
         const uint32_t n = h - l, prompt = a.prompt_len != nullptr ? a.prompt_len[which] : 0u;
         const int32_t* src = a.tokens + l;
@@ -229,8 +255,9 @@ __global__ void __launch_bounds__(kHistThreads) history_rebuild_kernel(const His
 #pragma unroll
             for (uint32_t e = 0; e < 8; ++e) {
                 if (tok[e] < t0 || tok[e] >= t1) continue;
-                if (k0 + e * kHistThreads < prompt) atomicOr(s_count + (tok[e] - t0), 0x80000000u);
-                else atomicAdd(s_count + (tok[e] - t0), 1u);
+                const uint32_t t = tok[e] - t0;
+                atomicOr(s_seen + t / 32u, 1u << (t & 31u));
+                if (k0 + e * kHistThreads >= prompt) atomicAdd(s_count + t, 1);
             }
         }
     };
@@ -259,12 +286,20 @@ __global__ void __launch_bounds__(kHistThreads) history_rebuild_kernel(const His
     }
     __syncthreads();
     const uint32_t words = (a.vocab + 31u) / 32u;
-    for (uint32_t i = tid; t0 + (i & ~31u) < t1; i += kHistThreads) {              // whole warps stay together: span % 32 = 0
-        const uint32_t c = t0 + i < t1 ? s_count[i] : 0u;
-        if (t0 + i < t1) a.counts[(size_t)slot * a.vocab + t0 + i] = (int32_t)(c & 0x7FFFFFFFu);
-        const uint32_t bits = __ballot_sync(0xFFFFFFFFu, c != 0u);
-        if (lane == 0) a.seen[(size_t)slot * words + (t0 + i) / 32u] = bits;
+    const uint32_t n = t1 - t0, upto = shift + n;                 // shared entries [shift, upto) are the table's
+    int32_t* table = row - shift;
+    for (uint32_t i = tid * 4u; i < upto; i += kHistThreads * 4u) {
+        const int4 v = *reinterpret_cast<const int4*>(s_hist + i);
+        if (i >= shift && i + 4u <= upto) {
+            *reinterpret_cast<int4*>(table + i) = v;
+        } else {
+            const int32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k)
+                if (i + k >= shift && i + k < upto) table[i + k] = e[k];
+        }
     }
+    for (uint32_t i = tid; i < (n + 31u) / 32u; i += kHistThreads) a.seen[(size_t)slot * words + t0 / 32u + i] = s_seen[i];
 }
 
 // Append: integer atomics, whose order does not show in the result.
@@ -331,13 +366,14 @@ mc_status_t mc_sm100_token_history(int32_t* d_counts, uint32_t* d_seen, uint32_t
         const uint64_t spans = (2ull * (uint32_t)sm_count() + n_seqs - 1u) / n_seqs;
         uint64_t span = ((uint64_t)table_vocab + spans - 1u) / spans;
         span = span < 2048u ? 2048u : (span > 16384u ? 16384u : (span + 31u) & ~(uint64_t)31u);
+        const size_t bytes = ((size_t)span + 4u) * 4u + (size_t)span / 8u + 16u;
         static SmemOptIn optin;
-        const cudaError_t e = optin.ensure(history_rebuild_kernel, span * 4u);
+        const cudaError_t e = optin.ensure(history_rebuild_kernel, bytes);
         if (e != cudaSuccess) {
-            set_error("mc_sm100_token_history: cannot raise shared memory to %u: %s", (uint32_t)span * 4u, cudaGetErrorString(e));
+            set_error("mc_sm100_token_history: cannot raise shared memory to %zu: %s", bytes, cudaGetErrorString(e));
             return MC_E_CUDA;
         }
-        (void)launch(history_rebuild_kernel, dim3(n_seqs, (uint32_t)((table_vocab + span - 1u) / span)), dim3(kHistThreads), (size_t)span * 4u,
+        (void)launch(history_rebuild_kernel, dim3(n_seqs, (uint32_t)((table_vocab + span - 1u) / span)), dim3(kHistThreads), bytes,
                      (cudaStream_t)stream, pdl != 0, a, n_seqs, (uint32_t)span);
         MCL_CHECK_LAUNCH("history_rebuild");
         return MC_OK;

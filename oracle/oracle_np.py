@@ -346,7 +346,7 @@ def logits_process_f32(logits_u16, rules, counts, seen, mask, bias_token, bias_v
         if counts is not None:
             k, c = seen[sl], counts[sl]
             if rep != 1 and rep != 0:
-                l = np.where(k, np.where(l > 0, l / rep, l * rep), l).astype(f)
+                l = np.where(k, np.where(l > 0, l * (f(1) / rep), l * rep), l).astype(f)
             l = np.where(k & (c > 0), (l - freq * c.astype(f)) - pres, l).astype(f)
         add = {}
         for t, v in zip(bias_token, bias_value):
