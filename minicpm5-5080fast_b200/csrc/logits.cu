@@ -19,16 +19,19 @@ struct LogitsArgs {
 // A CTA owns kSpan consecutive columns of a row (counted from a 16-byte boundary of the output, so that rows of any length
 // and stride are stored in 16-byte pieces but for their ends), a thread two pieces of eight.  Reading and writing the logits
 // is 4 bytes a token; seen bits and masks are 1/16 of that, and counts are gathered for seen tokens only.  At full batches the
-// instructions bound it, not the bytes (64 rows of 122753 with every rule: 36 us with all tokens through the fp32 path): most
-// tokens are neither seen nor listed and stay the bits that they are, a mask is a select on the packed words.
+// instructions bound it, not the bytes: most tokens are neither seen nor listed and stay the bits that they are, a mask is a
+// select on the packed words (64 rows of 122753 with every rule: 36 us with every token through the fp32 path, 24.5 us with
+// every piece that holds a touched token, 29.5 us with touched tokens always one a lane; the rule below 23 us, bound by latency
+// and instructions alike).
 // Biases: the entries that fall into the span are kept in list order in shared memory; the thread of a token's first entry
 // adds up the others behind it: a fixed order, no floating-point atomics, any list length (512 entries at a time).
-constexpr uint32_t kPiece = 8, kPieces = 2, kSpan = kLogitsThreads * kPiece * kPieces, kBiasBatch = 2 * kLogitsThreads;
+constexpr uint32_t kPiece = 8, kPieces = 2, kSpan = kLogitsThreads * kPiece * kPieces, kBiasBatch = 2 * kLogitsThreads, kFew = 64;
 
-__global__ void __launch_bounds__(kLogitsThreads) logits_process_kernel(const LogitsArgs a) {
+__global__ void __launch_bounds__(kLogitsThreads, 5) logits_process_kernel(const LogitsArgs a) {
     __shared__ __align__(16) uint32_t s_column[kBiasBatch + 4];
     __shared__ __align__(16) float s_sum[kSpan];
     __shared__ float s_value[kBiasBatch];
+    __shared__ uint2 s_touched[kLogitsThreads / 32][kFew];
     __shared__ uint32_t s_listed[kSpan / 32], s_once[kSpan / 32], s_again[kSpan / 32], s_warp[kBiasBatch / 32];
     const uint32_t row = blockIdx.y, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     pdl_trigger();
@@ -156,29 +159,37 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_process_kernel(const Lo
     // one reciprocal a row instead of a division a token: off by 2^-24 of the value, in front of a rounding of 2^-9
     const float grow = c.rep_penalty != 0.f ? c.rep_penalty : 1.f, shrink = __frcp_rn(grow);
     const int32_t* counts = history ? a.t.d_counts + (size_t)c.history_slot * a.t.table_vocab + a.index_base : nullptr;
+    auto edit = [&](float l, bool was_seen, int32_t n, bool has_bias, float b) {
+        l = was_seen ? __fmul_rn(l, l > 0.f ? shrink : grow) : l;
+        l = n > 0 ? __fsub_rn(__fsub_rn(l, __fmul_rn(c.freq_penalty, (float)n)), c.pres_penalty) : l;
+        return has_bias ? __fadd_rn(l, b) : l;
+    };
+    // a banned token's value does not matter any more
+    uint32_t touched[kPieces];
+#pragma unroll
+    for (uint32_t p = 0; p < kPieces; ++p) touched[p] = (seen[p] | listed[p]) & allowed[p];
+    // Few touched tokens in the warp (nearly everywhere but among a vocabulary's most frequent tokens): every piece goes out
+    // under its mask, then the touched tokens are edited one a lane.  Many: each lane edits its pieces, eight tokens side by side.
+    static_assert(kPieces == 2, "two pieces a thread");
+    const uint32_t mine = __popc(touched[0]) + __popc(touched[1]), total = __reduce_add_sync(0xFFFFFFFFu, mine);
+    const bool few = total <= kFew;
 #pragma unroll
     for (uint32_t p = 0; p < kPieces; ++p) {
         const int32_t f = first[p];
         uint32_t res[4] = {raw[p][0], raw[p][1], raw[p][2], raw[p][3]};
-        // a banned token's value does not matter any more
-        const uint32_t s = seen[p] & allowed[p], b = listed[p] & allowed[p];
-        if ((s | b) != 0u) {
-            // no branch per token: the eight chains run side by side
+        if (!few && touched[p] != 0u) {
             int32_t n_of[kPiece];
             float add[kPiece];
 #pragma unroll
-            for (int e = 0; e < (int)kPiece; ++e) n_of[e] = (s >> e) & 1u ? counts[f + e] : 0;
+            for (int e = 0; e < (int)kPiece; ++e) n_of[e] = ((seen[p] & touched[p]) >> e) & 1u ? counts[f + e] : 0;
             const float4 b0 = *reinterpret_cast<const float4*>(s_sum + (p * kLogitsThreads + tid) * kPiece);
             const float4 b1 = *reinterpret_cast<const float4*>(s_sum + (p * kLogitsThreads + tid) * kPiece + 4);
             add[0] = b0.x; add[1] = b0.y; add[2] = b0.z; add[3] = b0.w; add[4] = b1.x; add[5] = b1.y; add[6] = b1.z; add[7] = b1.w;
 #pragma unroll
             for (int e = 0; e < (int)kPiece; ++e) {
                 const uint32_t old = (e & 1) ? res[e >> 1] >> 16 : res[e >> 1] & 0xFFFFu;
-                float l = __uint_as_float(old << 16);
-                l = (s >> e) & 1u ? __fmul_rn(l, l > 0.f ? shrink : grow) : l;
-                l = n_of[e] > 0 ? __fsub_rn(__fsub_rn(l, __fmul_rn(c.freq_penalty, (float)n_of[e])), c.pres_penalty) : l;
-                l = (b >> e) & 1u ? __fadd_rn(l, add[e]) : l;
-                const uint32_t bits = ((s | b) >> e) & 1u ? f32_to_bf16_bits(l) : old;
+                const float l = edit(__uint_as_float(old << 16), (seen[p] >> e) & 1u, n_of[e], (listed[p] >> e) & 1u, add[e]);
+                const uint32_t bits = (touched[p] >> e) & 1u ? f32_to_bf16_bits(l) : old;
                 res[e >> 1] = (e & 1) ? (res[e >> 1] & 0xFFFFu) | (bits << 16) : (res[e >> 1] & 0xFFFF0000u) | bits;
             }
         }
@@ -198,6 +209,30 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_process_kernel(const Lo
             for (int e = 0; e < (int)kPiece; ++e)
                 if (f + e >= 0 && f + e < vocab) out[f + e] = (uint16_t)(res[e >> 1] >> (16 * (e & 1)));
         }
+    }
+    if (!few || total == 0u) return;
+    uint32_t upto = mine;
+#pragma unroll
+    for (uint32_t d = 1; d < 32; d <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+        if (lane >= d) upto += v;
+    }
+    uint32_t at = upto - mine;
+#pragma unroll
+    for (uint32_t p = 0; p < kPieces; ++p)
+        for (uint32_t t = touched[p]; t != 0u; t &= t - 1u, ++at) {
+            const uint32_t e = (uint32_t)__ffs((int)t) - 1u;
+            const uint32_t value = (e & 1u ? 0xFFFF0000u : 0xFFFFu) & (e < 4u ? (e < 2u ? raw[p][0] : raw[p][1]) : (e < 6u ? raw[p][2] : raw[p][3]));
+            s_touched[warp][at] = make_uint2(((p * kLogitsThreads + tid) * kPiece + e) | (((seen[p] >> e) & 1u) << 30) | (((listed[p] >> e) & 1u) << 31),
+                                             e & 1u ? value : value << 16);
+        }
+    __syncwarp();                                                // the list, and the pieces stored above, are the whole warp's
+    for (uint32_t k = lane; k < total; k += 32u) {
+        const uint2 t = s_touched[warp][k];
+        const uint32_t in_span = t.x & 0x3FFFFFFFu;
+        const int32_t col = span0 + (int32_t)in_span;
+        const bool was_seen = (t.x >> 30) & 1u;
+        out[col] = f32_to_bf16_bits(edit(__uint_as_float(t.y), was_seen, was_seen ? counts[col] : 0, t.x >> 31, s_sum[in_span]));
     }
 }
 
