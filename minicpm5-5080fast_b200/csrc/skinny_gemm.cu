@@ -34,7 +34,7 @@ namespace {
 constexpr int kTileN = 128;        // weight rows per CTA (MMA M)
 constexpr int kThreads = 320;      // 10 warps
 constexpr int kConvThreads = 256;  // warps 2..9
-constexpr uint32_t kConvGroup = 128;  // converter threads that share one K block (two groups; four groups of 64 ran into bounded-wait timeouts and are not used)
+constexpr uint32_t kConvGroup = 128;  // converter threads that share one K block (two groups)
 constexpr unsigned long long kWaitLimitNs = 200ull * 1000ull * 1000ull;   // a wait gives up after 200 ms
 
 __device__ int g_skinny_error;     // set when a bounded wait ran out (read back by tests)
@@ -256,7 +256,10 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         bool ok = true;
         for (uint32_t it = group; it < nloc && ok; it += kConvThreads / kConvGroup) {
             const uint32_t sr = it % RAWS, so = it % OPS;
-            ok = mbar_wait(raw_full(sr), (it / RAWS) & 1u, abortp, a.status);
+            // With an odd ring the other group had this stage last: until it has given the stage back, the barrier below may
+            // still stand a use earlier, and the parity of the use before that one would pass for ours.
+            if (it >= RAWS) ok = mbar_wait(raw_empty(sr), ((it / RAWS) - 1u) & 1u, abortp, a.status);
+            if (ok) ok = mbar_wait(raw_full(sr), (it / RAWS) & 1u, abortp, a.status);
             if (ok && it >= OPS) ok = mbar_wait(op_empty(so), ((it / OPS) - 1u) & 1u, abortp, a.status);
             if (!ok) break;
 #pragma unroll
