@@ -99,15 +99,6 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
-// Four e4m3 codes -> four bf16 of value * 2^-120 (the 7 magnitude bits dropped at bit 4), byte-wise: 7 integer operations
-// where placing pair by pair takes 8; then * 2^120, exact.
-__device__ __forceinline__ void widen4(uint32_t w, uint32_t& p01, uint32_t& p23) {
-    const uint32_t hi = ((w >> 4) & 0x07070707u) | (w & 0x80808080u), lo = (w << 4) & 0xF0F0F0F0u;
-    p01 = __byte_perm(lo, hi, 0x5140u);
-    p23 = __byte_perm(lo, hi, 0x7362u);
-    asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(p01) : "r"(0x7B807B80u));
-    asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(p23) : "r"(0x7B807B80u));
-}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");

@@ -248,11 +248,11 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         }
     } else if constexpr (E4) {
         // ---------------------------------------------------------------- e4m3 -> bf16 widening
-        // thread -> (row, 16-byte raw chunk): a quarter warp covers 8 rows of one chunk column, which
-        // makes the swizzled 16-byte stores of the operand tile bank-conflict free.
+        // thread -> (row, 16-byte raw chunk): a quarter warp covers two whole raw rows, 128 consecutive bytes; its swizzled
+        // 16-byte stores into the operand tile meet no bank twice either.
         // The eight warps work as groups of kConvGroup threads on alternate K blocks, so that several blocks are in
         // the (latency-bound) load -> place bits -> store -> fence chain at any time.
-        const uint32_t ct = (tid - 64u) & (kConvGroup - 1u), group = (tid - 64u) / kConvGroup;
+        const uint32_t ct = (tid - 64u) & (kConvGroup - 1u), group = (tid - 64u) / kConvGroup, row0 = ct >> 2, cc = ct & 3u;
         bool ok = true;
         for (uint32_t it = group; it < nloc && ok; it += kConvThreads / kConvGroup) {
             const uint32_t sr = it % RAWS, so = it % OPS;
@@ -260,31 +260,34 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             // still stand a use earlier, and the parity of the use before that one would pass for ours.
             if (it >= RAWS) ok = mbar_wait(raw_empty(sr), ((it / RAWS) - 1u) & 1u, abortp, a.status);
             if (ok) ok = mbar_wait(raw_full(sr), (it / RAWS) & 1u, abortp, a.status);
-            if (ok && it >= OPS) ok = mbar_wait(op_empty(so), ((it / OPS) - 1u) & 1u, abortp, a.status);
+            if (!ok) break;
+            // every load ahead of the first store, and the codes widened in registers before the operand stage is free
+            constexpr uint32_t PER = 512u / kConvGroup;
+            uint4 wide[PER][2];
+#pragma unroll
+            for (uint32_t i = 0; i < PER; ++i)
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(wide[i][0].x), "=r"(wide[i][0].y), "=r"(wide[i][0].z), "=r"(wide[i][0].w)
+                             : "r"(sRaw + sr * G::A_RAW + (row0 + (kConvGroup / 4u) * i) * 64u + cc * 16u));
+#pragma unroll
+            for (uint32_t i = 0; i < PER; ++i) {
+                const uint4 v = wide[i][0];
+                widen4(v.x, wide[i][0].x, wide[i][0].y); widen4(v.y, wide[i][0].z, wide[i][0].w);
+                widen4(v.z, wide[i][1].x, wide[i][1].y); widen4(v.w, wide[i][1].z, wide[i][1].w);
+            }
+            mbar_arrive(raw_empty(sr));
+            if (it >= OPS) ok = mbar_wait(op_empty(so), ((it / OPS) - 1u) & 1u, abortp, a.status);
             if (!ok) break;
 #pragma unroll
-            for (int i = 0; i < 512 / (int)kConvGroup; ++i) {
-                const uint32_t c = ct + kConvGroup * i;              // 0..511
-                const uint32_t row = (c & 7u) | ((c >> 5) << 3), cc = (c >> 3) & 3u;
-                uint4 v;
-                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                             : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                             : "r"(sRaw + sr * G::A_RAW + row * 64u + cc * 16u));
-                const uint32_t two120 = 0x7B807B80u;                  // 2^120 as bf16x2
-                uint32_t o[8];
-                o[0] = e4m3x2_to_bf16x2_scaled<0x1404u>(v.x); o[1] = e4m3x2_to_bf16x2_scaled<0x3424u>(v.x);
-                o[2] = e4m3x2_to_bf16x2_scaled<0x1404u>(v.y); o[3] = e4m3x2_to_bf16x2_scaled<0x3424u>(v.y);
-                o[4] = e4m3x2_to_bf16x2_scaled<0x1404u>(v.z); o[5] = e4m3x2_to_bf16x2_scaled<0x3424u>(v.z);
-                o[6] = e4m3x2_to_bf16x2_scaled<0x1404u>(v.w); o[7] = e4m3x2_to_bf16x2_scaled<0x3424u>(v.w);
+            for (uint32_t i = 0; i < PER; ++i) {
+                const uint32_t row = row0 + (kConvGroup / 4u) * i;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(o[j]) : "r"(two120));   // exact
-                const uint32_t d0 = sA + so * G::A_OP + swz(row, 2 * cc), d1 = sA + so * G::A_OP + swz(row, 2 * cc + 1);
-                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(d0), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
-                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(d1), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
+                for (uint32_t h = 0; h < 2; ++h)
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(sA + so * G::A_OP + swz(row, 2u * cc + h)),
+                                 "r"(wide[i][h].x), "r"(wide[i][h].y), "r"(wide[i][h].z), "r"(wide[i][h].w) : "memory");
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(conv_done(so));
-            mbar_arrive(raw_empty(sr));
         }
     }
 

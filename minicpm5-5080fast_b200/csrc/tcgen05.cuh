@@ -47,6 +47,16 @@ __device__ __forceinline__ uint64_t make_desc(uint32_t saddr) {
 // swizzled byte offset of 16-byte chunk `cc` (0..7) of tile row `row`
 __device__ __forceinline__ uint32_t swz(uint32_t row, uint32_t cc) { return row * kRowBytes + ((cc ^ (row & 7u)) << 4); }
 
+// Four e4m3 codes -> four bf16 of value * 2^-120 (the 7 magnitude bits dropped at bit 4), byte-wise: 7 integer operations
+// where placing pair by pair takes 8; then * 2^120, exact.
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& p01, uint32_t& p23) {
+    const uint32_t hi = ((w >> 4) & 0x07070707u) | (w & 0x80808080u), lo = (w << 4) & 0xF0F0F0F0u;
+    p01 = __byte_perm(lo, hi, 0x5140u);
+    p23 = __byte_perm(lo, hi, 0x7362u);
+    asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(p01) : "r"(0x7B807B80u));
+    asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(p23) : "r"(0x7B807B80u));
+}
+
 #endif  // __CUDACC__
 
 // Row-major [rows, K] matrix of 1- or 2-byte elements (pitch in elements), box = [box_rows x box_k], out-of-range reads are
