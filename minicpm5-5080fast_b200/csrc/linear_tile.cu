@@ -138,6 +138,12 @@ __device__ __forceinline__ void tile_commit(uint32_t bar, uint16_t pair_mask) {
                      ::"r"(bar), "h"(pair_mask) : "memory");
 }
 
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0u;
+}
+
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
     uint32_t r[32];
     asm volatile(
@@ -514,28 +520,33 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     for (uint32_t u = it < STAGES ? 0u : it - STAGES; u < it && ok; ++u) ok = tile_wait(empty(u % STAGES), (u / STAGES) & 1u, abortp, a.status);
                 }
             } else if (warp == EPI + 1u) {
-                if (lane == 0 && leader) {
-                    // -------------------------------------------------- MMA issuer
+                if (leader) {
+                    // -------------------------------------------------- MMA issuer: the warp together, one lane elected to issue
                     const uint16_t pair = (uint16_t)(CG == 2 ? 3u << lead : 1u);
                     bool ok = true;
-                    uint32_t it = 0, i = 0;
+                    uint32_t it = 0, i = 0, s = 0, par = 0;
                     for (uint32_t t = cid; t < a.tiles && ok; t += clusters, ++i) {
                         const uint32_t b = i % bufs;
                         if (i >= bufs) ok = tile_wait(acc_empty(b), ((i / bufs) - 1u) & 1u, abortp, a.status);
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t acc = tmem + b * G::COLS;
                         for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-                            const uint32_t s = it % STAGES;
-                            ok = tile_wait(full(s), (it / STAGES) & 1u, abortp, a.status);
+                            ok = tile_wait(full(s), par, abortp, a.status);
                             if (!ok) break;
                             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                             const uint64_t da = make_desc(sA + s * G::A), db = make_desc(sB + s * G::B);
+                            if (elect_lane()) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                tile_mma<CG>(tmem + b * G::COLS, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), IDESC, (kb > kb0 || k > 0) ? 1u : 0u);
-                            tile_commit<CG>(empty(s), pair);
+                                for (int k = 0; k < 4; ++k)
+                                    tile_mma<CG>(acc, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), IDESC, (kb > kb0 || k > 0) ? 1u : 0u);
+                                tile_commit<CG>(empty(s), pair);
+                            }
+                            __syncwarp();
+                            if (++s == STAGES) { s = 0; par ^= 1u; }
                         }
-                        if (ok) tile_commit<CG>(acc_full(b), pair);
+                        if (ok && elect_lane()) tile_commit<CG>(acc_full(b), pair);
+                        __syncwarp();
                     }
                 }
             } else if (warp == EPI + 2u) {
