@@ -373,15 +373,36 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint32_t tmem_cols = bufs * BN < 32u ? 32u : bufs * BN;
 
     pdl_trigger();
-    if (tid == 0) {
+    // One CTA per tile: its first stages are asked for before the tensor memory and the other roles are ready (weights before
+    // the previous kernel's end is waited for): -0.5 us a call.  A pair has to know its partner's barriers first, and where K
+    // is split the loop that asks holds up the cluster's first barrier by as much as it gains.
+    const uint32_t nloc = cid < a.tiles ? kb1 - kb0 : 0u;
+    const uint32_t early = CG == 1 && S == 1u ? min(nloc, 4u) : 0u;
+    static_assert(STAGES >= 4u && (WB == 2 || RAWS >= 4u), "the early stages are all the ring's");
+    if (tid == EPI * 32u) {
         abort_flag = 0;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
         for (uint32_t s = 0; s < STAGES; ++s) { mbar_init(full(s), 1u + (WB == 1 ? CONV_WARPS * CG : 0u)); mbar_init(empty(s), 1); }
         if constexpr (WB == 1)
             for (uint32_t s = 0; s < RAWS; ++s) { mbar_init(raw_full(s), 1); mbar_init(raw_empty(s), CONV_WARPS); }
         for (uint32_t b = 0; b < 2; ++b) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), EPI * CG); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+        if constexpr (CG == 1) {
+            uint32_t mt = 0, nt = 0;
+            if (nloc != 0u) tile_of(a, cid, mt, nt);
+            const int32_t m0 = (int32_t)(mt * 128u), n0 = (int32_t)(nt * BN);
+            for (uint32_t it = 0; it < early; ++it) {
+                const uint32_t bar = WB == 1 ? raw_full(it) : full(it);
+                mbar_expect_tx(bar, WB == 1 ? G::RAW : G::A + G::B);
+                tma_load_2d(WB == 1 ? sRaw + it * G::RAW : sB + it * G::B, &map_w, bar, (int32_t)((kb0 + it) * kBK), n0);
+            }
+            pdl_wait();
+            for (uint32_t it = 0; it < early; ++it) {
+                if constexpr (WB == 1) mbar_expect_tx(full(it), G::A);
+                tma_load_2d(sA + it * G::A, &map_x, full(it), (int32_t)((kb0 + it) * kBK), m0);
+            }
+        }
     }
     if (warp == EPI + 1u) {
         if constexpr (CG == 1) {
@@ -394,7 +415,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    cluster_sync();                                              // barriers and TMEM of every CTA are there
+    if (csize > 1u) cluster_sync();                              // barriers and TMEM of every CTA are there
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_slot;
     volatile int* abortp = &abort_flag;
@@ -508,6 +529,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                         const int32_t m0 = (int32_t)((mt * CG + sub) * 128u), n0 = (int32_t)(nt * BN + sub * G::BROWS);
                         for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
                             const uint32_t s = it % STAGES;
+                            if (it < early) continue;
                             if (it >= STAGES) ok = tile_wait(empty(s), ((it / STAGES) - 1u) & 1u, abortp, a.status);
                             if (!ok) break;
                             if (leader) mbar_expect_tx(full(s), CG * (G::A + (WB == 2 ? G::B : 0u)));
@@ -560,6 +582,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                         const int32_t n0 = (int32_t)(nt * BN + sub * G::BROWS);
                         for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
                             const uint32_t r = it % RAWS;
+                            if (it < early) continue;
                             if (it >= RAWS) ok = tile_wait(raw_empty(r), ((it / RAWS) - 1u) & 1u, abortp, a.status);
                             if (!ok) break;
                             mbar_expect_tx(raw_full(r), G::RAW);
@@ -623,7 +646,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         const unsigned long long t0 = global_timer_ns();
         while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
     }
-    cluster_sync();                                              // nobody addresses a CTA that has left
+    if (csize > 1u) cluster_sync();                              // nobody addresses a CTA that has left
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (warp == EPI + 1u) {
         if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");
