@@ -147,7 +147,12 @@ extern "C" mc_status_t mc_sm100_linear_epilogue(const void* d_w, const float* d_
         return launch_fast_fused(wb, d.gated != 0u, a, st, pdl != 0);
     }
     const bool tma = unit && (xs & 7u) == 0u;
-    if (M <= 64u && tma) return skinny_gemm_fused(wb == 2 ? SKINNY_W_BF16 : SKINNY_W_E4M3, d_w, d_x, xs, M, N, K, e, st, pdl != 0);
+    // Up to 64 rows the skinny kernel, which splits K eight ways and pads M to 16, 32 or 64.  From 33 rows on the tiled kernel
+    // is faster where K is short (M = 62, 480 x 448: 5.7 against 9.1 us) or the weights have many rows (M = 33, lm_head
+    // 122753 x 2304: 95 against 115 us; M = 64, 11520 x 2304: 15.1 against 19.3), slower elsewhere (M = 64, 2304 x 5760: 16.7
+    // against 14.2; M = 48, 20000 x 4096: 43.9 against 41.8).
+    const bool tiled = M > 64u || tile_forced() || (M > 32u && (K <= 768u || (N >= 4096u && K <= 3000u)));
+    if (!tiled && tma) return skinny_gemm_fused(wb == 2 ? SKINNY_W_BF16 : SKINNY_W_E4M3, d_w, d_x, xs, M, N, K, e, st, pdl != 0);
     if (tma) return linear_tile(wb, d_w, d_x, xs, M, N, K, e, st, pdl != 0);
     return linear_any(wb, d_w, d_x, xs, M, N, K, e, st, pdl != 0);
 }

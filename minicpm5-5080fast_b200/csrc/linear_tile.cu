@@ -702,18 +702,18 @@ mc_status_t launch_tile(const void* w, const uint16_t* x, uint32_t x_pitch, uint
 
 }  // namespace
 
-// The plan with the least estimated time.  The terms were fitted to 1600 timings on B200 (76 shapes, M 66 .. 8192, N 65 ..
-// 17408, K 256 .. 8160, both weight types, every plan); over them the choice is on average 0.4 % and at most 11 % slower than
+// The plan with the least estimated time.  The terms were fitted to 2200 timings on B200 (90 shapes, M 66 .. 8192, N 65 ..
+// 23000, K 256 .. 8100, both weight types, every plan); over them the choice is on average 0.4 % and at most 17 % slower than
 // the best plan, where 2 CTAs x 256 features for every call would be 30 % slower on average.  In us:
-//   a K block     0.28 - 0.29 whatever the tile's width (the feed from L2 bounds the narrow ones, the MMA the widest);
-//                 e4m3 0.35 - 0.40 (widening)
-//   an epilogue   1.2 for 64 columns, e4m3 1.5 times that (fewer registers)
-//   a K slice     3.3 for barriers and a cluster's start, 1.6 per 32 columns sent away
+//   a K block     0.21 - 0.30, not in proportion to the tile's width (what one SM draws from L2 bounds the narrow ones, the
+//                 MMA the widest); e4m3 0.27 - 0.40 (widening)
+//   an epilogue   0.8 for 64 columns, e4m3 1.5 times that (fewer registers)
+//   a K slice     4.0 for barriers and a cluster's start, 1.3 per 32 columns sent away
 TilePlan tile_plan(int wb, uint32_t M, uint32_t N, uint32_t K, uint32_t sms) {
     struct Form { uint32_t cg, bn, splits; double block[2]; };
-    static const Form forms[] = {{1, 64, 1, {0.28, 0.36}}, {1, 64, 2, {0.28, 0.36}}, {1, 128, 1, {0.28, 0.40}}, {1, 128, 2, {0.28, 0.40}},
-                                 {1, 128, 4, {0.28, 0.40}}, {2, 128, 1, {0.29, 0.35}}, {2, 128, 2, {0.29, 0.35}}, {2, 128, 4, {0.29, 0.35}},
-                                 {2, 256, 1, {0.29, 0.35}}, {2, 256, 2, {0.29, 0.35}}, {2, 256, 4, {0.29, 0.35}}};
+    static const Form forms[] = {{1, 64, 1, {0.22, 0.27}}, {1, 64, 2, {0.22, 0.27}}, {1, 128, 1, {0.24, 0.40}}, {1, 128, 2, {0.24, 0.40}},
+                                 {1, 128, 4, {0.24, 0.40}}, {2, 128, 1, {0.21, 0.31}}, {2, 128, 2, {0.21, 0.31}}, {2, 128, 4, {0.21, 0.31}},
+                                 {2, 256, 1, {0.30, 0.37}}, {2, 256, 2, {0.30, 0.37}}, {2, 256, 4, {0.30, 0.37}}};
     const uint32_t blocks = (K + kBK - 1) / kBK;
     TilePlan best{2, 256, 1};
     double least = 1e30;
@@ -725,10 +725,10 @@ TilePlan tile_plan(int wb, uint32_t M, uint32_t N, uint32_t K, uint32_t sms) {
         double room = size == 1u ? sms : size == 2u ? sms / 2u : size == 4u ? sms * 32u / 148u : sms * 14u / 148u;
         if (room < 1.0) room = 1.0;
         const double rounds = (double)(uint64_t)((tiles + room - 1.0) / room);
-        const double block = f.block[wb == 1 ? 1 : 0], epi = 1.2 * f.bn / 64.0 * (wb == 1 ? 1.5 : 1.0);
+        const double block = f.block[wb == 1 ? 1 : 0], epi = 0.8 * f.bn / 64.0 * (wb == 1 ? 1.5 : 1.0);
         const double slice = (double)((blocks + f.splits - 1u) / f.splits);
         const double t = f.splits == 1u ? rounds * (slice * block + epi)
-                                        : rounds * (3.3 + slice * block + 1.6 * (f.splits - 1.0) / f.splits * f.bn / 32.0) + epi / f.splits;
+                                        : rounds * (4.0 + slice * block + 1.3 * (f.splits - 1.0) / f.splits * f.bn / 32.0) + epi / f.splits;
         if (t < least) { least = t; best = {f.cg, f.bn, f.splits}; }
     }
     return best;
@@ -736,6 +736,7 @@ TilePlan tile_plan(int wb, uint32_t M, uint32_t N, uint32_t K, uint32_t sms) {
 
 // benchmark and test hook: every call takes this plan (cg = 0: the rule above)
 static std::atomic<uint32_t> g_forced{0};
+bool tile_forced() { return g_forced.load() != 0u; }
 void tile_force(uint32_t cg, uint32_t bn, uint32_t splits) { g_forced.store(cg == 0u ? 0u : (cg << 24) | (splits << 16) | bn); }
 
 mc_status_t linear_tile(int wb, const void* w, const uint16_t* x, uint32_t x_pitch, uint32_t M, uint32_t N, uint32_t K,

@@ -14,6 +14,7 @@ mc_status_t linear_tile(int wb, const void* w, const uint16_t* x, uint32_t x_pit
 struct TilePlan { uint32_t cg, bn, splits; };
 TilePlan tile_plan(int wb, uint32_t M, uint32_t N, uint32_t K, uint32_t sms);
 
+bool tile_forced();                                           // such a plan is set
 void tile_force(uint32_t cg, uint32_t bn, uint32_t splits);   // every call takes this plan; cg = 0: tile_plan
 
 // 1 when a bounded wait inside the kernel ran out since the last query (clears it), -1 on a CUDA error.

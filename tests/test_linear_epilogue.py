@@ -56,7 +56,7 @@ def test_tile_plan(pkg):
     """Host logic: every choice is a plan the kernel has, slices are never empty, big calls take the widest tile whole."""
     for wb in (1, 2):
         assert pkg.debug_tile_plan(wb, 8192, 11520, 2304) == (2, 256, 1)
-        assert pkg.debug_tile_plan(wb, 128, 2304, 5760)[2] > 1
+        assert pkg.debug_tile_plan(wb, 128, 2304, 5760, 148)[2] > 1
         for M in (65, 129, 500, 4000, 1 << 20):
             for N in (1, 63, 2304, 122753):
                 for K in (8, 64, 65, 2304, 30000):
