@@ -174,7 +174,7 @@ def _p(t) -> int | None:
 _current_stream = None
 
 
-def _stream(stream) -> int | None:
+def _stream(stream=None) -> int | None:
     """The handle itself: a torch.cuda.Stream object per call costs 3 us of host time, more than some kernels take."""
     if stream is None:
         global _current_stream
@@ -344,8 +344,16 @@ _EPILOGUE_SIZE = C.sizeof(Epilogue)
 def launch_linear_epilogue(w, scale, x, y, M, N, K, bias=None, residual=None, activation="none", gated=False, x_stride=0,
                            y_stride=0, residual_stride=0, stream=None, pdl=False):
     """y = act(x W^T * scale + bias) [* up] + residual for any M; activation: a key of ACTIVATIONS."""
-    e = Epilogue(_EPILOGUE_SIZE, ACTIVATIONS[activation], gated, x_stride, y_stride, residual_stride, _p(bias), _p(residual))
-    _check((_lib or lib()).mc_sm100_linear_epilogue(_p(w), _p(scale), _p(x), _p(y), M, N, K, C.byref(e), _stream(stream), pdl))
+    e = Epilogue(_EPILOGUE_SIZE, ACTIVATIONS[activation], gated, x_stride, y_stride, residual_stride,
+                 None if bias is None else _p(bias), None if residual is None else _p(residual))
+    try:                                          # tensors, without a call of _p for each
+        wp, xp, yp = w.data_ptr(), x.data_ptr(), y.data_ptr()
+    except AttributeError:
+        wp, xp, yp = _p(w), _p(x), _p(y)
+    rc = (_lib or lib()).mc_sm100_linear_epilogue(wp, None if scale is None else _p(scale), xp, yp, M, N, K, C.byref(e),
+                                                  (_current_stream or _stream)() if stream is None else _stream(stream), pdl)
+    if rc:
+        _check(rc)
 
 
 class LogitsTables(C.Structure):
@@ -359,15 +367,18 @@ _TABLES_SIZE = C.sizeof(LogitsTables)
 def logits_tables(table_vocab, counts=None, seen=None, masks=None, bias_token=None, bias_value=None, status=None) -> LogitsTables:
     """Tables of logits_process out of device tensors (their sizes give the numbers of rows); the caller keeps the tensors."""
     words = (table_vocab + 31) // 32
-    return LogitsTables(_TABLES_SIZE, table_vocab, counts.numel() // table_vocab if counts is not None else 0,
-                        masks.numel() // words if masks is not None else 0, bias_token.numel() if bias_token is not None else 0, 0,
-                        _p(counts), _p(seen), _p(masks), _p(bias_token), _p(bias_value), _p(status))
+    return LogitsTables(_TABLES_SIZE, table_vocab, 0 if counts is None else counts.numel() // table_vocab, 0 if masks is None else masks.numel() // words,
+                        0 if bias_token is None else bias_token.numel(), 0, None if counts is None else _p(counts), None if seen is None else _p(seen),
+                        None if masks is None else _p(masks), None if bias_token is None else _p(bias_token),
+                        None if bias_value is None else _p(bias_value), None if status is None else _p(status))
 
 
 def logits_process(logits, out, n_rows, vocab, row_stride, out_stride, cfg, tables, index_base=0, stream=None, pdl=False):
     """cfg: device tensor of n_rows x 8 words (rep, freq, pres penalty as f32 bits, history slot, mask row, bias begin, bias count, 0)."""
-    _check((_lib or lib()).mc_sm100_logits_process(_p(logits), _p(out), n_rows, vocab, row_stride, out_stride, index_base, _p(cfg),
-                                                   C.byref(tables), _stream(stream), pdl))
+    rc = (_lib or lib()).mc_sm100_logits_process(_p(logits), _p(out), n_rows, vocab, row_stride, out_stride, index_base, _p(cfg), C.byref(tables),
+                                                 (_current_stream or _stream)() if stream is None else _stream(stream), pdl)
+    if rc:
+        _check(rc)
 
 
 def token_history(counts, seen, tokens, n_seqs, table_vocab, offsets=None, prompt_len=None, slots=None, n_tokens=None, n_slots=None,
@@ -376,8 +387,12 @@ def token_history(counts, seen, tokens, n_seqs, table_vocab, offsets=None, promp
         n_tokens = tokens.numel()
     if n_slots is None:
         n_slots = counts.numel() // table_vocab
-    _check((_lib or lib()).mc_sm100_token_history(_p(counts), _p(seen), n_slots, table_vocab, _p(tokens), n_tokens, _p(offsets), _p(prompt_len),
-                                                  _p(slots), n_seqs, rebuild, _p(status), _stream(stream), pdl))
+    rc = (_lib or lib()).mc_sm100_token_history(_p(counts), _p(seen), n_slots, table_vocab, _p(tokens), n_tokens,
+                                                None if offsets is None else _p(offsets), None if prompt_len is None else _p(prompt_len),
+                                                None if slots is None else _p(slots), n_seqs, rebuild, None if status is None else _p(status),
+                                                (_current_stream or _stream)() if stream is None else _stream(stream), pdl)
+    if rc:
+        _check(rc)
 
 
 def linear_host(kind, w, scale, h_x, h_y, M, N, K, x_stage, y_stage, workspace=None, ws_size=0, stream=None):
