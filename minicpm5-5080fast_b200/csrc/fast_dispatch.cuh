@@ -13,7 +13,13 @@ namespace mcl {
 template <int WB, int R, int U, bool PRE, bool DB, int PRO, int EPI, int T, int MINB = 1>
 inline mc_status_t launch_fast_one(const RowsArgs& a, cudaStream_t stream, bool pdl) {
     auto kern = gemv_fast_kernel<WB, R, U, PRE, DB, PRO, EPI, T, MINB>;
-    const size_t smem = (size_t)a.K * (WB == 1 ? 4u : 2u) + (PRO == PRO_RESNORM ? (size_t)a.K * 4u : 0u);
+    const uint32_t groups = (a.N + R - 1) / R;
+    uint32_t gx = (uint32_t)sm_count();
+    if (groups < gx) gx = groups;
+    if (EPI == EPI_ARGMAX && gx > kArgmaxCands) gx = kArgmaxCands;
+    // fused epilogue: bias and residual entries of a CTA's groups
+    const size_t fused = EPI == EPI_FUSED || EPI == EPI_FUSED_GATED ? (size_t)((groups + gx - 1u) / gx) * (R + (EPI == EPI_FUSED ? R : 1)) * 2u : 0u;
+    const size_t smem = (size_t)a.K * (WB == 1 ? 4u : 2u) + (PRO == PRO_RESNORM ? (size_t)a.K * 4u : 0u) + fused;
     if (smem > 200u * 1024u) {
         set_error("gemv: activation of %zu bytes does not fit in shared memory", smem);
         return MC_E_UNSUPPORTED;
@@ -24,10 +30,6 @@ inline mc_status_t launch_fast_one(const RowsArgs& a, cudaStream_t stream, bool 
         set_error("gemv: cannot raise shared memory to %zu: %s", smem, cudaGetErrorString(e));
         return MC_E_CUDA;
     }
-    const uint32_t groups = (a.N + R - 1) / R;
-    uint32_t gx = (uint32_t)sm_count();
-    if (groups < gx) gx = groups;
-    if (EPI == EPI_ARGMAX && gx > kArgmaxCands) gx = kArgmaxCands;
     RowsArgs b = a;     // a.pf arrives as the raw hint (ptr, bytes); cut it into one slice per CTA
     b.pf = make_prefetch_args(NextWeights{a.pf.ptr, a.pf.bytes}, gx);
     (void)launch(kern, dim3(gx), dim3(T), smem, stream, pdl, b);

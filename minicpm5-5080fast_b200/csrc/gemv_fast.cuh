@@ -237,12 +237,8 @@ __global__ void __launch_bounds__(THREADS, MINB) gemv_fast_kernel(const RowsArgs
     float scA[R], scB[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) { scA[r] = 1.f; scB[r] = 1.f; }
-    // fused epilogue: the rows' biases travel the same way (no second register buffer in its tile shapes); the group's
-    // residual, which the previous kernel may write, is asked for after the wait and ahead of the arithmetic
     constexpr bool FUSED = EPI == EPI_FUSED || EPI == EPI_FUSED_GATED;
-    static_assert(!(FUSED && DB), "one bias buffer");
-    constexpr int OUTS = EPI == EPI_FUSED_GATED ? 1 : R;
-    uint16_t bias_b[FUSED ? R : 1], res_b[FUSED ? OUTS : 1];
+    constexpr int OUTS = EPI == EPI_FUSED_GATED ? 1 : R;       // outputs of a group
     auto issue = [&](auto& raw, float (&sc)[R], uint32_t g, uint32_t i0) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -250,9 +246,6 @@ __global__ void __launch_bounds__(THREADS, MINB) gemv_fast_kernel(const RowsArgs
             const uint8_t* wr = wbase + (size_t)row * row_bytes;
             if constexpr (WB == 1) {
                 if (i0 == 0u && row < a.N) sc[r] = __ldg(a.scale + row);
-            }
-            if constexpr (FUSED) {
-                if (i0 == 0u) bias_b[r] = (a.ep.bias != nullptr && row < a.N) ? __ldg(a.ep.bias + row) : (uint16_t)0;
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -262,6 +255,8 @@ __global__ void __launch_bounds__(THREADS, MINB) gemv_fast_kernel(const RowsArgs
         }
     };
 
+    // the fused call keeps plain stream order unless its caller allows the weights to be read ahead of it
+    if constexpr (FUSED) { if (a.ep.wait_first) pdl_wait(); }
     uint32_t g = blockIdx.x + warp * gridDim.x;
     if (g < groups) {
         issue(rawA, scA, g, 0);
@@ -355,6 +350,22 @@ __global__ void __launch_bounds__(THREADS, MINB) gemv_fast_kernel(const RowsArgs
             put_x8<WB>(xh, xb, c, bits, inexact);
         }
     }
+    // Fused epilogue: biases and residuals of all of this CTA's groups, group blockIdx.x + i * gridDim.x at entry i.  (Loaded
+    // group by group in the loop below they cost it registers, and so weights in flight: lm_head 103 us against 88.)
+    const uint32_t cta_groups = FUSED && blockIdx.x < groups ? (groups - blockIdx.x + gridDim.x - 1u) / gridDim.x : 0u;
+    uint16_t* s_bias = xb + K;
+    uint16_t* s_res = s_bias + cta_groups * R;
+    if constexpr (FUSED) {
+        const uint32_t outs = EPI == EPI_FUSED_GATED ? a.N / 2u : a.N;
+        for (uint32_t i = threadIdx.x; i < cta_groups * R; i += THREADS) {
+            const uint32_t row = (blockIdx.x + i / R * gridDim.x) * R + i % R;
+            s_bias[i] = a.ep.bias != nullptr && row < a.N ? a.ep.bias[row] : (uint16_t)0;
+        }
+        for (uint32_t i = threadIdx.x; i < cta_groups * OUTS; i += THREADS) {
+            const uint32_t out = (blockIdx.x + i / OUTS * gridDim.x) * OUTS + i % OUTS;
+            s_res[i] = a.ep.res != nullptr && out < outs ? a.ep.res[out] : (uint16_t)0x8000u;   // -0 leaves every sum as it is
+        }
+    }
     const bool fallback = __syncthreads_or(inexact ? 1 : 0) != 0;   // also the staging barrier
 
     float best_v = -INFINITY;
@@ -442,13 +453,14 @@ __global__ void __launch_bounds__(THREADS, MINB) gemv_fast_kernel(const RowsArgs
         if constexpr (FUSED) {
             if (lane == 0u) {
                 auto bf = [](uint16_t b) { return __uint_as_float((uint32_t)b << 16); };
+                const uint32_t i = (g - blockIdx.x) / gridDim.x;
 #pragma unroll
                 for (int o = 0; o < OUTS; ++o) {
                     const uint32_t out = g * OUTS + o;
                     float v;
-                    if constexpr (EPI == EPI_FUSED_GATED) v = epi_act(tot[0] + bf(bias_b[0]), a.ep.act) * (tot[R - 1] + bf(bias_b[FUSED ? R - 1 : 0]));
-                    else v = epi_act(tot[o] + bf(bias_b[FUSED ? o : 0]), a.ep.act);
-                    if (out < (EPI == EPI_FUSED_GATED ? a.N / 2u : a.N)) a.y[out] = f32_to_bf16_bits(v + bf(res_b[FUSED ? o : 0]));
+                    if constexpr (EPI == EPI_FUSED_GATED) v = epi_act(tot[0] + bf(s_bias[i * R]), a.ep.act) * (tot[R - 1] + bf(s_bias[i * R + R - 1]));
+                    else v = epi_act(tot[o] + bf(s_bias[i * R + o]), a.ep.act);
+                    if (out < (EPI == EPI_FUSED_GATED ? a.N / 2u : a.N)) a.y[out] = f32_to_bf16_bits(v + bf(s_res[i * OUTS + o]));
                 }
             }
         } else if (lane < ndst) {      // the sums are the same in every lane
@@ -510,14 +522,6 @@ __global__ void __launch_bounds__(THREADS, MINB) gemv_fast_kernel(const RowsArgs
         for (; g < groups; g += gstep) {
             float2 acc_a[R], acc_b[R];
             zero(acc_a, acc_b);
-            if constexpr (FUSED) {
-#pragma unroll
-                for (int o = 0; o < OUTS; ++o) {
-                    const uint32_t out = g * OUTS + o;
-                    // -0 leaves every sum as it is
-                    res_b[o] = (a.ep.res != nullptr && out < (EPI == EPI_FUSED_GATED ? a.N / 2u : a.N)) ? a.ep.res[out] : (uint16_t)0x8000u;
-                }
-            }
             for (uint32_t i0 = 0; i0 < per_lane; i0 += U) {
                 if (!first) issue(rawA, scA, g, i0);
                 if (!skip_mac) mac_batch(rawA, first, i0, acc_a, acc_b);

@@ -135,16 +135,18 @@ extern "C" mc_status_t mc_sm100_linear_epilogue(const void* d_w, const float* d_
         set_error("mc_sm100_linear_epilogue: residual and y are one buffer with strides %u and %u", rs, ys);
         return MC_E_INVALID_ARGUMENT;
     }
-    const EpiArgs e{d_scale, d.d_bias, d.d_residual, d_y, ys, rs, d.activation, d.gated};
+    const EpiArgs e{d_scale, d.d_bias, d.d_residual, d_y, ys, rs, d.activation, d.gated, pdl != 0 ? 0u : 1u};
     const cudaStream_t st = (cudaStream_t)stream;
+    // Every kernel below is launched with the programmatic attribute, so that its launch and set-up run under the end of the
+    // previous kernel; what it reads before that end is nothing (e.wait_first), or with `pdl` the weights.
     // rows that a 16-byte unit divides, at aligned addresses: the kernels that stream
     const bool unit = aligned16(d_w) && aligned16(d_x) && ((uint64_t)K * (uint32_t)wb) % 16u == 0u;
-    if (M == 1u && unit && (uint64_t)K * (wb == 1 ? 4u : 2u) <= 200u * 1024u) {       // the activation in shared memory
+    if (M == 1u && unit && (uint64_t)K * (wb == 1 ? 4u : 2u) + (uint64_t)N / 16u <= 200u * 1024u) {       // the activation in shared memory
         RowsArgs a{};
         a.w = d_w; a.scale = d_scale; a.x = d_x; a.y = d_y; a.N = N; a.K = K; a.y_stride = ys; a.kseg = K; a.ep = e;
         const NextWeights nw = take_next_weights();
         a.pf.ptr = static_cast<const uint8_t*>(nw.ptr); a.pf.bytes = nw.bytes;
-        return launch_fast_fused(wb, d.gated != 0u, a, st, pdl != 0);
+        return launch_fast_fused(wb, d.gated != 0u, a, st, true);
     }
     const bool tma = unit && (xs & 7u) == 0u;
     // Up to 64 rows the skinny kernel, which splits K eight ways and pads M to 16, 32 or 64.  From 33 rows on the tiled kernel
@@ -152,9 +154,9 @@ extern "C" mc_status_t mc_sm100_linear_epilogue(const void* d_w, const float* d_
     // 122753 x 2304: 95 against 115 us; M = 64, 11520 x 2304: 15.1 against 19.3), slower elsewhere (M = 64, 2304 x 5760: 16.7
     // against 14.2; M = 48, 20000 x 4096: 43.9 against 41.8).
     const bool tiled = M > 64u || tile_forced() || (M > 32u && (K <= 768u || (N >= 4096u && K <= 3000u)));
-    if (!tiled && tma) return skinny_gemm_fused(wb == 2 ? SKINNY_W_BF16 : SKINNY_W_E4M3, d_w, d_x, xs, M, N, K, e, st, pdl != 0);
-    if (tma) return linear_tile(wb, d_w, d_x, xs, M, N, K, e, st, pdl != 0);
-    return linear_any(wb, d_w, d_x, xs, M, N, K, e, st, pdl != 0);
+    if (!tiled && tma) return skinny_gemm_fused(wb == 2 ? SKINNY_W_BF16 : SKINNY_W_E4M3, d_w, d_x, xs, M, N, K, e, st, true);
+    if (tma) return linear_tile(wb, d_w, d_x, xs, M, N, K, e, st, true);
+    return linear_any(wb, d_w, d_x, xs, M, N, K, e, st, true);
 }
 
 extern "C" void mc_sm100_debug_set_tile_plan(uint32_t cg, uint32_t bn, uint32_t splits) { tile_force(cg, bn, splits); }

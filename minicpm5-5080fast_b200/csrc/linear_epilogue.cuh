@@ -13,6 +13,7 @@ struct EpiArgs {
     uint16_t* y;               // [M, y_stride] bf16
     uint32_t y_stride, res_stride;
     uint32_t act, gated;
+    uint32_t wait_first;       // 1: nothing is read before the previous kernel in the stream has ended, the weights neither
 };
 
 #if defined(__CUDACC__)

@@ -392,6 +392,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             uint32_t mt = 0, nt = 0;
             if (nloc != 0u) tile_of(a, cid, mt, nt);
             const int32_t m0 = (int32_t)(mt * 128u), n0 = (int32_t)(nt * BN);
+            if (a.ep.wait_first) pdl_wait();
             for (uint32_t it = 0; it < early; ++it) {
                 const uint32_t bar = WB == 1 ? raw_full(it) : full(it);
                 mbar_expect_tx(bar, WB == 1 ? G::RAW : G::A + G::B);

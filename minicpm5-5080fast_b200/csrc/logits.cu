@@ -360,9 +360,11 @@ using namespace mcl;
 
 extern "C" {
 
+// The kernels of this file wait for the previous kernel before they read anything; they are always launched with the
+// programmatic attribute, which lets their launch and set-up run under its end.
 mc_status_t mc_sm100_logits_process(const uint16_t* d_logits, uint16_t* d_out, uint32_t n_rows, uint32_t vocab, uint32_t row_stride,
                                     uint32_t out_stride, int32_t index_base, const mc_sm100_logits_config_t* d_cfg,
-                                    const mc_sm100_logits_tables_t* tables, void* stream, int32_t pdl) {
+                                    const mc_sm100_logits_tables_t* tables, void* stream, int32_t) {
     clear_error();
     const char* who = "mc_sm100_logits_process";
     if (d_logits == nullptr || d_out == nullptr || d_cfg == nullptr || tables == nullptr || n_rows == 0 || n_rows > 65535u || vocab == 0 ||
@@ -380,14 +382,14 @@ mc_status_t mc_sm100_logits_process(const uint16_t* d_logits, uint16_t* d_out, u
     }
     const LogitsArgs a{d_logits, d_out, vocab, row_stride, out_stride, index_base, d_cfg, t};
     (void)launch(logits_process_kernel, dim3((vocab + kPiece - 1u + kSpan - 1u) / kSpan, n_rows), dim3(kLogitsThreads), 0,
-                 (cudaStream_t)stream, pdl != 0, a);
+                 (cudaStream_t)stream, true, a);
     MCL_CHECK_LAUNCH("logits_process");
     return MC_OK;
 }
 
 mc_status_t mc_sm100_token_history(int32_t* d_counts, uint32_t* d_seen, uint32_t n_slots, uint32_t table_vocab, const int32_t* d_tokens,
                                    uint32_t n_tokens, const uint32_t* d_offsets, const uint32_t* d_prompt_len, const int32_t* d_slots,
-                                   uint32_t n_seqs, int32_t rebuild, int32_t* d_status, void* stream, int32_t pdl) {
+                                   uint32_t n_seqs, int32_t rebuild, int32_t* d_status, void* stream, int32_t) {
     clear_error();
     if (d_counts == nullptr || d_seen == nullptr || n_slots == 0 || n_slots > 0x7FFFFFFFu || table_vocab == 0 || table_vocab > 0x40000000u ||
         (d_tokens == nullptr && n_tokens != 0u) || n_seqs == 0 || n_seqs > 0x7FFFFFFFu || (d_offsets == nullptr && n_tokens < n_seqs) ||
@@ -409,11 +411,11 @@ mc_status_t mc_sm100_token_history(int32_t* d_counts, uint32_t* d_seen, uint32_t
             return MC_E_CUDA;
         }
         (void)launch(history_rebuild_kernel, dim3(n_seqs, (uint32_t)((table_vocab + span - 1u) / span)), dim3(kHistThreads), bytes,
-                     (cudaStream_t)stream, pdl != 0, a, n_seqs, (uint32_t)span);
+                     (cudaStream_t)stream, true, a, n_seqs, (uint32_t)span);
         MCL_CHECK_LAUNCH("history_rebuild");
         return MC_OK;
     }
-    (void)launch(history_add_kernel, dim3(n_seqs, d_offsets != nullptr ? 8 : 1), dim3(kLogitsThreads), 0, (cudaStream_t)stream, pdl != 0, a);
+    (void)launch(history_add_kernel, dim3(n_seqs, d_offsets != nullptr ? 8 : 1), dim3(kLogitsThreads), 0, (cudaStream_t)stream, true, a);
     MCL_CHECK_LAUNCH("history_add");
     return MC_OK;
 }

@@ -155,6 +155,7 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     constexpr uint32_t W_BYTES = E4 ? G::A_RAW : G::A_OP;
     const uint32_t pre = nloc < WS ? nloc : WS;
     if (tid == 0) {
+        if constexpr (EXT) { if (a.ep.wait_first) pdl_wait(); }
         abort_flag = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
         for (uint32_t s = 0; s < OPS; ++s) { mbar_init(op_full(s), 1); mbar_init(op_empty(s), 1); }
