@@ -277,15 +277,20 @@ typedef enum mc_sm100_activation_t {
     MC_SM100_ACT_NONE = 0, MC_SM100_ACT_RELU = 1, MC_SM100_ACT_GELU = 2, MC_SM100_ACT_GELU_TANH = 3, MC_SM100_ACT_SILU = 4
 } mc_sm100_activation_t;
 
-typedef struct mc_sm100_epilogue_t {
-    uint32_t struct_size;            /* caller sets sizeof(mc_sm100_epilogue_t) */
+typedef struct mc_sm100_linear_epilogue_t {
+    uint32_t struct_size;            /* caller sets sizeof(mc_sm100_linear_epilogue_t) */
+    uint32_t M, N, K;                /* rows of x, rows of W, products of a sum */
     uint32_t activation;             /* mc_sm100_activation_t */
     uint32_t gated;                  /* 1: W's rows are interleaved (gate_j, up_j) as mc_sm100_interleave_rows leaves them */
     uint32_t x_stride, y_stride, residual_stride;   /* elements from row to row; 0 = compact (K, N_out, N_out) */
+    uint32_t reserved;               /* must be zero */
+    const void* d_w;                 /* [N, K] bf16, or e4m3 codes */
+    const float* d_scale;            /* [N] fp32 for e4m3 codes; NULL = bf16 weights */
+    const uint16_t* d_x;             /* [M, x_stride] bf16 */
+    uint16_t* d_y;                   /* [M, y_stride] bf16 */
     const uint16_t* d_bias;          /* [N] bf16 or NULL (gated: interleaved like the rows of W) */
-    const uint16_t* d_residual;      /* [M, N_out] bf16 or NULL; may be d_y itself, with the same stride */
-    uint32_t reserved[2];            /* must be zero */
-} mc_sm100_epilogue_t;
+    const uint16_t* d_residual;      /* [M, residual_stride] bf16 or NULL; may be d_y itself, with the same stride */
+} mc_sm100_linear_epilogue_t;
 
 /* A linear for any number of rows, from one token to a long prompt chunk, with what follows it:
  *   z[m,n] = scale[n] * sum_k W[n,k] x[m,k] + bias[n]
@@ -293,15 +298,15 @@ typedef struct mc_sm100_epilogue_t {
  *          = act(z[m,2j]) * z[m,2j+1]           gated, N_out = N / 2
  *   y[m,j] = bf16( v[m,j] + residual[m,j] )
  * Everything between the products and y stays in fp32: one rounding.  (mc_sm100_gate_up_swiglu rounds gate and up to
- * bf16 first, as the reference's pair of kernels does; this call does not.)  d_scale == NULL: bf16 weights (d_w read as
- * uint16_t), otherwise e4m3 codes with one fp32 scale per row (codes 0x7F / 0xFF count as +/-480, as everywhere here).
- * epilogue == NULL: the plain linear.  Any M, N, K >= 1 (gated: N even) and any stride >= the row; operands aligned to
- * their elements.  16-byte aligned d_w and d_x, K * (bytes per weight) and x_stride * 2 multiples of 16 take the
- * tensor-core kernels that stream by TMA; anything else a slower kernel with plain loads.  x and y must not overlap.
- * Results do not depend on the launch: no atomics, a fixed order of every sum. */
-MC_SM100_API mc_status_t mc_sm100_linear_epilogue(const void* d_w, const float* d_scale, const uint16_t* d_x, uint16_t* d_y,
-                                                  uint32_t M, uint32_t N, uint32_t K, const mc_sm100_epilogue_t* epilogue,
-                                                  void* stream, int32_t pdl);
+ * bf16 first, as the reference's pair of kernels does; this call does not.)  The e4m3 codes 0x7F / 0xFF count as +/-480, as
+ * everywhere here.  Any M, N, K >= 1 (gated: N even) and any stride >= the row; operands aligned to their elements.  16-byte
+ * aligned d_w and d_x, K * (bytes per weight) and x_stride * 2 multiples of 16 take the kernels that stream; anything else a
+ * slower one with plain loads.  y overlaps neither x nor, but for the whole, the residual.  Results do not depend on the
+ * launch: no atomics, a fixed order of every sum.
+ * The arguments come in one struct (copied before the call returns).  The kernel's launch and set-up may run under the end
+ * of the previous kernel in the stream, but with pdl == 0 it reads nothing, and with pdl != 0 only the weights and what
+ * belongs to them (scale), before that end. */
+MC_SM100_API mc_status_t mc_sm100_linear_epilogue(const mc_sm100_linear_epilogue_t* call, void* stream, int32_t pdl);
 
 /* ------------------------------------------------------- lm_head / greedy --- */
 
@@ -418,31 +423,50 @@ typedef struct mc_sm100_logits_tables_t {
     int32_t* d_status;               /* optional: set to 1 when a row names a slot, a mask or entries outside the tables */
 } mc_sm100_logits_tables_t;
 
-/* Edits bf16 logits [n_rows, vocab] by the rows' rules, in this order and in fp32 with one rounding at the end:
- * repetition penalty, frequency and presence penalty, biases (a token listed several times takes their sum, added in
- * list order; tokens outside the logits are passed over), grammar mask (a token that is not allowed becomes -infinity,
- * whatever it held, a NaN too).  A row whose mask leaves nothing becomes -infinity throughout.  A row that names a slot,
- * mask or entries outside the tables goes without them, and *d_status says so.  d_out may be d_logits itself with the
- * same stride; logits kept for their probabilities go to another buffer.  Columns from vocab to the stride are not
- * touched.  index_base: token of column 0 (vocab shards).  Replaces rep_penalty_mark / rep_penalty_apply
+typedef struct mc_sm100_logits_process_t {
+    uint32_t struct_size;            /* caller sets sizeof(mc_sm100_logits_process_t) */
+    uint32_t n_rows, vocab;          /* rows (<= 65535) and columns of the logits */
+    uint32_t row_stride, out_stride; /* elements from row to row */
+    int32_t  index_base;             /* token of column 0 (vocab shards) */
+    const uint16_t* d_logits;
+    uint16_t* d_out;                 /* may be d_logits itself, with the same stride */
+    const mc_sm100_logits_config_t* d_cfg;   /* [n_rows] in device memory */
+} mc_sm100_logits_process_t;
+
+/* Edits bf16 logits by the rows' rules, in this order and in fp32 with one rounding at the end: repetition penalty,
+ * frequency and presence penalty, biases (a token listed several times takes their sum, added in list order; tokens
+ * outside the logits are passed over), grammar mask (a token that is not allowed becomes -infinity, whatever it held, a NaN
+ * too).  A row whose mask leaves nothing becomes -infinity throughout.  A row that names a slot, mask or entries outside the
+ * tables goes without them, and *d_status says so.  Logits kept for their probabilities go to another buffer.  Columns from
+ * vocab to the stride are not touched.  Replaces rep_penalty_mark / rep_penalty_apply
  * (native/kernels/sm120/sampling.cu:293-324) in front of mc_sm100_sample_topk_topp / mc_sm100_argmax_bf16; biases, masks
- * and the other two penalties have no counterpart there.  n_rows <= 65535. */
-MC_SM100_API mc_status_t mc_sm100_logits_process(const uint16_t* d_logits, uint16_t* d_out, uint32_t n_rows, uint32_t vocab,
-                                                 uint32_t row_stride, uint32_t out_stride, int32_t index_base,
-                                                 const mc_sm100_logits_config_t* d_cfg, const mc_sm100_logits_tables_t* tables,
+ * and the other two penalties have no counterpart there.  Both structs are copied before the call returns.  Nothing is read
+ * before the end of the previous kernel in the stream, whatever `pdl` says; only launch and set-up run under it. */
+MC_SM100_API mc_status_t mc_sm100_logits_process(const mc_sm100_logits_process_t* call, const mc_sm100_logits_tables_t* tables,
                                                  void* stream, int32_t pdl);
+
+typedef struct mc_sm100_token_history_t {
+    uint32_t struct_size;            /* caller sets sizeof(mc_sm100_token_history_t) */
+    uint32_t n_slots, table_vocab, n_tokens, n_seqs;
+    uint32_t rebuild;                /* 0 or 1 */
+    int32_t*  d_counts;              /* [n_slots, table_vocab] */
+    uint32_t* d_seen;                /* [n_slots, ceil(table_vocab / 32)] */
+    const int32_t*  d_tokens;        /* [n_tokens] */
+    const uint32_t* d_offsets;       /* [n_seqs + 1] or NULL */
+    const uint32_t* d_prompt_len;    /* [n_seqs] or NULL */
+    const int32_t*  d_slots;         /* [n_seqs] or NULL */
+    int32_t* d_status;               /* or NULL */
+} mc_sm100_token_history_t;
 
 /* The history those penalties read.  Sequence i (of n_seqs) is d_tokens[d_offsets[i] .. d_offsets[i + 1]) -- without
  * d_offsets the single token i, as a sampler leaves them -- and belongs to slot d_slots[i] (without d_slots: i).  Its
  * first d_prompt_len[i] tokens (without d_prompt_len: none) are prompt: they set the seen bit only; the others also add 1
- * to their count.  rebuild != 0: every slot named starts from nothing (a request is admitted, or comes back), otherwise
+ * to their count.  rebuild: every slot named starts from nothing (a request is admitted, or comes back), otherwise
  * the tokens are added to what is there.  Several sequences may name one slot.  Tokens outside [0, table_vocab) are passed
  * over (a sampler's -1); a sequence whose slot is outside [0, n_slots) or whose offsets leave [0, n_tokens] is passed over
- * and sets *d_status (optional) to 1.  Slots that no sequence names are not touched. */
-MC_SM100_API mc_status_t mc_sm100_token_history(int32_t* d_counts, uint32_t* d_seen, uint32_t n_slots, uint32_t table_vocab,
-                                                const int32_t* d_tokens, uint32_t n_tokens, const uint32_t* d_offsets,
-                                                const uint32_t* d_prompt_len, const int32_t* d_slots, uint32_t n_seqs,
-                                                int32_t rebuild, int32_t* d_status, void* stream, int32_t pdl);
+ * and sets *d_status to 1.  Slots that no sequence names are not touched.  The struct is copied before the call returns;
+ * `pdl` as for mc_sm100_logits_process. */
+MC_SM100_API mc_status_t mc_sm100_token_history(const mc_sm100_token_history_t* call, void* stream, int32_t pdl);
 
 /* ------------------------------------------------- host-buffer convenience -- */
 

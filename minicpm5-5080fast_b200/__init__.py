@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmc_sm100a_linear.so")
@@ -65,9 +66,9 @@ SIGNATURES = {
     "mc_sm100_sampling_exchange_bytes": (C.c_size_t, [_u32, _u32]),
     "mc_sm100_sample_topk_topp_sharded": (_i32, [_vp, _u32, _u32, _u32, _i32, _vp, _vp, _vp, _vp, _vp, _u32, _vp, _u32, _u32,
                                                  C.c_uint64, _vp, _vp, _i32]),
-    "mc_sm100_linear_epilogue": (_i32, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _i32]),
-    "mc_sm100_logits_process": (_i32, [_vp, _vp, _u32, _u32, _u32, _u32, _i32, _vp, _vp, _vp, _i32]),
-    "mc_sm100_token_history": (_i32, [_vp, _vp, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _u32, _i32, _vp, _vp, _i32]),
+    "mc_sm100_linear_epilogue": (_i32, [_vp, _vp, _i32]),
+    "mc_sm100_logits_process": (_i32, [_vp, _vp, _vp, _i32]),
+    "mc_sm100_token_history": (_i32, [_vp, _vp, _i32]),
     "mc_sm100_linear_host": (_i32, [_i32, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp, C.c_size_t, _vp]),
     "mc_sm100_stack_sizes": (_i32, [_vp, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]),
     "mc_sm100_stack_section": (_i32, [_vp, _u32, _u32, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]),
@@ -330,53 +331,49 @@ def sample_topk_topp_sharded(logits, n_rows, vocab, row_stride, index_base, cfg,
                                                    timeout_ns, _p(status), _stream(stream), int(pdl)))
 
 
+# The three calls below take their arguments in one struct, packed here: a ctypes call with a dozen arguments costs the host
+# more than a launch.  Formats: uint32 / int32 fields, then pointers, as the header declares them.
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+LINEAR_CALL, LOGITS_CALL = struct.Struct("=10I6Q"), struct.Struct("=5Ii3Q")
+LOGITS_TABLES, HISTORY_CALL = struct.Struct("=6I6Q"), struct.Struct("=6I7Q")
+_pack_linear, _pack_logits, _pack_tables, _pack_history = LINEAR_CALL.pack, LOGITS_CALL.pack, LOGITS_TABLES.pack, HISTORY_CALL.pack
 
 
-class Epilogue(C.Structure):
-    _fields_ = [("struct_size", _u32), ("activation", _u32), ("gated", _u32), ("x_stride", _u32), ("y_stride", _u32),
-                ("residual_stride", _u32), ("d_bias", _vp), ("d_residual", _vp), ("reserved", _u32 * 2)]
-
-
-_EPILOGUE_SIZE = C.sizeof(Epilogue)
+def _a(t) -> int:
+    """Address of a tensor (or an address), 0 for None."""
+    if t is None:
+        return 0
+    return t if t.__class__ is int else t.data_ptr()
 
 
 def launch_linear_epilogue(w, scale, x, y, M, N, K, bias=None, residual=None, activation="none", gated=False, x_stride=0,
                            y_stride=0, residual_stride=0, stream=None, pdl=False):
     """y = act(x W^T * scale + bias) [* up] + residual for any M; activation: a key of ACTIVATIONS."""
-    e = Epilogue(_EPILOGUE_SIZE, ACTIVATIONS[activation], gated, x_stride, y_stride, residual_stride,
-                 None if bias is None else _p(bias), None if residual is None else _p(residual))
-    try:                                          # tensors, without a call of _p for each
-        wp, xp, yp = w.data_ptr(), x.data_ptr(), y.data_ptr()
+    try:                                          # tensors, without a call of _a for each
+        call = _pack_linear(88, M, N, K, ACTIVATIONS[activation], gated, x_stride, y_stride, residual_stride, 0, w.data_ptr(),
+                            0 if scale is None else scale.data_ptr(), x.data_ptr(), y.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                            0 if residual is None else residual.data_ptr())
     except AttributeError:
-        wp, xp, yp = _p(w), _p(x), _p(y)
-    rc = (_lib or lib()).mc_sm100_linear_epilogue(wp, None if scale is None else _p(scale), xp, yp, M, N, K, C.byref(e),
-                                                  (_current_stream or _stream)() if stream is None else _stream(stream), pdl)
+        call = _pack_linear(88, M, N, K, ACTIVATIONS[activation], gated, x_stride, y_stride, residual_stride, 0, _a(w), _a(scale), _a(x), _a(y),
+                            _a(bias), _a(residual))
+    rc = (_lib or lib()).mc_sm100_linear_epilogue(call, (_current_stream or _stream)() if stream is None else _stream(stream), pdl)
     if rc:
         _check(rc)
 
 
-class LogitsTables(C.Structure):
-    _fields_ = [("struct_size", _u32), ("table_vocab", _u32), ("n_slots", _u32), ("n_masks", _u32), ("n_bias", _u32), ("reserved", _u32),
-                ("d_counts", _vp), ("d_seen", _vp), ("d_mask", _vp), ("d_bias_token", _vp), ("d_bias_value", _vp), ("d_status", _vp)]
-
-
-_TABLES_SIZE = C.sizeof(LogitsTables)
-
-
-def logits_tables(table_vocab, counts=None, seen=None, masks=None, bias_token=None, bias_value=None, status=None) -> LogitsTables:
+def logits_tables(table_vocab, counts=None, seen=None, masks=None, bias_token=None, bias_value=None, status=None) -> bytes:
     """Tables of logits_process out of device tensors (their sizes give the numbers of rows); the caller keeps the tensors."""
-    words = (table_vocab + 31) // 32
-    return LogitsTables(_TABLES_SIZE, table_vocab, 0 if counts is None else counts.numel() // table_vocab, 0 if masks is None else masks.numel() // words,
-                        0 if bias_token is None else bias_token.numel(), 0, None if counts is None else _p(counts), None if seen is None else _p(seen),
-                        None if masks is None else _p(masks), None if bias_token is None else _p(bias_token),
-                        None if bias_value is None else _p(bias_value), None if status is None else _p(status))
+    return _pack_tables(72, table_vocab, 0 if counts is None else counts.numel() // table_vocab,
+                        0 if masks is None else masks.numel() // ((table_vocab + 31) // 32), 0 if bias_token is None else bias_token.numel(), 0,
+                        0 if counts is None else counts.data_ptr(), 0 if seen is None else seen.data_ptr(), 0 if masks is None else masks.data_ptr(),
+                        0 if bias_token is None else bias_token.data_ptr(), 0 if bias_value is None else bias_value.data_ptr(),
+                        0 if status is None else status.data_ptr())
 
 
 def logits_process(logits, out, n_rows, vocab, row_stride, out_stride, cfg, tables, index_base=0, stream=None, pdl=False):
     """cfg: device tensor of n_rows x 8 words (rep, freq, pres penalty as f32 bits, history slot, mask row, bias begin, bias count, 0)."""
-    rc = (_lib or lib()).mc_sm100_logits_process(_p(logits), _p(out), n_rows, vocab, row_stride, out_stride, index_base, _p(cfg), C.byref(tables),
-                                                 (_current_stream or _stream)() if stream is None else _stream(stream), pdl)
+    rc = (_lib or lib()).mc_sm100_logits_process(_pack_logits(48, n_rows, vocab, row_stride, out_stride, index_base, _a(logits), _a(out), _a(cfg)),
+                                                 tables, (_current_stream or _stream)() if stream is None else _stream(stream), pdl)
     if rc:
         _check(rc)
 
@@ -387,9 +384,8 @@ def token_history(counts, seen, tokens, n_seqs, table_vocab, offsets=None, promp
         n_tokens = tokens.numel()
     if n_slots is None:
         n_slots = counts.numel() // table_vocab
-    rc = (_lib or lib()).mc_sm100_token_history(_p(counts), _p(seen), n_slots, table_vocab, _p(tokens), n_tokens,
-                                                None if offsets is None else _p(offsets), None if prompt_len is None else _p(prompt_len),
-                                                None if slots is None else _p(slots), n_seqs, rebuild, None if status is None else _p(status),
+    rc = (_lib or lib()).mc_sm100_token_history(_pack_history(80, n_slots, table_vocab, n_tokens, n_seqs, rebuild, _a(counts), _a(seen), _a(tokens),
+                                                              _a(offsets), _a(prompt_len), _a(slots), _a(status)),
                                                 (_current_stream or _stream)() if stream is None else _stream(stream), pdl)
     if rc:
         _check(rc)

@@ -108,20 +108,21 @@ bool aligned_to(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t
 
 using namespace mcl;
 
-extern "C" mc_status_t mc_sm100_linear_epilogue(const void* d_w, const float* d_scale, const uint16_t* d_x, uint16_t* d_y, uint32_t M,
-                                                uint32_t N, uint32_t K, const mc_sm100_epilogue_t* ep, void* stream, int32_t pdl) {
+extern "C" mc_status_t mc_sm100_linear_epilogue(const mc_sm100_linear_epilogue_t* call, void* stream, int32_t pdl) {
     clear_error();
-    const int wb = d_scale == nullptr ? 2 : 1;
-    mc_sm100_epilogue_t d{};
-    if (ep != nullptr) {
-        if (ep->struct_size != sizeof(mc_sm100_epilogue_t) || ep->activation > MC_SM100_ACT_SILU || ep->gated > 1u ||
-            ep->reserved[0] != 0u || ep->reserved[1] != 0u) {
-            set_error("mc_sm100_linear_epilogue: invalid epilogue (struct_size=%u activation=%u gated=%u)", ep->struct_size,
-                      ep->activation, ep->gated);
-            return MC_E_INVALID_ARGUMENT;
-        }
-        d = *ep;
+    if (call == nullptr || call->struct_size != sizeof(mc_sm100_linear_epilogue_t) || call->activation > MC_SM100_ACT_SILU || call->gated > 1u ||
+        call->reserved != 0u) {
+        set_error("mc_sm100_linear_epilogue: invalid call struct (struct_size=%u activation=%u gated=%u)", call ? call->struct_size : 0u,
+                  call ? call->activation : 0u, call ? call->gated : 0u);
+        return MC_E_INVALID_ARGUMENT;
     }
+    const mc_sm100_linear_epilogue_t& d = *call;
+    const void* d_w = d.d_w;
+    const float* d_scale = d.d_scale;
+    const uint16_t* d_x = d.d_x;
+    uint16_t* d_y = d.d_y;
+    const uint32_t M = d.M, N = d.N, K = d.K;
+    const int wb = d_scale == nullptr ? 2 : 1;
     const uint32_t n_out = d.gated ? N / 2u : N;
     const uint32_t xs = d.x_stride ? d.x_stride : K, ys = d.y_stride ? d.y_stride : n_out, rs = d.residual_stride ? d.residual_stride : n_out;
     if (d_w == nullptr || d_x == nullptr || d_y == nullptr || M == 0 || N == 0 || K == 0 || (d.gated && (N & 1u) != 0) || xs < K ||

@@ -362,13 +362,18 @@ extern "C" {
 
 // The kernels of this file wait for the previous kernel before they read anything; they are always launched with the
 // programmatic attribute, which lets their launch and set-up run under its end.
-mc_status_t mc_sm100_logits_process(const uint16_t* d_logits, uint16_t* d_out, uint32_t n_rows, uint32_t vocab, uint32_t row_stride,
-                                    uint32_t out_stride, int32_t index_base, const mc_sm100_logits_config_t* d_cfg,
-                                    const mc_sm100_logits_tables_t* tables, void* stream, int32_t) {
+mc_status_t mc_sm100_logits_process(const mc_sm100_logits_process_t* call, const mc_sm100_logits_tables_t* tables, void* stream, int32_t) {
     clear_error();
     const char* who = "mc_sm100_logits_process";
-    if (d_logits == nullptr || d_out == nullptr || d_cfg == nullptr || tables == nullptr || n_rows == 0 || n_rows > 65535u || vocab == 0 ||
-        vocab > 0x40000000u || row_stride < vocab || out_stride < vocab || index_base < 0 || (d_logits == d_out && row_stride != out_stride)) {
+    if (call == nullptr || call->struct_size != sizeof(mc_sm100_logits_process_t)) {
+        set_error("%s: invalid call struct (struct_size=%u)", who, call ? call->struct_size : 0u);
+        return MC_E_INVALID_ARGUMENT;
+    }
+    const uint32_t n_rows = call->n_rows, vocab = call->vocab, row_stride = call->row_stride, out_stride = call->out_stride;
+    const int32_t index_base = call->index_base;
+    if (call->d_logits == nullptr || call->d_out == nullptr || call->d_cfg == nullptr || tables == nullptr || n_rows == 0 || n_rows > 65535u ||
+        vocab == 0 || vocab > 0x40000000u || row_stride < vocab || out_stride < vocab || index_base < 0 ||
+        (call->d_logits == call->d_out && row_stride != out_stride) || ((reinterpret_cast<uintptr_t>(call->d_logits) | reinterpret_cast<uintptr_t>(call->d_out)) & 1u) != 0u) {
         set_error("%s: invalid args (rows=%u vocab=%u strides=%u,%u index_base=%d)", who, n_rows, vocab, row_stride, out_stride, index_base);
         return MC_E_INVALID_ARGUMENT;
     }
@@ -380,25 +385,29 @@ mc_status_t mc_sm100_logits_process(const uint16_t* d_logits, uint16_t* d_out, u
                   t.table_vocab, t.n_slots, t.n_masks, t.n_bias, index_base, (unsigned long long)((uint64_t)index_base + vocab));
         return MC_E_INVALID_ARGUMENT;
     }
-    const LogitsArgs a{d_logits, d_out, vocab, row_stride, out_stride, index_base, d_cfg, t};
+    const LogitsArgs a{call->d_logits, call->d_out, vocab, row_stride, out_stride, index_base, call->d_cfg, t};
     (void)launch(logits_process_kernel, dim3((vocab + kPiece - 1u + kSpan - 1u) / kSpan, n_rows), dim3(kLogitsThreads), 0,
                  (cudaStream_t)stream, true, a);
     MCL_CHECK_LAUNCH("logits_process");
     return MC_OK;
 }
 
-mc_status_t mc_sm100_token_history(int32_t* d_counts, uint32_t* d_seen, uint32_t n_slots, uint32_t table_vocab, const int32_t* d_tokens,
-                                   uint32_t n_tokens, const uint32_t* d_offsets, const uint32_t* d_prompt_len, const int32_t* d_slots,
-                                   uint32_t n_seqs, int32_t rebuild, int32_t* d_status, void* stream, int32_t) {
+mc_status_t mc_sm100_token_history(const mc_sm100_token_history_t* call, void* stream, int32_t) {
     clear_error();
-    if (d_counts == nullptr || d_seen == nullptr || n_slots == 0 || n_slots > 0x7FFFFFFFu || table_vocab == 0 || table_vocab > 0x40000000u ||
-        (d_tokens == nullptr && n_tokens != 0u) || n_seqs == 0 || n_seqs > 0x7FFFFFFFu || (d_offsets == nullptr && n_tokens < n_seqs) ||
-        (d_slots == nullptr && n_seqs > n_slots)) {
-        set_error("mc_sm100_token_history: invalid args (slots=%u vocab=%u tokens=%u sequences=%u)", n_slots, table_vocab, n_tokens, n_seqs);
+    if (call == nullptr || call->struct_size != sizeof(mc_sm100_token_history_t) || call->rebuild > 1u) {
+        set_error("mc_sm100_token_history: invalid call struct (struct_size=%u rebuild=%u)", call ? call->struct_size : 0u, call ? call->rebuild : 0u);
         return MC_E_INVALID_ARGUMENT;
     }
-    const HistoryArgs a{d_counts, d_seen, n_slots, table_vocab, d_tokens, n_tokens, d_offsets, d_prompt_len, d_slots, d_status};
-    if (rebuild != 0) {
+    const mc_sm100_token_history_t& d = *call;
+    const uint32_t n_seqs = d.n_seqs, table_vocab = d.table_vocab;
+    if (d.d_counts == nullptr || d.d_seen == nullptr || d.n_slots == 0 || d.n_slots > 0x7FFFFFFFu || table_vocab == 0 || table_vocab > 0x40000000u ||
+        (d.d_tokens == nullptr && d.n_tokens != 0u) || n_seqs == 0 || n_seqs > 0x7FFFFFFFu || (d.d_offsets == nullptr && d.n_tokens < n_seqs) ||
+        (d.d_slots == nullptr && n_seqs > d.n_slots)) {
+        set_error("mc_sm100_token_history: invalid args (slots=%u vocab=%u tokens=%u sequences=%u)", d.n_slots, table_vocab, d.n_tokens, n_seqs);
+        return MC_E_INVALID_ARGUMENT;
+    }
+    const HistoryArgs a{d.d_counts, d.d_seen, d.n_slots, table_vocab, d.d_tokens, d.n_tokens, d.d_offsets, d.d_prompt_len, d.d_slots, d.d_status};
+    if (d.rebuild != 0u) {
         // Spans of 2048 to 16384 tokens: as many CTAs as two rounds of SMs, and no more (each reads the whole token list).
         const uint64_t spans = (2ull * (uint32_t)sm_count() + n_seqs - 1u) / n_seqs;
         uint64_t span = ((uint64_t)table_vocab + spans - 1u) / spans;
@@ -415,7 +424,7 @@ mc_status_t mc_sm100_token_history(int32_t* d_counts, uint32_t* d_seen, uint32_t
         MCL_CHECK_LAUNCH("history_rebuild");
         return MC_OK;
     }
-    (void)launch(history_add_kernel, dim3(n_seqs, d_offsets != nullptr ? 8 : 1), dim3(kLogitsThreads), 0, (cudaStream_t)stream, true, a);
+    (void)launch(history_add_kernel, dim3(n_seqs, d.d_offsets != nullptr ? 8 : 1), dim3(kLogitsThreads), 0, (cudaStream_t)stream, true, a);
     MCL_CHECK_LAUNCH("history_add");
     return MC_OK;
 }

@@ -1,7 +1,5 @@
 """mc_sm100_linear_epilogue against the formula in 64 bits.  The bound on each element is the oracle's (accumulation,
 activation, one rounding), derived beside it."""
-import ctypes as C
-
 import numpy as np
 import pytest
 
@@ -42,14 +40,16 @@ def test_refusals(pkg):
     with pytest.raises(pkg.McError) as e:                          # in place needs one stride
         call(16, None, 16, 48, 2, 8, 8, residual=48, residual_stride=8, y_stride=16, **ok)
     assert "one buffer" in e.value.message
-    lib, ep = pkg.lib(), pkg.Epilogue(C.sizeof(pkg.Epilogue))
-    for field, value in (("struct_size", 4), ("activation", 5), ("gated", 2)):
-        bad = pkg.Epilogue.from_buffer_copy(ep)
-        setattr(bad, field, value)
-        assert lib.mc_sm100_linear_epilogue(16, None, 16, 16, 1, 8, 8, C.cast(C.byref(bad), C.c_void_p), None, 0) == pkg.MC_E_INVALID_ARGUMENT
-        assert "invalid epilogue" in pkg.last_error()
-    ep.reserved[1] = 1
-    assert lib.mc_sm100_linear_epilogue(16, None, 16, 16, 1, 8, 8, C.cast(C.byref(ep), C.c_void_p), None, 0) == pkg.MC_E_INVALID_ARGUMENT
+    # the struct itself: size, activation, gate, reserved word
+    lib, good = pkg.lib(), [88, 1, 8, 8, 0, 0, 0, 0, 0, 0, 16, 0, 16, 16, 0, 0]
+    for field, value in ((0, 84), (4, 5), (5, 2), (9, 1)):
+        bad = list(good)
+        bad[field] = value
+        assert lib.mc_sm100_linear_epilogue(pkg.LINEAR_CALL.pack(*bad), None, 0) == pkg.MC_E_INVALID_ARGUMENT
+        assert "invalid call struct" in pkg.last_error()
+    assert lib.mc_sm100_linear_epilogue(None, None, 0) == pkg.MC_E_INVALID_ARGUMENT
+    with pytest.raises(KeyError):
+        call(16, None, 16, 16, 1, 8, 8, activation="swish", **ok)
 
 
 def test_tile_plan(pkg):

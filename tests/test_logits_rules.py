@@ -1,7 +1,5 @@
 """mc_sm100_logits_process bit for bit against the fp32 restatement of its stated order (and within rounding of 64 bits),
 mc_sm100_token_history exactly, and a step that uses both with the linears and the sampler around them."""
-import ctypes as C
-
 import numpy as np
 import pytest
 
@@ -22,11 +20,11 @@ def test_restatement_known_answers():
     assert counts.tolist() == [[9] * 4, [0, 0, 2, 0]] and seen[1].tolist() == [True, False, True, False]
 
 
+FIELDS = ("struct_size", "table_vocab", "n_slots", "n_masks", "n_bias", "reserved", "d_counts", "d_seen", "d_mask", "d_bias_token", "d_bias_value", "d_status")
+
+
 def _tables(pkg, **kw):
-    t = pkg.LogitsTables(struct_size=C.sizeof(pkg.LogitsTables), table_vocab=100)
-    for k, v in kw.items():
-        setattr(t, k, v)
-    return t
+    return pkg.LOGITS_TABLES.pack(*[{"struct_size": 72, "table_vocab": 100, **kw}.get(f, 0) for f in FIELDS])
 
 
 def test_logits_refusals(pkg):
@@ -42,8 +40,13 @@ def test_logits_refusals(pkg):
               dict(n_bias=3, d_bias_token=16)):
         assert "invalid tables" in call(t=_tables(pkg, **t)), t
     assert "invalid tables" in call(base=1)                        # columns beyond the tables' vocabulary
-    lib = pkg.lib()
-    assert lib.mc_sm100_logits_process(16, 16, 1, 8, 8, 8, 0, 16, None, None, 0) == pkg.MC_E_INVALID_ARGUMENT
+    assert "invalid args" in call(logits=17) and "invalid args" in call(out=17)
+    lib, good = pkg.lib(), [48, 1, 8, 8, 8, 0, 16, 16, 16]
+    assert lib.mc_sm100_logits_process(pkg.LOGITS_CALL.pack(*good), None, None, 0) == pkg.MC_E_INVALID_ARGUMENT
+    assert lib.mc_sm100_logits_process(None, _tables(pkg), None, 0) == pkg.MC_E_INVALID_ARGUMENT
+    good[0] = 40
+    assert lib.mc_sm100_logits_process(pkg.LOGITS_CALL.pack(*good), _tables(pkg), None, 0) == pkg.MC_E_INVALID_ARGUMENT
+    assert "struct_size=40" in pkg.last_error()
 
 
 def test_history_refusals(pkg):
@@ -53,6 +56,10 @@ def test_history_refusals(pkg):
         with pytest.raises(pkg.McError) as e:
             pkg.token_history(**{**base, **kw}, stream=16)
         assert e.value.status == pkg.MC_E_INVALID_ARGUMENT and "invalid args" in e.value.message, kw
+    for head in ((76, 2, 10, 2, 2, 0), (80, 2, 10, 2, 2, 2)):
+        assert pkg.lib().mc_sm100_token_history(pkg.HISTORY_CALL.pack(*head, 16, 16, 16, 0, 0, 0, 0), None, 0) == pkg.MC_E_INVALID_ARGUMENT
+        assert "invalid call struct" in pkg.last_error()
+    assert pkg.lib().mc_sm100_token_history(None, None, 0) == pkg.MC_E_INVALID_ARGUMENT
 
 
 # ---- GPU: logits -----------------------------------------------------------------------------------------------------
