@@ -282,6 +282,24 @@ __global__ void __launch_bounds__(THREADS, MINB) gemv_fast_kernel(const RowsArgs
     const bool tagged = a.sh.in_tagged != 0u;
     const uint32_t in_tag = tagged ? shard_tag(a.sh, a.sh.in_seq_mul, a.sh.in_seq_add) : 0u;
 
+    // Fused epilogue: biases and residuals of all of this CTA's groups, group blockIdx.x + i * gridDim.x at entry i.  (Loaded
+    // group by group in the loop below they cost it registers, and so weights in flight: lm_head 103 us against 85.)  Each
+    // thread's first of them is asked for ahead of the activation.
+    const uint32_t cta_groups = FUSED && blockIdx.x < groups ? (groups - blockIdx.x + gridDim.x - 1u) / gridDim.x : 0u;
+    uint16_t* s_bias = xb + K;
+    uint16_t* s_res = s_bias + cta_groups * R;
+    auto bias_of = [&](uint32_t i) {
+        const uint32_t row = (blockIdx.x + i / R * gridDim.x) * R + i % R;
+        return a.ep.bias != nullptr && i < cta_groups * R && row < a.N ? a.ep.bias[row] : (uint16_t)0;
+    };
+    auto res_of = [&](uint32_t i) {
+        const uint32_t out = (blockIdx.x + i / OUTS * gridDim.x) * OUTS + i % OUTS;
+        const bool in = a.ep.res != nullptr && i < cta_groups * OUTS && out < (EPI == EPI_FUSED_GATED ? a.N / 2u : a.N);
+        return in ? a.ep.res[out] : (uint16_t)0x8000u;                               // -0 leaves every sum as it is
+    };
+    uint16_t first_bias = 0, first_res = 0;
+    if constexpr (FUSED) { first_bias = bias_of(threadIdx.x); first_res = res_of(threadIdx.x); }
+
     // ---- activation: global -> (prologue) -> shared, eight elements per thread and step ----
     bool inexact = false;
     const uint32_t nchunk = K / 8u;
@@ -350,21 +368,11 @@ __global__ void __launch_bounds__(THREADS, MINB) gemv_fast_kernel(const RowsArgs
             put_x8<WB>(xh, xb, c, bits, inexact);
         }
     }
-    // Fused epilogue: biases and residuals of all of this CTA's groups, group blockIdx.x + i * gridDim.x at entry i.  (Loaded
-    // group by group in the loop below they cost it registers, and so weights in flight: lm_head 103 us against 88.)
-    const uint32_t cta_groups = FUSED && blockIdx.x < groups ? (groups - blockIdx.x + gridDim.x - 1u) / gridDim.x : 0u;
-    uint16_t* s_bias = xb + K;
-    uint16_t* s_res = s_bias + cta_groups * R;
     if constexpr (FUSED) {
-        const uint32_t outs = EPI == EPI_FUSED_GATED ? a.N / 2u : a.N;
-        for (uint32_t i = threadIdx.x; i < cta_groups * R; i += THREADS) {
-            const uint32_t row = (blockIdx.x + i / R * gridDim.x) * R + i % R;
-            s_bias[i] = a.ep.bias != nullptr && row < a.N ? a.ep.bias[row] : (uint16_t)0;
-        }
-        for (uint32_t i = threadIdx.x; i < cta_groups * OUTS; i += THREADS) {
-            const uint32_t out = (blockIdx.x + i / OUTS * gridDim.x) * OUTS + i % OUTS;
-            s_res[i] = a.ep.res != nullptr && out < outs ? a.ep.res[out] : (uint16_t)0x8000u;   // -0 leaves every sum as it is
-        }
+        if (threadIdx.x < cta_groups * R) s_bias[threadIdx.x] = first_bias;
+        if (threadIdx.x < cta_groups * OUTS) s_res[threadIdx.x] = first_res;
+        for (uint32_t i = threadIdx.x + THREADS; i < cta_groups * R; i += THREADS) s_bias[i] = bias_of(i);
+        for (uint32_t i = threadIdx.x + THREADS; i < cta_groups * OUTS; i += THREADS) s_res[i] = res_of(i);
     }
     const bool fallback = __syncthreads_or(inexact ? 1 : 0) != 0;   // also the staging barrier
 
