@@ -305,6 +305,19 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint32_t per_n = kTileN / S;                               // features per owner (S divides 128)
     constexpr uint32_t PITCH = NPAD + 4;                             // fp32 per feature row: 16-byte aligned pushes, spread banks
     const uint32_t part_s = base + G::bytes(OPS, E4 ? RAWS : 0);     // part[S][per_n][PITCH] fp32
+    // fused epilogue: this thread's outputs (the slice is a power of two wide), and its first residuals under the products
+    const uint32_t e_gate = EXT ? a.ep.gated : 0u, e_outs = per_n >> e_gate, e_shift = 31u - (uint32_t)__clz((int)e_outs);
+    const uint32_t e_base = ((uint32_t)n0 + rank * per_n) >> e_gate, e_limit = a.N >> e_gate;
+    auto res_of = [&](uint32_t idx) {
+        const uint32_t m = idx >> e_shift, j = e_base + (idx & (e_outs - 1u));
+        return a.ep.res != nullptr && m < a.M && j < e_limit ? a.ep.res[(size_t)m * a.ep.res_stride + j] : (uint16_t)0x8000u;   // -0 changes no sum
+    };
+    uint16_t e_res[4] = {0x8000u, 0x8000u, 0x8000u, 0x8000u};
+    if constexpr (EXT) {
+        pdl_wait();   // the residual may be the previous kernel's: every thread that reads it waits for itself
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) e_res[e] = res_of(tid + e * kThreads);
+    }
     asm volatile("barrier.cluster.wait;" ::: "memory");              // completes the arrive of the prologue
     if (warp >= 2 && warp < 6) {
         const uint32_t q = warp & 3u;       // the TMEM lane quarter this warp may read
@@ -380,10 +393,7 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             return f32_to_bf16_bits(swiglu_f32(gb, ub));
         };
         if constexpr (EXT) {
-            pdl_wait();   // the residual may be the previous kernel's: every thread that reads it waits for itself
-            // one output per thread and turn, features fastest; the slice is a power of two wide
-            const uint32_t gate = a.ep.gated, outs = per_n >> gate, sh = 31u - (uint32_t)__clz((int)outs);
-            const uint32_t obase = nbase >> gate, olimit = a.N >> gate;
+            // one output per thread and turn, features fastest; residuals four turns ahead
             auto z_of = [&](uint32_t n_rel, uint32_t m) {
                 float z = partial_sum(n_rel, m);
                 const uint32_t n = nbase + n_rel;
@@ -391,14 +401,14 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 if (a.ep.bias != nullptr) z += __uint_as_float((uint32_t)a.ep.bias[n] << 16);
                 return z;
             };
-            for (uint32_t idx = tid; idx < outs * a.M; idx += kThreads) {
-                const uint32_t m = idx >> sh, j_rel = idx & (outs - 1u), j = obase + j_rel;
-                if (j < olimit && !failed) {
-                    float r = -0.f;
-                    if (a.ep.res != nullptr) r = __uint_as_float((uint32_t)a.ep.res[(size_t)m * a.ep.res_stride + j] << 16);
-                    const float v = gate ? epi_act(z_of(2u * j_rel, m), a.ep.act) * z_of(2u * j_rel + 1u, m) : epi_act(z_of(j_rel, m), a.ep.act);
-                    a.y[(size_t)m * a.ep.y_stride + j] = f32_to_bf16_bits(v + r);
+            for (uint32_t idx = tid; idx < e_outs * a.M; idx += kThreads) {
+                const uint32_t m = idx >> e_shift, j_rel = idx & (e_outs - 1u), j = e_base + j_rel;
+                const uint16_t next = res_of(idx + 4u * kThreads);
+                if (j < e_limit && !failed) {
+                    const float z = z_of(j_rel << e_gate, m), v = epi_act(z, a.ep.act) * (e_gate ? z_of(2u * j_rel + 1u, m) : 1.0f);
+                    a.y[(size_t)m * a.ep.y_stride + j] = f32_to_bf16_bits(v + __uint_as_float((uint32_t)e_res[0] << 16));
                 }
+                e_res[0] = e_res[1]; e_res[1] = e_res[2]; e_res[2] = e_res[3]; e_res[3] = next;
             }
         } else if (a.out.world != 0u) {
             // pairs of adjacent outputs (the slice holds an even number of them, starting at an even column)
