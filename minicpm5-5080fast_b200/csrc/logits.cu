@@ -263,32 +263,33 @@ __device__ __forceinline__ bool history_seq(const HistoryArgs& a, uint32_t seq, 
 // writes each count and seen bit once: no clearing pass, no global atomics, one launch; the token
 // list is read once per span (from L2 after the first).  Of several sequences that name a slot the first owns it and the
 // others add to its counts.
-constexpr uint32_t kHistThreads = 512;
+constexpr uint32_t kHistThreads = 256;
 
-__global__ void __launch_bounds__(kHistThreads) history_rebuild_kernel(const HistoryArgs a, uint32_t n_seqs, uint32_t span) {
+__global__ void __launch_bounds__(kHistThreads, 4) history_rebuild_kernel(const HistoryArgs a, uint32_t n_seqs, uint32_t span) {
     extern __shared__ __align__(16) int32_t s_hist[];            // [span + 4] counts, [span / 32] seen bits
     __shared__ uint32_t s_same[kHistThreads / 32];
     pdl_trigger();
     pdl_wait();
     const uint32_t seq = blockIdx.x, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     uint32_t slot, lo, hi;
-    if (!history_seq(a, seq, slot, lo, hi)) return;
+    const bool valid = history_seq(a, seq, slot, lo, hi);
+    for (uint32_t i = tid; i < (span + 4u + span / 32u + 3u) / 4u; i += kHistThreads) reinterpret_cast<uint4*>(s_hist)[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (!valid) return;
     const uint32_t t0 = blockIdx.y * span, t1 = min(a.vocab, t0 + span);
     // counts stand in shared memory as far from a 16-byte boundary as in the table: rows of any length go out 16 bytes at a time
     int32_t* row = a.counts + (size_t)slot * a.vocab + t0;
     const uint32_t shift = (uint32_t)((reinterpret_cast<uintptr_t>(row) & 15u) >> 2);
     int32_t* s_count = s_hist + shift;
     uint32_t* s_seen = reinterpret_cast<uint32_t*>(s_hist + span + 4u);
-    for (uint32_t i = tid; i < (span + 4u + span / 32u + 3u) / 4u; i += kHistThreads) reinterpret_cast<uint4*>(s_hist)[i] = make_uint4(0u, 0u, 0u, 0u);
     auto add = [&](uint32_t which, uint32_t l, uint32_t h) {
         const uint32_t n = h - l, prompt = a.prompt_len != nullptr ? a.prompt_len[which] : 0u;
         const int32_t* src = a.tokens + l;
-        for (uint32_t k0 = tid; k0 < n; k0 += kHistThreads * 8u) {
-            uint32_t tok[8];
+        for (uint32_t k0 = tid; k0 < n; k0 += kHistThreads * 16u) {
+            uint32_t tok[16];
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) tok[e] = k0 + e * kHistThreads < n ? (uint32_t)src[k0 + e * kHistThreads] : 0xFFFFFFFFu;
+            for (uint32_t e = 0; e < 16; ++e) tok[e] = k0 + e * kHistThreads < n ? (uint32_t)src[k0 + e * kHistThreads] : 0xFFFFFFFFu;
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) {
+            for (uint32_t e = 0; e < 16; ++e) {
                 if (tok[e] < t0 || tok[e] >= t1) continue;
                 const uint32_t t = tok[e] - t0;
                 atomicOr(s_seen + t / 32u, 1u << (t & 31u));
@@ -408,10 +409,11 @@ mc_status_t mc_sm100_token_history(const mc_sm100_token_history_t* call, void* s
     }
     const HistoryArgs a{d.d_counts, d.d_seen, d.n_slots, table_vocab, d.d_tokens, d.n_tokens, d.d_offsets, d.d_prompt_len, d.d_slots, d.d_status};
     if (d.rebuild != 0u) {
-        // Spans of 2048 to 16384 tokens: as many CTAs as two rounds of SMs, and no more (each reads the whole token list).
-        const uint64_t spans = (2ull * (uint32_t)sm_count() + n_seqs - 1u) / n_seqs;
-        uint64_t span = ((uint64_t)table_vocab + spans - 1u) / spans;
-        span = span < 2048u ? 2048u : (span > 16384u ? 16384u : (span + 31u) & ~(uint64_t)31u);
+        // One round of CTAs, four to an SM (512 threads, 56 KB each) where the batch allows it: spans of 2048 to 13664 tokens.
+        // 64 slots of 122753: 9 spans, 576 CTAs in one round; with spans of 16384 (three CTAs to an SM, two rounds) 13.5 us.
+        const uint64_t spans = 4ull * (uint32_t)sm_count() / n_seqs;
+        uint64_t span = spans == 0 ? table_vocab : ((uint64_t)table_vocab + spans - 1u) / spans;
+        span = span < 2048u ? 2048u : (span > 13664u ? 13664u : (span + 31u) & ~(uint64_t)31u);
         const size_t bytes = ((size_t)span + 4u) * 4u + (size_t)span / 8u + 16u;
         static SmemOptIn optin;
         const cudaError_t e = optin.ensure(history_rebuild_kernel, bytes);
