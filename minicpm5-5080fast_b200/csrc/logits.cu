@@ -16,8 +16,8 @@ struct LogitsArgs {
     mc_sm100_logits_tables_t t;
 };
 
-// A CTA owns kSpan consecutive columns of a row (counted from a 16-byte boundary of the output, so that rows of any length
-// and stride are stored in 16-byte pieces but for their ends), a thread two pieces of eight.  Reading and writing the logits
+// A CTA owns kSpan consecutive columns of a row (counted from a 32-byte boundary of the output, so that rows of any length
+// and stride move in 32-byte accesses but for their ends), a thread sixteen.  Reading and writing the logits
 // is 4 bytes a token; seen bits and masks are 1/16 of that, and counts are gathered for seen tokens only.  At full batches the
 // instructions bound it, not the bytes: most tokens are neither seen nor listed and stay the bits that they are, a mask is a
 // select on the packed words (64 rows of 122753 with every rule: 36 us with every token through the fp32 path, 24.5 us with
@@ -25,7 +25,7 @@ struct LogitsArgs {
 // and instructions alike).
 // Biases: the entries that fall into the span are kept in list order in shared memory; the thread of a token's first entry
 // adds up the others behind it: a fixed order, no floating-point atomics, any list length (512 entries at a time).
-constexpr uint32_t kPiece = 8, kPieces = 2, kSpan = kLogitsThreads * kPiece * kPieces, kBiasBatch = 2 * kLogitsThreads, kFew = 64;
+constexpr uint32_t kOwn = 16, kSpan = kLogitsThreads * kOwn, kBiasBatch = 2 * kLogitsThreads, kFew = 64;
 
 __global__ void __launch_bounds__(kLogitsThreads, 5) logits_process_kernel(const LogitsArgs a) {
     __shared__ __align__(16) uint32_t s_column[kBiasBatch + 4];
@@ -39,26 +39,21 @@ __global__ void __launch_bounds__(kLogitsThreads, 5) logits_process_kernel(const
     const mc_sm100_logits_config_t c = a.cfg[row];
     const uint16_t* in = a.in + (size_t)row * a.row_stride;
     uint16_t* out = a.out + (size_t)row * a.out_stride;
-    // piece p: columns first[p] .. + 7; those below 0 or beyond the row are not there
-    const int32_t head = (int32_t)((reinterpret_cast<uintptr_t>(out) & 15u) >> 1), vocab = (int32_t)a.vocab;
-    const int32_t span0 = (int32_t)(blockIdx.x * kSpan) - head;
-    int32_t first[kPieces];
-    uint32_t raw[kPieces][4];
-    const bool together = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0u;
+    // this thread's columns first .. + 15; those below 0 or beyond the row are not there
+    const int32_t head = (int32_t)((reinterpret_cast<uintptr_t>(out) & 31u) >> 1), vocab = (int32_t)a.vocab;
+    const int32_t span0 = (int32_t)(blockIdx.x * kSpan) - head, first = span0 + (int32_t)(tid * kOwn);
+    const bool together = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 31u) == 0u;
+    const bool whole = first >= 0 && first + (int32_t)kOwn <= vocab;
+    uint32_t raw[8];
+    if (together && whole) {
+        asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(raw[0]), "=r"(raw[1]), "=r"(raw[2]), "=r"(raw[3]), "=r"(raw[4]), "=r"(raw[5]), "=r"(raw[6]), "=r"(raw[7]) : "l"(in + first));
+    } else {
 #pragma unroll
-    for (uint32_t p = 0; p < kPieces; ++p) {
-        first[p] = span0 + (int32_t)((p * kLogitsThreads + tid) * kPiece);
-        const int32_t f = first[p];
-        if (together && f >= 0 && f + (int32_t)kPiece <= vocab) {
-            const uint4 v = *reinterpret_cast<const uint4*>(in + f);
-            raw[p][0] = v.x; raw[p][1] = v.y; raw[p][2] = v.z; raw[p][3] = v.w;
-        } else {
+        for (int k = 0; k < 8; ++k) raw[k] = 0u;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) raw[p][k] = 0u;
-#pragma unroll
-            for (int e = 0; e < (int)kPiece; ++e)
-                if (f + e >= 0 && f + e < vocab) raw[p][e >> 1] |= (uint32_t)in[f + e] << (16 * (e & 1));
-        }
+        for (int e = 0; e < (int)kOwn; ++e)
+            if (first + e >= 0 && first + e < vocab) raw[e >> 1] |= (uint32_t)in[first + e] << (16 * (e & 1));
     }
     const uint32_t words = (a.t.table_vocab + 31u) / 32u;
     const bool history = c.history_slot >= 0 && (uint32_t)c.history_slot < a.t.n_slots;
@@ -67,21 +62,17 @@ __global__ void __launch_bounds__(kLogitsThreads, 5) logits_process_kernel(const
     if (a.t.d_status != nullptr && blockIdx.x == 0u && tid == 0u &&
         ((c.history_slot >= 0 && !history) || (c.mask_row >= 0 && !masked) || (c.bias_count != 0u && end64 > a.t.n_bias)))
         *a.t.d_status = 1;
-    // the bits of a table row that belong to a piece, bit e = column first + e, 0 where there is none
-    auto bits_of = [&](const uint32_t* table_row, int32_t f) -> uint32_t {
-        const int32_t lo = f < 0 ? 0 : f, hi = f + (int32_t)kPiece < vocab ? f + (int32_t)kPiece : vocab;
-        if (hi <= lo) return 0u;
-        const uint32_t t0 = (uint32_t)(a.index_base + lo), t1 = (uint32_t)(a.index_base + hi - 1);
-        const uint32_t w0 = table_row[t0 >> 5], w1 = table_row[t1 >> 5];
-        return (__funnelshift_r(w0, w1, t0 & 31u) & ((1u << (hi - lo)) - 1u)) << (lo - f);
+    // the bits of a table row that belong to the columns, bit e = column first + e, 0 where there is none
+    const int32_t c_lo = first < 0 ? 0 : first, c_hi = first + (int32_t)kOwn < vocab ? first + (int32_t)kOwn : vocab;
+    const uint32_t bit0 = (uint32_t)(a.index_base + c_lo), bit1 = (uint32_t)(a.index_base + c_hi - 1);
+    auto bits_of = [&](const uint32_t* table_row) -> uint32_t {
+        if (c_hi <= c_lo) return 0u;
+        const uint32_t w0 = table_row[bit0 >> 5], w1 = table_row[bit1 >> 5];
+        return (__funnelshift_r(w0, w1, bit0 & 31u) & ((1u << (c_hi - c_lo)) - 1u)) << (c_lo - first);
     };
-    uint32_t seen[kPieces], allowed[kPieces], listed[kPieces];
-#pragma unroll
-    for (uint32_t p = 0; p < kPieces; ++p) {
-        seen[p] = history ? bits_of(a.t.d_seen + (size_t)c.history_slot * words, first[p]) : 0u;
-        allowed[p] = masked ? bits_of(a.t.d_mask + (size_t)c.mask_row * words, first[p]) : 0xFFu;
-        listed[p] = 0u;
-    }
+    const uint32_t seen = history ? bits_of(a.t.d_seen + (size_t)c.history_slot * words) : 0u;
+    const uint32_t allowed = masked ? bits_of(a.t.d_mask + (size_t)c.mask_row * words) : 0xFFFFu;
+    uint32_t listed = 0u;
     const uint64_t end = end64 < a.t.n_bias ? end64 : a.t.n_bias;
     if (c.bias_begin < end) {                                                        // the same for every thread
         const int32_t lo = span0 < 0 ? 0 : span0, hi = span0 + (int32_t)kSpan < vocab ? span0 + (int32_t)kSpan : vocab;
@@ -150,11 +141,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 5) logits_process_kernel(const
             }
             __syncthreads();
         }
-#pragma unroll
-        for (uint32_t p = 0; p < kPieces; ++p) {
-            const uint32_t at = (p * kLogitsThreads + tid) * kPiece;
-            listed[p] = (s_listed[at >> 5] >> (at & 31u)) & 0xFFu;
-        }
+        listed = (s_listed[tid >> 1] >> (16u * (tid & 1u))) & 0xFFFFu;
     }
     // one reciprocal a row instead of a division a token: off by 2^-24 of the value, in front of a rounding of 2^-9
     const float grow = c.rep_penalty != 0.f ? c.rep_penalty : 1.f, shrink = __frcp_rn(grow);
@@ -164,51 +151,54 @@ __global__ void __launch_bounds__(kLogitsThreads, 5) logits_process_kernel(const
         l = n > 0 ? __fsub_rn(__fsub_rn(l, __fmul_rn(c.freq_penalty, (float)n)), c.pres_penalty) : l;
         return has_bias ? __fadd_rn(l, b) : l;
     };
-    // a banned token's value does not matter any more
-    uint32_t touched[kPieces];
-#pragma unroll
-    for (uint32_t p = 0; p < kPieces; ++p) touched[p] = (seen[p] | listed[p]) & allowed[p];
+    const uint32_t touched = (seen | listed) & allowed;          // a banned token's value does not matter any more
     // Few touched tokens in the warp (nearly everywhere but among a vocabulary's most frequent tokens): every piece goes out
-    // under its mask, then the touched tokens are edited one a lane.  Many: each lane edits its pieces, eight tokens side by side.
-    static_assert(kPieces == 2, "two pieces a thread");
-    const uint32_t mine = __popc(touched[0]) + __popc(touched[1]), total = __reduce_add_sync(0xFFFFFFFFu, mine);
+    // under its mask, then the touched tokens are edited one a lane.  Many: each lane edits its own, eight side by side.
+    const uint32_t mine = __popc(touched), total = __reduce_add_sync(0xFFFFFFFFu, mine);
     const bool few = total <= kFew;
+    uint32_t res[8];
 #pragma unroll
-    for (uint32_t p = 0; p < kPieces; ++p) {
-        const int32_t f = first[p];
-        uint32_t res[4] = {raw[p][0], raw[p][1], raw[p][2], raw[p][3]};
-        if (!few && touched[p] != 0u) {
-            int32_t n_of[kPiece];
-            float add[kPiece];
+    for (int k = 0; k < 8; ++k) res[k] = raw[k];
+    if (!few) {
 #pragma unroll
-            for (int e = 0; e < (int)kPiece; ++e) n_of[e] = ((seen[p] & touched[p]) >> e) & 1u ? counts[f + e] : 0;
-            const float4 b0 = *reinterpret_cast<const float4*>(s_sum + (p * kLogitsThreads + tid) * kPiece);
-            const float4 b1 = *reinterpret_cast<const float4*>(s_sum + (p * kLogitsThreads + tid) * kPiece + 4);
+        for (uint32_t h = 0; h < 2; ++h) {
+            const uint32_t t = touched >> (8u * h), s = seen >> (8u * h), b = listed >> (8u * h);
+            if ((t & 0xFFu) == 0u) continue;
+            const uint32_t at = tid * kOwn + 8u * h;
+            int32_t n_of[8];
+            float add[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) n_of[e] = ((s & t) >> e) & 1u ? counts[span0 + (int32_t)at + e] : 0;
+            const float4 b0 = *reinterpret_cast<const float4*>(s_sum + at), b1 = *reinterpret_cast<const float4*>(s_sum + at + 4);
             add[0] = b0.x; add[1] = b0.y; add[2] = b0.z; add[3] = b0.w; add[4] = b1.x; add[5] = b1.y; add[6] = b1.z; add[7] = b1.w;
 #pragma unroll
-            for (int e = 0; e < (int)kPiece; ++e) {
-                const uint32_t old = (e & 1) ? res[e >> 1] >> 16 : res[e >> 1] & 0xFFFFu;
-                const float l = edit(__uint_as_float(old << 16), (seen[p] >> e) & 1u, n_of[e], (listed[p] >> e) & 1u, add[e]);
-                const uint32_t bits = (touched[p] >> e) & 1u ? f32_to_bf16_bits(l) : old;
-                res[e >> 1] = (e & 1) ? (res[e >> 1] & 0xFFFFu) | (bits << 16) : (res[e >> 1] & 0xFFFF0000u) | bits;
+            for (int e = 0; e < 8; ++e) {
+                uint32_t& word = res[4 * h + (e >> 1)];
+                const uint32_t old = (e & 1) ? word >> 16 : word & 0xFFFFu;
+                const float l = edit(__uint_as_float(old << 16), (s >> e) & 1u, n_of[e], (b >> e) & 1u, add[e]);
+                const uint32_t bits = (t >> e) & 1u ? f32_to_bf16_bits(l) : old;
+                word = (e & 1) ? (word & 0xFFFFu) | (bits << 16) : (word & 0xFFFF0000u) | bits;
             }
         }
-        if (masked) {
+    }
+    if (masked) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t keep = ((allowed[p] >> (2 * k)) & 1u) * 0xFFFFu + ((allowed[p] >> (2 * k + 1)) & 1u) * 0xFFFF0000u;
-                res[k] = (res[k] & keep) | (0xFF80FF80u & ~keep);                    // -infinity
-            }
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t keep = ((allowed >> (2 * k)) & 1u) * 0xFFFFu + ((allowed >> (2 * k + 1)) & 1u) * 0xFFFF0000u;
+            res[k] = (res[k] & keep) | (0xFF80FF80u & ~keep);                        // -infinity
         }
-        if (f >= 0 && f + (int32_t)kPiece <= vocab) {
-            // in place, a piece that stays as it was is not written
-            if (in != out || res[0] != raw[p][0] || res[1] != raw[p][1] || res[2] != raw[p][2] || res[3] != raw[p][3])
-                *reinterpret_cast<uint4*>(out + f) = make_uint4(res[0], res[1], res[2], res[3]);
-        } else {
+    }
+    if (whole) {
+        uint32_t changed = in != out ? 1u : 0u;                  // in place, what stays as it was is not written
 #pragma unroll
-            for (int e = 0; e < (int)kPiece; ++e)
-                if (f + e >= 0 && f + e < vocab) out[f + e] = (uint16_t)(res[e >> 1] >> (16 * (e & 1)));
-        }
+        for (int k = 0; k < 8; ++k) changed |= res[k] ^ raw[k];
+        if (changed != 0u)
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out + first), "r"(res[0]), "r"(res[1]), "r"(res[2]), "r"(res[3]),
+                         "r"(res[4]), "r"(res[5]), "r"(res[6]), "r"(res[7]) : "memory");
+    } else {
+#pragma unroll
+        for (int e = 0; e < (int)kOwn; ++e)
+            if (first + e >= 0 && first + e < vocab) out[first + e] = (uint16_t)(res[e >> 1] >> (16 * (e & 1)));
     }
     if (!few || total == 0u) return;
     uint32_t upto = mine;
@@ -218,15 +208,12 @@ __global__ void __launch_bounds__(kLogitsThreads, 5) logits_process_kernel(const
         if (lane >= d) upto += v;
     }
     uint32_t at = upto - mine;
-#pragma unroll
-    for (uint32_t p = 0; p < kPieces; ++p)
-        for (uint32_t t = touched[p]; t != 0u; t &= t - 1u, ++at) {
-            const uint32_t e = (uint32_t)__ffs((int)t) - 1u;
-            const uint32_t value = (e & 1u ? 0xFFFF0000u : 0xFFFFu) & (e < 4u ? (e < 2u ? raw[p][0] : raw[p][1]) : (e < 6u ? raw[p][2] : raw[p][3]));
-            s_touched[warp][at] = make_uint2(((p * kLogitsThreads + tid) * kPiece + e) | (((seen[p] >> e) & 1u) << 30) | (((listed[p] >> e) & 1u) << 31),
-                                             e & 1u ? value : value << 16);
-        }
-    __syncwarp();                                                // the list, and the pieces stored above, are the whole warp's
+    for (uint32_t t = touched; t != 0u; t &= t - 1u, ++at) {
+        const uint32_t e = (uint32_t)__ffs((int)t) - 1u, q = e >> 1;
+        const uint32_t w4 = q & 4u ? (q & 2u ? (q & 1u ? raw[7] : raw[6]) : (q & 1u ? raw[5] : raw[4])) : (q & 2u ? (q & 1u ? raw[3] : raw[2]) : (q & 1u ? raw[1] : raw[0]));
+        s_touched[warp][at] = make_uint2((tid * kOwn + e) | (((seen >> e) & 1u) << 30) | (((listed >> e) & 1u) << 31), e & 1u ? w4 & 0xFFFF0000u : w4 << 16);
+    }
+    __syncwarp();                                                // the list, and what was stored above, are the whole warp's
     for (uint32_t k = lane; k < total; k += 32u) {
         const uint2 t = s_touched[warp][k];
         const uint32_t in_span = t.x & 0x3FFFFFFFu;
@@ -387,7 +374,7 @@ mc_status_t mc_sm100_logits_process(const mc_sm100_logits_process_t* call, const
         return MC_E_INVALID_ARGUMENT;
     }
     const LogitsArgs a{call->d_logits, call->d_out, vocab, row_stride, out_stride, index_base, call->d_cfg, t};
-    (void)launch(logits_process_kernel, dim3((vocab + kPiece - 1u + kSpan - 1u) / kSpan, n_rows), dim3(kLogitsThreads), 0,
+    (void)launch(logits_process_kernel, dim3((vocab + kOwn - 1u + kSpan - 1u) / kSpan, n_rows), dim3(kLogitsThreads), 0,
                  (cudaStream_t)stream, true, a);
     MCL_CHECK_LAUNCH("logits_process");
     return MC_OK;
