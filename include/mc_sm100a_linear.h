@@ -299,7 +299,7 @@ typedef struct mc_sm100_linear_epilogue_t {
  *   y[m,j] = bf16( v[m,j] + residual[m,j] )
  * Everything between the products and y stays in fp32: one rounding.  (mc_sm100_gate_up_swiglu rounds gate and up to
  * bf16 first, as the reference's pair of kernels does; this call does not.)  The e4m3 codes 0x7F / 0xFF count as +/-480, as
- * everywhere here.  Any M, N, K >= 1 (gated: N even) and any stride >= the row; operands aligned to their elements.  16-byte
+ * everywhere here.  M, N, K from 1 to 2^30 (gated: N even) and any stride >= the row; operands aligned to their elements.  16-byte
  * aligned d_w and d_x, K * (bytes per weight) and x_stride * 2 multiples of 16 take the kernels that stream; anything else a
  * slower one with plain loads.  y overlaps neither x nor, but for the whole, the residual.  Results do not depend on the
  * launch: no atomics, a fixed order of every sum.
@@ -408,7 +408,7 @@ typedef struct mc_sm100_logits_config_t {
     uint32_t flags;                  /* must be zero */
 } mc_sm100_logits_config_t;
 
-/* Tables over the whole vocabulary (also when the logits are a shard of it).  A table of bits holds token t in bit t % 32
+/* Tables over the whole vocabulary (also when the logits are a shard of it), table_vocab <= 2^28.  A table of bits holds token t in bit t % 32
  * of word t / 32, rows of ceil(table_vocab / 32) words. */
 typedef struct mc_sm100_logits_tables_t {
     uint32_t struct_size;            /* caller sets sizeof(mc_sm100_logits_tables_t) */
@@ -437,7 +437,8 @@ typedef struct mc_sm100_logits_process_t {
  * frequency and presence penalty, biases (a token listed several times takes their sum, added in list order; tokens
  * outside the logits are passed over), grammar mask (a token that is not allowed becomes -infinity, whatever it held, a NaN
  * too).  A row whose mask leaves nothing becomes -infinity throughout.  A row that names a slot, mask or entries outside the
- * tables goes without them, and *d_status says so.  Logits kept for their probabilities go to another buffer.  Columns from
+ * tables goes without them, and *d_status says so.  Logits kept for their probabilities go to another buffer, which then
+ * does not overlap them.  Columns from
  * vocab to the stride are not touched.  Replaces rep_penalty_mark / rep_penalty_apply
  * (native/kernels/sm120/sampling.cu:293-324) in front of mc_sm100_sample_topk_topp / mc_sm100_argmax_bf16; biases, masks
  * and the other two penalties have no counterpart there.  Both structs are copied before the call returns.  Nothing is read

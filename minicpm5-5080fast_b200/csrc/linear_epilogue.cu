@@ -125,7 +125,8 @@ extern "C" mc_status_t mc_sm100_linear_epilogue(const mc_sm100_linear_epilogue_t
     const int wb = d_scale == nullptr ? 2 : 1;
     const uint32_t n_out = d.gated ? N / 2u : N;
     const uint32_t xs = d.x_stride ? d.x_stride : K, ys = d.y_stride ? d.y_stride : n_out, rs = d.residual_stride ? d.residual_stride : n_out;
-    if (d_w == nullptr || d_x == nullptr || d_y == nullptr || M == 0 || N == 0 || K == 0 || (d.gated && (N & 1u) != 0) || xs < K ||
+    constexpr uint32_t kMost = 1u << 30;             // row and column numbers stay in 31 bits, with a tile to spare
+    if (d_w == nullptr || d_x == nullptr || d_y == nullptr || M == 0 || N == 0 || K == 0 || M > kMost || N > kMost || K > kMost || (d.gated && (N & 1u) != 0) || xs < K ||
         ys < n_out || (d.d_residual != nullptr && rs < n_out) || !aligned_to(d_w, (uintptr_t)wb) || !aligned_to(d_scale, 4) ||
         !aligned_to(d_x, 2) || !aligned_to(d_y, 2) || !aligned_to(d.d_bias, 2) || !aligned_to(d.d_residual, 2)) {
         set_error("mc_sm100_linear_epilogue: invalid args (M=%u N=%u K=%u gated=%u x_stride=%u y_stride=%u residual_stride=%u)", M, N, K,

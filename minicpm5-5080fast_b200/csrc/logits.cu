@@ -73,22 +73,25 @@ __global__ void __launch_bounds__(kLogitsThreads, 5) logits_process_kernel(const
     const uint32_t seen = history ? bits_of(a.t.d_seen + (size_t)c.history_slot * words) : 0u;
     const uint32_t allowed = masked ? bits_of(a.t.d_mask + (size_t)c.mask_row * words) : 0xFFFFu;
     uint32_t listed = 0u;
-    const uint64_t end = end64 < a.t.n_bias ? end64 : a.t.n_bias;
-    if (c.bias_begin < end) {                                                        // the same for every thread
+    const uint32_t begin = c.bias_begin, end = (uint32_t)(end64 < a.t.n_bias ? end64 : a.t.n_bias);
+    if (begin < end) {                                                               // the same for every thread
         const int32_t lo = span0 < 0 ? 0 : span0, hi = span0 + (int32_t)kSpan < vocab ? span0 + (int32_t)kSpan : vocab;
-        for (uint32_t w = tid; w < kSpan / 32; w += kLogitsThreads) s_listed[w] = 0u;
-        for (uint64_t j0 = c.bias_begin; j0 < end; j0 += kBiasBatch) {
+        const bool one = end - begin <= kBiasBatch;
+        if (!one)
+            for (uint32_t w = tid; w < kSpan / 32; w += kLogitsThreads) s_listed[w] = 0u;
+        for (uint32_t j0 = begin; j0 < end; j0 = end - j0 > kBiasBatch ? j0 + kBiasBatch : end) {
             uint32_t col[2], hits[2];
             float value[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint64_t j = j0 + h * kLogitsThreads + tid;
+                const uint32_t d = (uint32_t)h * kLogitsThreads + tid;
                 int32_t column = -1;
                 value[h] = 0.f;
                 // tokens and index_base are not negative, or the difference is: no overflow
-                if (j < end) { const int32_t tok = a.t.d_bias_token[j]; column = tok < 0 ? -1 : tok - a.index_base; value[h] = a.t.d_bias_value[j]; }
+                if (d < end - j0) { const int32_t tok = a.t.d_bias_token[j0 + d]; column = tok < 0 ? -1 : tok - a.index_base; value[h] = a.t.d_bias_value[j0 + d]; }
                 col[h] = column >= lo && column < hi ? (uint32_t)(column - span0) : 0xFFFFFFFFu;
             }
+            for (uint32_t w = tid; w < kSpan / 32; w += kLogitsThreads) s_once[w] = s_again[w] = 0u;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 hits[h] = __ballot_sync(0xFFFFFFFFu, col[h] != 0xFFFFFFFFu);
@@ -107,41 +110,35 @@ __global__ void __launch_bounds__(kLogitsThreads, 5) logits_process_kernel(const
             for (int h = 0; h < 2; ++h) {
                 const uint32_t at = h * (kLogitsThreads / 32) + warp, before = __shfl_sync(0xFFFFFFFFu, upto, at) - __popc(hits[h]);
                 if (col[h] != 0xFFFFFFFFu) {
-                    const uint32_t k = before + __popc(hits[h] & ((1u << lane) - 1u));
+                    const uint32_t k = before + __popc(hits[h] & ((1u << lane) - 1u)), bit = 1u << (col[h] & 31u);
                     s_column[k] = col[h]; s_value[k] = value[h];
+                    if (atomicOr(&s_once[col[h] >> 5], bit) & bit) atomicOr(&s_again[col[h] >> 5], bit);
                 }
             }
+            if (tid < 4u) s_column[total + tid] = 0xFFFFFFFFu;                       // the walk reads four at a time
             __syncthreads();
-            if (total != 0u) {                                                       // the same for every thread
-                for (uint32_t w = tid; w < kSpan / 32; w += kLogitsThreads) s_once[w] = s_again[w] = 0u;
-                if (tid < 4u) s_column[total + tid] = 0xFFFFFFFFu;                   // the walk reads four at a time
-                __syncthreads();
-                for (uint32_t k = tid; k < total; k += kLogitsThreads) {
-                    const uint32_t mine = s_column[k], bit = 1u << (mine & 31u);
-                    if (atomicOr(&s_once[mine >> 5], bit) & bit) atomicOr(&s_again[mine >> 5], bit);
-                }
-                __syncthreads();
-                for (uint32_t k = tid; k < total; k += kLogitsThreads) {
-                    const uint32_t mine = s_column[k], bit = 1u << (mine & 31u);
-                    float sum = s_listed[mine >> 5] & bit ? s_sum[mine] : 0.f;       // from the batches before
-                    bool owner = true;
-                    if (s_again[mine >> 5] & bit) {                                  // the first of its entries adds them up in order
-                        for (uint32_t o = 0; o < total; o += 4u) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(s_column + o);
-                            const uint32_t cols[4] = {v.x, v.y, v.z, v.w};
+            for (uint32_t k = tid; k < total; k += kLogitsThreads) {
+                const uint32_t mine = s_column[k], bit = 1u << (mine & 31u);
+                float sum = !one && (s_listed[mine >> 5] & bit) ? s_sum[mine] : 0.f; // from the batches before
+                bool owner = true;
+                if (s_again[mine >> 5] & bit) {                                      // the first of its entries adds them up in order
+                    for (uint32_t o = 0; o < total; o += 4u) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(s_column + o);
+                        const uint32_t cols[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                            for (uint32_t e = 0; e < 4; ++e)
-                                if (cols[e] == mine) { if (o + e < k) owner = false; sum = __fadd_rn(sum, s_value[o + e]); }
-                        }
-                    } else sum = __fadd_rn(sum, s_value[k]);
-                    if (owner) s_sum[mine] = sum;
-                }
-                __syncthreads();
-                for (uint32_t w = tid; w < kSpan / 32; w += kLogitsThreads) s_listed[w] |= s_once[w];
+                        for (uint32_t e = 0; e < 4; ++e)
+                            if (cols[e] == mine) { if (o + e < k) owner = false; sum = __fadd_rn(sum, s_value[o + e]); }
+                    }
+                } else sum = __fadd_rn(sum, s_value[k]);
+                if (owner) s_sum[mine] = sum;
             }
             __syncthreads();
+            if (!one) {
+                for (uint32_t w = tid; w < kSpan / 32; w += kLogitsThreads) s_listed[w] |= s_once[w];
+                __syncthreads();
+            }
         }
-        listed = (s_listed[tid >> 1] >> (16u * (tid & 1u))) & 0xFFFFu;
+        listed = ((one ? s_once : s_listed)[tid >> 1] >> (16u * (tid & 1u))) & 0xFFFFu;
     }
     // one reciprocal a row instead of a division a token: off by 2^-24 of the value, in front of a rounding of 2^-9
     const float grow = c.rep_penalty != 0.f ? c.rep_penalty : 1.f, shrink = __frcp_rn(grow);
@@ -360,13 +357,13 @@ mc_status_t mc_sm100_logits_process(const mc_sm100_logits_process_t* call, const
     const uint32_t n_rows = call->n_rows, vocab = call->vocab, row_stride = call->row_stride, out_stride = call->out_stride;
     const int32_t index_base = call->index_base;
     if (call->d_logits == nullptr || call->d_out == nullptr || call->d_cfg == nullptr || tables == nullptr || n_rows == 0 || n_rows > 65535u ||
-        vocab == 0 || vocab > 0x40000000u || row_stride < vocab || out_stride < vocab || index_base < 0 ||
+        vocab == 0 || row_stride < vocab || out_stride < vocab || index_base < 0 ||
         (call->d_logits == call->d_out && row_stride != out_stride) || ((reinterpret_cast<uintptr_t>(call->d_logits) | reinterpret_cast<uintptr_t>(call->d_out)) & 1u) != 0u) {
         set_error("%s: invalid args (rows=%u vocab=%u strides=%u,%u index_base=%d)", who, n_rows, vocab, row_stride, out_stride, index_base);
         return MC_E_INVALID_ARGUMENT;
     }
     const mc_sm100_logits_tables_t& t = *tables;
-    if (t.struct_size != sizeof(mc_sm100_logits_tables_t) || t.reserved != 0u || t.table_vocab > 0x7FFFFFFFu ||
+    if (t.struct_size != sizeof(mc_sm100_logits_tables_t) || t.reserved != 0u || t.table_vocab > 0x10000000u ||
         (uint64_t)index_base + vocab > t.table_vocab || (t.n_slots != 0u && (t.d_counts == nullptr || t.d_seen == nullptr)) ||
         (t.n_masks != 0u && t.d_mask == nullptr) || (t.n_bias != 0u && (t.d_bias_token == nullptr || t.d_bias_value == nullptr))) {
         set_error("%s: invalid tables (struct_size=%u table_vocab=%u slots=%u masks=%u biases=%u) for columns %d..%llu", who, t.struct_size,
@@ -388,7 +385,7 @@ mc_status_t mc_sm100_token_history(const mc_sm100_token_history_t* call, void* s
     }
     const mc_sm100_token_history_t& d = *call;
     const uint32_t n_seqs = d.n_seqs, table_vocab = d.table_vocab;
-    if (d.d_counts == nullptr || d.d_seen == nullptr || d.n_slots == 0 || d.n_slots > 0x7FFFFFFFu || table_vocab == 0 || table_vocab > 0x40000000u ||
+    if (d.d_counts == nullptr || d.d_seen == nullptr || d.n_slots == 0 || d.n_slots > 0x7FFFFFFFu || table_vocab == 0 || table_vocab > 0x10000000u ||
         (d.d_tokens == nullptr && d.n_tokens != 0u) || n_seqs == 0 || n_seqs > 0x7FFFFFFFu || (d.d_offsets == nullptr && d.n_tokens < n_seqs) ||
         (d.d_slots == nullptr && n_seqs > d.n_slots)) {
         set_error("mc_sm100_token_history: invalid args (slots=%u vocab=%u tokens=%u sequences=%u)", d.n_slots, table_vocab, d.n_tokens, n_seqs);

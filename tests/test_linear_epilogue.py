@@ -28,6 +28,10 @@ def test_refusals(pkg):
         with pytest.raises(pkg.McError) as e:
             call(w, None, x, y, M, N, K, **ok)
         assert e.value.status == pkg.MC_E_INVALID_ARGUMENT and "invalid args" in e.value.message
+    for M, N, K in ((2 ** 30 + 1, 8, 8), (1, 2 ** 30 + 1, 8), (1, 8, 2 ** 30 + 8)):
+        with pytest.raises(pkg.McError) as e:
+            call(16, None, 16, 16, M, N, K, **ok)
+        assert e.value.status == pkg.MC_E_INVALID_ARGUMENT
     for kw in (dict(gated=True, N=7), dict(x_stride=7), dict(y_stride=7), dict(residual=32, residual_stride=7), dict(bias=33), dict(residual=33)):
         kw = dict(kw)
         N = kw.pop("N", 8)
@@ -300,3 +304,54 @@ def test_streams_and_graph(pkg):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(y[0], ref[0]) and torch.equal(y[1], ref[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [3, 70])
+def test_rows_more_than_2_32_elements_apart(pkg, M):
+    """Strides whose last row starts beyond 32-bit element numbers; what lies between the rows stays as it was."""
+    import torch
+    N, K = 72, 96
+    far = (2 ** 32 // (M - 1) // 8 + 3) * 8
+    g = torch.Generator(device="cuda")
+    g.manual_seed(M)
+    w, x, r = ((torch.randn(*s, generator=g, device="cuda") * 0.5).bfloat16() for s in ((N, K), (M, K), (M, N)))
+    buf = torch.zeros((M - 1) * far + max(N, K), dtype=torch.bfloat16, device="cuda")
+    rows = torch.as_strided(buf, (M, max(N, K)), (far, 1))
+    rows[:, :K] = x
+    near, y = torch.empty(M, N, dtype=torch.bfloat16, device="cuda"), torch.empty(M, N, dtype=torch.bfloat16, device="cuda")
+    pkg.launch_linear_epilogue(w, None, x, near, M, N, K, residual=r, activation="silu")
+    pkg.launch_linear_epilogue(w, None, buf, y, M, N, K, residual=r, activation="silu", x_stride=far)
+    assert torch.equal(near, y)
+    rows[:, :N] = r
+    pkg.launch_linear_epilogue(w, None, x, buf, M, N, K, residual=buf, activation="silu", y_stride=far, residual_stride=far)
+    assert torch.equal(near, rows[:, :N])
+    rows[:, :] = 0
+    assert int(torch.count_nonzero(buf)) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 20, 200])
+def test_waits_for_the_kernel_before(pkg, M):
+    """Weights, activation, bias and residual written by the kernel just before, without pdl: plain stream order."""
+    import torch
+    N, K = 1200, 1600
+    g = torch.Generator(device="cuda")
+    g.manual_seed(M)
+    src = [(torch.randn(*s, generator=g, device="cuda") * 0.1).bfloat16() for s in ((N, K), (M, K), (N,), (M, N))]
+    want = torch.empty(M, N, dtype=torch.bfloat16, device="cuda")
+    pkg.launch_linear_epilogue(src[0], None, src[1], want, M, N, K, bias=src[2], residual=src[3])
+    dst = [torch.zeros_like(t) for t in src]
+    y = torch.empty_like(want)
+    big = torch.zeros(1 << 26, device="cuda")
+    for _ in range(5):
+        for t in dst:
+            t.zero_()
+        y.zero_()
+        torch.cuda.synchronize()
+        big.add_(1.0)                                              # the copies queue up behind it
+        for d, t in zip(dst, src):
+            d.copy_(t)
+        pkg.launch_linear_epilogue(dst[0], None, dst[1], y, M, N, K, bias=dst[2], residual=dst[3])
+        pkg.launch_linear_epilogue(dst[0], None, dst[1], y, M, N, K, bias=dst[2], residual=dst[3])
+        assert torch.equal(y, want)

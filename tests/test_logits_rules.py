@@ -311,6 +311,30 @@ def test_history_reports_what_it_passes_over(pkg):
             status.zero_()
 
 
+@pytest.mark.gpu
+def test_tables_beyond_32_bits(pkg):
+    """Counts of slots whose entries lie beyond 2^32: rebuilt, added to, and read by the penalties."""
+    import gpu_util as g
+    import torch
+    vocab, slots = 122753, 35100
+    assert (slots - 1) * vocab > 2 ** 32
+    words = (vocab + 31) // 32
+    counts, seen = torch.zeros(slots * vocab, dtype=torch.int32, device="cuda"), torch.zeros(slots * words, dtype=torch.int32, device="cuda")
+    d_slots = g.dev(np.int32([slots - 1, 2]))
+    tok = np.int32([5, 7, 7, vocab - 1, 0, 0])
+    pkg.token_history(counts, seen, g.dev(tok), 2, vocab, offsets=g.dev(np.uint32([0, 4, 6])), prompt_len=g.dev(np.uint32([1, 1])), slots=d_slots, rebuild=True)
+    pkg.token_history(counts, seen, g.dev(np.int32([9, 9])), 2, vocab, slots=d_slots)
+    last, third = counts[-vocab:].cpu().numpy(), counts[2 * vocab:3 * vocab].cpu().numpy()
+    assert last.nonzero()[0].tolist() == [7, 9, vocab - 1] and last[[7, 9, vocab - 1]].tolist() == [2, 1, 1]
+    assert third.nonzero()[0].tolist() == [0, 9] and int(torch.count_nonzero(counts)) == 5
+    known = np.unpackbits(seen[-words:].cpu().numpy().view(np.uint8), bitorder="little")[:vocab].astype(bool)
+    assert known.nonzero()[0].tolist() == [5, 7, 9, vocab - 1]
+    logits = onp.f32_to_bf16(np.random.default_rng(1).standard_normal((1, vocab)).astype(np.float32) * 3)
+    out = g.empty_u16(1, vocab)
+    pkg.logits_process(g.dev(logits), out, 1, vocab, vocab, vocab, g.dev(_config([(1.5, 0.5, 0.25, slots - 1, -1, 0, 0)])), pkg.logits_tables(vocab, counts=counts, seen=seen))
+    _same(g.host_u16(out), onp.logits_process_f32(logits[0], (1.5, 0.5, 0.25), last, known, None, [], [])[None])
+
+
 # ---- GPU: together ---------------------------------------------------------------------------------------------------
 @pytest.mark.gpu
 def test_prompt_then_steps_eager_and_replayed(pkg):
