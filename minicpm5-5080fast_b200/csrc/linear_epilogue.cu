@@ -2,6 +2,7 @@
 #include "linear_epilogue.cuh"
 
 #include "fast_dispatch.cuh"
+#include "linear_rows.cuh"
 #include "linear_tile.cuh"
 #include "skinny_gemm.cuh"
 
@@ -156,6 +157,8 @@ extern "C" mc_status_t mc_sm100_linear_epilogue(const mc_sm100_linear_epilogue_t
     // 122753 x 2304: 95 against 115 us; M = 64, 11520 x 2304: 15.1 against 19.3), slower elsewhere (M = 64, 2304 x 5760: 16.7
     // against 14.2; M = 48, 20000 x 4096: 43.9 against 41.8).
     const bool tiled = M > 64u || tile_forced() || (M > 32u && (K <= 768u || (N >= 4096u && K <= 3000u)));
+    if (wb == 1 && M <= 16u && tma && !tile_forced() && linear_rows_ok(M, K, xs))
+        return linear_rows(static_cast<const uint8_t*>(d_w), d_x, xs, M, N, K, e, st, true);
     if (!tiled && tma) return skinny_gemm_fused(wb == 2 ? SKINNY_W_BF16 : SKINNY_W_E4M3, d_w, d_x, xs, M, N, K, e, st, true);
     if (tma) return linear_tile(wb, d_w, d_x, xs, M, N, K, e, st, true);
     return linear_any(wb, d_w, d_x, xs, M, N, K, e, st, true);

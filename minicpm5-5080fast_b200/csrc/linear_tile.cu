@@ -138,12 +138,6 @@ __device__ __forceinline__ void tile_commit(uint32_t bar, uint16_t pair_mask) {
                      ::"r"(bar), "h"(pair_mask) : "memory");
 }
 
-__device__ __forceinline__ bool elect_lane() {
-    uint32_t p;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
-    return p != 0u;
-}
-
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
     uint32_t r[32];
     asm volatile(

@@ -35,6 +35,7 @@ constexpr int kTileN = 128;        // weight rows per CTA (MMA M)
 constexpr int kThreads = 320;      // 10 warps
 constexpr int kConvThreads = 256;  // warps 2..9
 constexpr uint32_t kConvGroup = 128;  // converter threads that share one K block (two groups)
+constexpr uint32_t kNapNs = 1000000u;   // a poll may sleep this long; spinning warps take issue slots from working ones
 constexpr unsigned long long kWaitLimitNs = 200ull * 1000ull * 1000ull;   // a wait gives up after 200 ms
 
 __device__ int g_skinny_error;     // set when a bounded wait ran out (read back by tests)
@@ -47,14 +48,14 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
         uint32_t done;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(done)
-            : "r"(bar), "r"(parity)
+            : "r"(bar), "r"(parity), "r"(kNapNs)
             : "memory");
         if (done) return true;
         if (*abort_flag) return false;
-        if ((spin & 63u) == 63u) {            // look at the clock now and then; bound the wait in TIME
+        if ((spin & 15u) == 15u) {            // look at the clock now and then; bound the wait in TIME
             unsigned long long now;
             asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
             if (t0 == 0) t0 = now;
@@ -228,25 +229,27 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            // ------------------------------------------------------------ MMA issuer
-            bool ok = true;
-            for (uint32_t it = 0; it < nloc && ok; ++it) {
-                const uint32_t s = it % OPS;
-                const uint32_t par = (it / OPS) & 1u;
-                ok = mbar_wait(op_full(s), par, abortp, a.status);
-                if (ok && E4) ok = mbar_wait(conv_done(s), par, abortp, a.status);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t da = make_desc(sA + s * G::A_OP), db = make_desc(sB + s * G::B_OP);
+        // ---------------------------------------------------------------- MMA issuer: the warp together, one lane elected to issue
+        bool ok = true;
+        uint32_t s = 0, par = 0;
+        for (uint32_t it = 0; it < nloc && ok; ++it) {
+            ok = mbar_wait(op_full(s), par, abortp, a.status);
+            if (ok && E4) ok = mbar_wait(conv_done(s), par, abortp, a.status);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint64_t da = make_desc(sA + s * G::A_OP), db = make_desc(sB + s * G::B_OP);
+            if (elect_lane()) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)   // 4 x (K = 32 bytes) per 128-byte row
                     mma_issue<MODE == SKINNY_W8A8>(tmem_base, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), IDESC,
                                                    (it > 0 || k > 0) ? 1u : 0u);
                 mma_commit(op_empty(s));      // frees the stage once the MMAs have read it
             }
-            if (ok && nloc > 0) mma_commit(accum_bar);
+            __syncwarp();
+            if (++s == OPS) { s = 0; par ^= 1u; }
         }
+        if (ok && nloc > 0 && elect_lane()) mma_commit(accum_bar);
+        __syncwarp();
     } else if constexpr (E4) {
         // ---------------------------------------------------------------- e4m3 -> bf16 widening
         // thread -> (row, 16-byte raw chunk): a quarter warp covers two whole raw rows, 128 consecutive bytes; its swizzled

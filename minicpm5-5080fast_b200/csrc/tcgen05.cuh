@@ -47,6 +47,14 @@ __device__ __forceinline__ uint64_t make_desc(uint32_t saddr) {
 // swizzled byte offset of 16-byte chunk `cc` (0..7) of tile row `row`
 __device__ __forceinline__ uint32_t swz(uint32_t row, uint32_t cc) { return row * kRowBytes + ((cc ^ (row & 7u)) << 4); }
 
+// One lane of a converged warp.  A loop that the whole warp runs, with the issue elected, keeps addresses in uniform registers;
+// run by lane 0 alone it took 0.28 us a K block where this takes 0.22.
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0u;
+}
+
 // Four e4m3 codes -> four bf16 of value * 2^-120 (the 7 magnitude bits dropped at bit 4), byte-wise: 7 integer operations
 // where placing pair by pair takes 8; then * 2^120, exact.
 __device__ __forceinline__ void widen4(uint32_t w, uint32_t& p01, uint32_t& p23) {
