@@ -183,6 +183,7 @@ struct ChunkIO {
     uint32_t buf, lane, own, own_swz, across, col;      // shared addresses of this lane's row / first piece; its first column
     uint32_t m_base;
     int32_t rows_left;                                  // rows from this lane's first piece's to the end of y
+    uint32_t res_first = 0;                             // first residual of this lane's row, where it crosses alone
     uint16_t* y;
     const uint16_t* res;
 
@@ -197,10 +198,13 @@ struct ChunkIO {
         res = a.ep.res != nullptr ? a.ep.res + (size_t)(m_base + row) * a.ep.res_stride + col : nullptr;
     }
     __device__ __forceinline__ uint32_t own_piece(uint32_t k) const { return own + ((k ^ own_swz) << 4); }
-    __device__ __forceinline__ uint32_t element(uint32_t row, uint32_t c) const { return buf + row * ROW_BYTES + (((c >> 3) ^ swizzle(row)) << 4) + (c & 7u) * 2u; }
 
-    // Aligned rows, ahead of use and without registers; beyond the edges zeros, which are not stored.
-    __device__ __forceinline__ void fetch_res(uint32_t j0) const {
+    __device__ __forceinline__ uint32_t odd_res(uint32_t row) const {   // a row of the residual starts in the upper half of a word
+        return ((uint32_t)(reinterpret_cast<uintptr_t>(a.ep.res) >> 1) + row * a.ep.res_stride) & 1u;
+    }
+    // Ahead of use and without registers; beyond the edges zeros, which are not stored.
+    __device__ __forceinline__ void fetch_res(uint32_t j0) {
+        if (!a.res_vec) { fetch_words(j0); return; }
         const uint32_t bytes = j0 + col + 8u <= a.n_out ? 16u : (j0 + col < a.n_out ? 2u * (a.n_out - j0 - col) : 0u);
 #pragma unroll
         for (uint32_t i = 0; i < PIECES; ++i) {
@@ -210,26 +214,30 @@ struct ChunkIO {
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    // Rows at any address: a lane holds one column of every row (gated: of every second row); eight rows in flight.
-    __device__ __forceinline__ void res_elements(uint32_t j0) const {
-        const uint32_t c = lane & (OUTS - 1u), r0 = lane / OUTS;
+    // Rows of the residual anywhere: the halves [odd, odd + OUTS) of each, two a word, and the first one of an odd row alone; a
+    // half-warp (gated: a quarter) takes a row.  odd is the same for all rows of a lane: their distance is even.  M 2595, N 19101,
+    // K 696: 104 us; with element loads through registers, eight in flight, 117.
+    __device__ __forceinline__ void fetch_words(uint32_t j0) {
+        constexpr uint32_t LW = LG + 2u, WORDS = 1u << LW, WROWS = 32u >> LW;
+        const uint32_t r0 = lane >> LW, w = lane & (WORDS - 1u), e = j0 + 2u * w + odd_res(r0);
+        const uint32_t bytes = e + 2u <= a.n_out ? 4u : (e < a.n_out ? 2u : 0u);
         const int32_t left = (int32_t)a.M - (int32_t)(m_base + r0);
-        const bool in = j0 + c < a.n_out;
-        const uint16_t* src = a.ep.res + (size_t)(m_base + r0) * a.ep.res_stride + j0 + c;
-        const size_t step = (size_t)(32u / OUTS) * a.ep.res_stride;
+        const uint16_t* from = a.ep.res + (size_t)(m_base + r0) * a.ep.res_stride + e;
+        const uint16_t* none = reinterpret_cast<const uint16_t*>(reinterpret_cast<uintptr_t>(a.ep.res + 1) & ~(uintptr_t)3);     // aligned, not read
+        const uint32_t to = buf + kResBuf + r0 * ROW_BYTES + (w & 3u) * 4u;
 #pragma unroll
-        for (uint32_t r = 0; r < OUTS; r += 8u) {
-            uint16_t v[8];
-#pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) {
-                v[e] = in && (int32_t)((r + e) * (32u / OUTS)) < left ? *src : (uint16_t)0x8000u;
-                src += step;
-            }
-#pragma unroll
-            for (uint32_t e = 0; e < 8; ++e)
-                asm volatile("st.shared.u16 [%0], %1;" ::"r"(kResBuf + element(r0 + (r + e) * (32u / OUTS), c)), "h"(v[e]) : "memory");
+        for (uint32_t i = 0; i < WORDS; ++i) {
+            const bool in = (int32_t)(i * WROWS) < left && bytes != 0u;
+            const uint16_t* src = in ? from + (size_t)(i * WROWS) * a.ep.res_stride : none;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + i * 128u + (((w >> 2) ^ (i & (PIECES - 1u))) << 4)), "l"(src), "r"(in ? bytes : 0u) : "memory");
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        res_first = 0u;
+        if (m_base + lane < a.M && odd_res(lane)) res_first = a.ep.res[(size_t)(m_base + lane) * a.ep.res_stride + j0];
     }
+    // Rows of y anywhere: a lane holds one column of every row (gated: of every second row), so that one instruction writes all
+    // of a row's chunk.  Two rows an instruction in 4-byte words are slower, though they are half as many (M 2595, K 64: 66 us at
+    // N 19102, with the ends of odd rows apart 75 at N 19101; so 56 at either).
     __device__ __forceinline__ void store_elements(uint32_t j0) const {
         const uint32_t c = lane & (OUTS - 1u), r0 = lane / OUTS;
         const int32_t left = (int32_t)a.M - (int32_t)(m_base + r0);
@@ -240,8 +248,10 @@ struct ChunkIO {
         for (uint32_t r = 0; r < OUTS; r += 8u) {
             uint16_t v[8];
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e)
-                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v[e]) : "r"(element(r0 + (r + e) * (32u / OUTS), c)) : "memory");
+            for (uint32_t e = 0; e < 8; ++e) {
+                const uint32_t row = r0 + (r + e) * (32u / OUTS);
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v[e]) : "r"(buf + row * ROW_BYTES + (((c >> 3) ^ swizzle(row)) << 4) + (c & 7u) * 2u) : "memory");
+            }
 #pragma unroll
             for (uint32_t e = 0; e < 8; ++e) {
                 if (in && (int32_t)((r + e) * (32u / OUTS)) < left) *dst = v[e];
@@ -273,10 +283,9 @@ struct ChunkIO {
     }
     // v: the 32 finished accumulators of this lane's row, columns n .. n + 31 (tile column c); col_s: staged scales, biases
     template <uint32_t BN>
-    __device__ __forceinline__ void finish(float (&v)[32], uint32_t n, uint32_t c, uint32_t col_s, bool has_scale, bool has_bias, uint32_t next_n) const {
+    __device__ __forceinline__ void finish(float (&v)[32], uint32_t n, uint32_t c, uint32_t col_s, bool has_scale, bool has_bias, uint32_t next_n) {
         const uint32_t j0 = GATED ? n >> 1 : n;
         const bool has_res = a.ep.res != nullptr;
-        if (has_res && !a.res_vec) res_elements(j0);
         if (has_scale) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
@@ -310,14 +319,20 @@ struct ChunkIO {
         else if (act == MC_SM100_ACT_RELU) apply([](float z) { return epi_act(z, MC_SM100_ACT_RELU); });
         else if (GATED) apply([](float z) { return z; });
         if (has_res) {
-            if (a.res_vec) asm volatile("cp.async.wait_group 0;" ::: "memory");
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncwarp();
+            uint32_t before = res_first << 16;
+            const uint32_t shift = a.res_vec ? 0u : 16u * odd_res(lane);
 #pragma unroll
             for (uint32_t k = 0; k < PIECES; ++k) {
                 const uint4 m = lds16(own_piece(k) + kResBuf);
                 const uint32_t r[4] = {m.x, m.y, m.z, m.w};
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) { v[8 * k + 2 * e] += bf16lo(r[e]); v[8 * k + 2 * e + 1] += bf16hi(r[e]); }
+                for (uint32_t e = 0; e < 4; ++e) {
+                    const uint32_t h = __funnelshift_l(before, r[e], shift);
+                    v[8 * k + 2 * e] += bf16lo(h); v[8 * k + 2 * e + 1] += bf16hi(h);
+                    before = r[e];
+                }
             }
         }
 #pragma unroll
@@ -325,7 +340,7 @@ struct ChunkIO {
             sts16(own_piece(k), make_uint4(pack_bf16(v[8 * k], v[8 * k + 1]), pack_bf16(v[8 * k + 2], v[8 * k + 3]),
                                            pack_bf16(v[8 * k + 4], v[8 * k + 5]), pack_bf16(v[8 * k + 6], v[8 * k + 7])));
         __syncwarp();                                                  // pieces written, residual read
-        if (has_res && a.res_vec && next_n != 0xFFFFFFFFu) fetch_res(GATED ? next_n >> 1 : next_n);
+        if (has_res && next_n != 0xFFFFFFFFu) fetch_res(GATED ? next_n >> 1 : next_n);
         store(j0);
         __syncwarp();
     }
@@ -444,7 +459,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 uint32_t mt, nt;
                 tile_of(a, t, mt, nt);
                 const uint32_t b = i % bufs, n0 = nt * BN;
-                const IO io(a, sBuf + warp * kWarpBuf, lane, (mt * CG + sub) * 128u + q * 32u);
+                IO io(a, sBuf + warp * kWarpBuf, lane, (mt * CG + sub) * 128u + q * 32u);
                 if (has_scale || has_bias) {
                     asm volatile("bar.sync 1, %0;" ::"n"(EPI * 32u) : "memory");     // the previous tile's have been read
                     if (tid < BN) {
@@ -457,7 +472,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 // this CTA finishes columns [c_lo, c_hi), this warp every GROUPS-th chunk of them
                 const uint32_t per = BN / S, c_lo = split * per, c_hi = n0 + c_lo + per <= a.N ? c_lo + per : (a.N - n0 > c_lo ? a.N - n0 : c_lo);
                 const uint32_t c_first = c_lo + group * 32u;
-                if (a.ep.res != nullptr && a.res_vec && c_first < c_hi) io.fetch_res((n0 + c_first) >> a.ep.gated);
+                if (a.ep.res != nullptr && c_first < c_hi) io.fetch_res((n0 + c_first) >> a.ep.gated);
                 if (ok) ok = tile_wait(acc_full(b), (i / bufs) & 1u, abortp, a.status);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t taddr = tmem + b * G::COLS + ((q * 32u) << 16);

@@ -180,6 +180,32 @@ def test_strides_in_place_and_alignment(pkg, M):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("y_at,r_at", [(1, 1), (1, 0), (0, 1), (3, 2)])
+def test_output_and_residual_at_any_address(pkg, y_at, r_at, gated):
+    """y and the residual begin anywhere in an allocation, rows even and odd numbers of elements apart: what stands around y stays."""
+    import gpu_util as g
+    import torch
+    for M, N, y_pad, r_pad in ((70, 74, 0, 0), (1, 66, 0, 0), (33, 130, 1, 0), (200, 262, 0, 1), (131, 140, 3, 2)):
+        w, _, _, x, b, r = _make(M, N, 80, False, True, True, gated, M + y_at)
+        n_out = N // 2 if gated else N
+        ly, lr = n_out + y_pad, n_out + r_pad
+        y = torch.full((y_at + M * ly + 8,), 0x7FC0, dtype=torch.int16, device="cuda")
+        res = torch.zeros(r_at + M * lr, dtype=torch.int16, device="cuda")
+        res[r_at:] = g.dev(_wide(r, r_pad)).reshape(-1)
+        pkg.launch_linear_epilogue(g.dev(w), None, g.dev(x), y[y_at:], M, N, 80, bias=g.dev(b), residual=res[r_at:], activation="gelu_tanh", gated=gated,
+                                   y_stride=ly, residual_stride=lr)
+        g.sync()
+        flat = g.host_u16(y).reshape(-1)
+        got = flat[y_at:y_at + M * ly].reshape(M, ly)
+        assert np.all(flat[:y_at] == 0x7FC0) and np.all(flat[y_at + M * ly:] == 0x7FC0) and np.all(got[:, n_out:] == 0x7FC0)
+        f = onp.bf16_to_f32
+        want, bound = onp.linear_epilogue_f64(f(w), f(x), None, f(b), f(r), "gelu_tanh", gated)
+        d = np.abs(f(got[:, :n_out]).astype(np.float64) - want)
+        assert np.all(d <= bound), (M, N, float(np.max(d / bound)))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M", [1, 9, 64, 200])
 def test_a_row_that_is_not_finite_stays_alone(pkg, M):
     import gpu_util as g
