@@ -363,8 +363,16 @@ def launch_linear_epilogue(w, scale, x, y, M, N, K, bias=None, residual=None, ac
 
 def logits_tables(table_vocab, counts=None, seen=None, masks=None, bias_token=None, bias_value=None, status=None) -> bytes:
     """Tables of logits_process out of device tensors (their sizes give the numbers of rows); the caller keeps the tensors."""
-    return _pack_tables(72, table_vocab, 0 if counts is None else counts.numel() // table_vocab,
-                        0 if masks is None else masks.numel() // ((table_vocab + 31) // 32), 0 if bias_token is None else bias_token.numel(), 0,
+    words = (table_vocab + 31) // 32
+    slots = 0 if counts is None else counts.numel() // table_vocab                          # one without the other is refused
+    if seen is not None:
+        n = seen.numel() // words
+        slots = n if counts is None or n < slots else slots
+    biases = 0 if bias_token is None else bias_token.numel()
+    if bias_value is not None:
+        n = bias_value.numel()
+        biases = n if bias_token is None or n < biases else biases
+    return _pack_tables(72, table_vocab, slots, 0 if masks is None else masks.numel() // words, biases, 0,
                         0 if counts is None else counts.data_ptr(), 0 if seen is None else seen.data_ptr(), 0 if masks is None else masks.data_ptr(),
                         0 if bias_token is None else bias_token.data_ptr(), 0 if bias_value is None else bias_value.data_ptr(),
                         0 if status is None else status.data_ptr())

@@ -152,14 +152,17 @@ extern "C" mc_status_t mc_sm100_linear_epilogue(const mc_sm100_linear_epilogue_t
         return launch_fast_fused(wb, d.gated != 0u, a, st, true);
     }
     const bool tma = unit && (xs & 7u) == 0u;
-    // Up to 64 rows the skinny kernel, which splits K eight ways and pads M to 16, 32 or 64.  From 33 rows on the tiled kernel
-    // is faster where K is short (M = 62, 480 x 448: 5.7 against 9.1 us) or the weights have many rows (M = 33, lm_head
-    // 122753 x 2304: 95 against 115 us; M = 64, 11520 x 2304: 15.1 against 19.3), slower elsewhere (M = 64, 2304 x 5760: 16.7
-    // against 14.2; M = 48, 20000 x 4096: 43.9 against 41.8).
-    const bool tiled = M > 64u || tile_forced() || (M > 32u && (K <= 768u || (N >= 4096u && K <= 3000u)));
+    // Up to 64 rows the skinny kernel, which splits K eight ways and pads M to 16, 32 or 64.  From 17 rows on the tiled kernel
+    // is faster where K is short for the padded M (M = 32, 4096 x 448: 5.0 against 6.4 us; M = 64, 2304 x 1024: 6.8 against 9.1)
+    // or the weights have many rows (M = 33, lm_head 122753 x 2304: 95 against 115; M = 64, 11520 x 3008: 17.4 against 22.1);
+    // elsewhere it is slower (M = 32, 2304 x 1024 level; M = 64, 2304 x 5760: 16.7 against 12.9; M = 33, 20000 x 5760: 59 against
+    // 51).  Over 560 shapes the rule is within 0.5 % of the better one on average, 18 % in the worst case (M = 33, 480 x 1024).
+    const bool short_k = M > 16u && K <= (M <= 32u ? 512u : 1024u), tall = M > 24u && N >= 5000u && K <= 72u * M;
+    const bool tiled = M > 64u || tile_forced() || short_k || tall;
     if (wb == 1 && M <= 16u && tma && !tile_forced() && linear_rows_ok(M, K, xs))
         return linear_rows(static_cast<const uint8_t*>(d_w), d_x, xs, M, N, K, e, st, true);
     if (!tiled && tma) return skinny_gemm_fused(wb == 2 ? SKINNY_W_BF16 : SKINNY_W_E4M3, d_w, d_x, xs, M, N, K, e, st, true);
+    (void)take_next_weights();                       // a hint left for this call is consumed
     if (tma) return linear_tile(wb, d_w, d_x, xs, M, N, K, e, st, true);
     return linear_any(wb, d_w, d_x, xs, M, N, K, e, st, true);
 }

@@ -21,7 +21,7 @@ namespace mcl {
 
 namespace {
 
-constexpr uint32_t kBK = 64;                                   // K elements per stage
+constexpr uint32_t kBK = 64;                                   // K elements of a block: rows of 128 bytes
 constexpr uint32_t kRing = 196608;                             // bytes of the rings
 constexpr uint32_t kResBuf = 2048;                             // an epilogue warp's residual chunk stands behind its output chunk
 constexpr uint32_t kWarpBuf = 4096;
@@ -30,8 +30,14 @@ constexpr unsigned long long kTileWaitNs = 200ull * 1000ull * 1000ull;
 
 __device__ int g_tile_error;
 
+// K blocks of a stage.  A turn of the producer or of the MMA warp (wait, four copies or eight MMAs, arrival) takes 350 - 390
+// cycles whatever the tile's width: at one block a stage that is 0.20 us a block, where the MMAs of 128 features take 0.13.
+// 256 features keep the tensor pipe busy for longer than a turn, and e4m3's widening does.
+constexpr uint32_t stage_blocks(int wb, int bn) { return wb == 2 && bn < 256 ? 2u : 1u; }
+
 template <int WB, int CG, int BN> struct TileGeom {
-    static constexpr uint32_t A = 128u * kRowBytes, BROWS = BN / CG, B = BROWS * kRowBytes, RAW = WB == 1 ? BROWS * kBK : 0u;
+    static constexpr uint32_t KPS = stage_blocks(WB, BN), BROWS = BN / CG;
+    static constexpr uint32_t A1 = 128u * kRowBytes, B1 = BROWS * kRowBytes, A = KPS * A1, B = KPS * B1, RAW = WB == 1 ? BROWS * kBK : 0u;
     static constexpr uint32_t RAWS = WB == 1 ? (kRing / 4u / RAW < 8u ? kRing / 4u / RAW : 8u) : 0u;
     // Even: a raw stage is then always the same group's.  With an odd count the groups take turns on a stage, and the one that
     // is ahead can find the parity of the use before the last where it waits for the last: it would pass too early.
@@ -353,7 +359,7 @@ template <int WB, int CG, int BN>
 __global__ void __launch_bounds__(TileGeom<WB, CG, BN>::THREADS, 1)
 linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const TileArgs a) {
     using G = TileGeom<WB, CG, BN>;
-    constexpr uint32_t STAGES = G::STAGES, RAWS = G::RAWS, EPI = G::EPI;
+    constexpr uint32_t STAGES = G::STAGES, RAWS = G::RAWS, EPI = G::EPI, KPS = G::KPS;
     constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((128 * CG) >> 4) << 24);
     constexpr uint32_t CONV_WARPS = 4;                           // warps that widen one K block
 
@@ -383,11 +389,11 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 
     pdl_trigger();
     // One CTA per tile: its first stages are asked for before the tensor memory and the other roles are ready (weights before
-    // the previous kernel's end is waited for): -0.5 us a call.  A pair has to know its partner's barriers first, and where K
-    // is split the loop that asks holds up the cluster's first barrier by as much as it gains.
+    // the previous kernel's end is waited for): -0.5 us a call.  A pair has to know its partner's barriers first.
     const uint32_t nloc = cid < a.tiles ? kb1 - kb0 : 0u;
-    const uint32_t early = CG == 1 && S == 1u ? min(nloc, 4u) : 0u;
-    static_assert(STAGES >= 4u && (WB == 2 || RAWS >= 4u), "the early stages are all the ring's");
+    constexpr uint32_t EARLY = 4u / KPS;
+    const uint32_t early = CG == 1 ? min(nloc, EARLY) : 0u;
+    static_assert(STAGES >= EARLY && (WB == 2 || RAWS >= EARLY), "the early stages are all the ring's");
     if (tid == EPI * 32u) {
         abort_flag = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
@@ -405,12 +411,15 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             for (uint32_t it = 0; it < early; ++it) {
                 const uint32_t bar = WB == 1 ? raw_full(it) : full(it);
                 mbar_expect_tx(bar, WB == 1 ? G::RAW : G::A + G::B);
-                tma_load_2d(WB == 1 ? sRaw + it * G::RAW : sB + it * G::B, &map_w, bar, (int32_t)((kb0 + it) * kBK), n0);
+#pragma unroll
+                for (uint32_t h = 0; h < KPS; ++h)
+                    tma_load_2d(WB == 1 ? sRaw + it * G::RAW : sB + it * G::B + h * G::B1, &map_w, bar, (int32_t)(((kb0 + it) * KPS + h) * kBK), n0);
             }
             pdl_wait();
             for (uint32_t it = 0; it < early; ++it) {
                 if constexpr (WB == 1) mbar_expect_tx(full(it), G::A);
-                tma_load_2d(sA + it * G::A, &map_x, full(it), (int32_t)((kb0 + it) * kBK), m0);
+#pragma unroll
+                for (uint32_t h = 0; h < KPS; ++h) tma_load_2d(sA + it * G::A + h * G::A1, &map_x, full(it), (int32_t)(((kb0 + it) * KPS + h) * kBK), m0);
             }
         }
     }
@@ -425,7 +434,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (csize > 1u) cluster_sync();                              // barriers and TMEM of every CTA are there
+    if constexpr (CG == 2) cluster_sync();                       // barriers and TMEM of every CTA are there
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_slot;
     volatile int* abortp = &abort_flag;
@@ -469,31 +478,36 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     load_column(t + clusters);                                       // of the next tile, under this one's work
                     asm volatile("bar.sync 1, %0;" ::"n"(EPI * 32u) : "memory");
                 }
-                // this CTA finishes columns [c_lo, c_hi), this warp every GROUPS-th chunk of them
-                const uint32_t per = BN / S, c_lo = split * per, c_hi = n0 + c_lo + per <= a.N ? c_lo + per : (a.N - n0 > c_lo ? a.N - n0 : c_lo);
+                // This CTA finishes columns [c_lo, c_hi), this warp every GROUPS-th chunk of them.  More slices than chunks: a
+                // chunk's rows are dealt out too, in `parts` of rows.
+                const uint32_t per = max(BN / S, 32u), parts = per * S / BN, rows = 128u / parts, part_of_warp = q * parts / 4u;
+                const uint32_t c_lo = split / parts * per;
+                uint32_t c_hi = n0 + c_lo + per <= a.N ? c_lo + per : (a.N - n0 > c_lo ? a.N - n0 : c_lo);
+                if (part_of_warp != split % parts) c_hi = c_lo;
                 const uint32_t c_first = c_lo + group * 32u;
                 if (a.ep.res != nullptr && c_first < c_hi) io.fetch_res((n0 + c_first) >> a.ep.gated);
                 if (ok) ok = tile_wait(acc_full(b), (i / bufs) & 1u, abortp, a.status);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t taddr = tmem + b * G::COLS + ((q * 32u) << 16);
-                const uint32_t row = q * 32u + lane;
+                const uint32_t row = q * 32u + lane - part_of_warp * rows;          // in its part
                 auto release = [&]() {                                               // this warp has read its part of the accumulator
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) { if (CG == 2) arrive_remote(map_to_rank(acc_empty(b), lead)); else mbar_arrive(acc_empty(b)); }
                 };
                 if (S > 1u) {
-                    // the cluster's rings are idle: they become the exchange [source split][row][per] of fp32
+                    // the cluster's rings are idle: they become the exchange [source split][row of the part][per] of fp32
                     cluster_sync();
                     uint32_t turn = 0;
                     for (uint32_t o = 0; o < S; ++o) {
                         if (o == split) continue;
                         const uint32_t src = split < o ? split : split - 1u;
-                        const uint32_t dst = map_to_rank(base + (src * 128u + row) * per * 4u, o * CG + sub);
+                        if (part_of_warp != o % parts) continue;
+                        const uint32_t dst = map_to_rank(base + (src * rows + row) * per * 4u, o * CG + sub);
                         for (uint32_t c = 0; c < per; c += 32u, ++turn) {
                             if (turn % GROUPS != group) continue;
                             float v[32];
-                            tmem_ld32(taddr + o * per + c, v);
+                            tmem_ld32(taddr + o / parts * per + c, v);
 #pragma unroll
                             for (int k = 0; k < 8; ++k)
                                 asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};"
@@ -511,7 +525,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     if (S > 1u) {
                         // this CTA's own part first, then the others in split order
                         for (uint32_t src = 0; src + 1u < S; ++src) {
-                            const uint32_t at = base + (src * 128u + row) * per * 4u;
+                            const uint32_t at = base + (src * rows + row) * per * 4u;
 #pragma unroll
                             for (int k = 0; k < 8; ++k) {
                                 const float4 f = lds_f4(at + (((((c - c_lo) >> 2) + k) ^ (row & 7u)) << 4));
@@ -544,8 +558,12 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                             if (!ok) break;
                             if (leader) mbar_expect_tx(full(s), CG * (G::A + (WB == 2 ? G::B : 0u)));
                             const uint32_t bar = CG == 2 ? map_to_rank(full(s), lead) : full(s);
-                            tile_load<CG>(sA + s * G::A, &map_x, bar, (int32_t)(kb * kBK), m0);
-                            if constexpr (WB == 2) tile_load<CG>(sB + s * G::B, &map_w, bar, (int32_t)(kb * kBK), n0);
+#pragma unroll
+                            for (uint32_t h = 0; h < KPS; ++h) {                     // a block beyond K comes as zeros
+                                const int32_t k = (int32_t)((kb * KPS + h) * kBK);
+                                tile_load<CG>(sA + s * G::A + h * G::A1, &map_x, bar, k, m0);
+                                if constexpr (WB == 2) tile_load<CG>(sB + s * G::B + h * G::B1, &map_w, bar, k, n0);
+                            }
                         }
                     }
                     // the last arrivals of the MMAs on this CTA's stages: none is under way when the CTA leaves
@@ -570,8 +588,10 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                             const uint64_t da = make_desc(sA + s * G::A), db = make_desc(sB + s * G::B);
                             if (elect_lane()) {
 #pragma unroll
-                                for (int k = 0; k < 4; ++k)
-                                    tile_mma<CG>(acc, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), IDESC, (kb > kb0 || k > 0) ? 1u : 0u);
+                                for (uint32_t k = 0; k < 4u * KPS; ++k) {           // 32 bytes of K each; addresses in units of 16 bytes
+                                    const uint64_t ka = (k >> 2) * (G::A1 >> 4) + (k & 3u) * 2u, kw = (k >> 2) * (G::B1 >> 4) + (k & 3u) * 2u;
+                                    tile_mma<CG>(acc, da + ka, db + kw, IDESC, (kb > kb0 || k > 0) ? 1u : 0u);
+                                }
                                 tile_commit<CG>(empty(s), pair);
                             }
                             __syncwarp();
@@ -656,7 +676,9 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         const unsigned long long t0 = global_timer_ns();
         while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
     }
-    if (csize > 1u) cluster_sync();                              // nobody addresses a CTA that has left
+    // Nobody addresses a CTA that has left.  Without pairs the last that arrives from outside is in front of the exchange's second
+    // barrier, and nothing comes from outside before its first: two barriers of a split call instead of four.
+    if constexpr (CG == 2) cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (warp == EPI + 1u) {
         if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");
@@ -685,6 +707,7 @@ mc_status_t launch_tile(const void* w, const uint16_t* x, uint32_t x_pitch, uint
         set_error("mc_sm100_linear_epilogue: M=%u N=%u make too many tiles", a.M, a.N);
         return MC_E_UNSUPPORTED;
     }
+    a.nkb = (K + G::KPS * kBK - 1u) / (G::KPS * kBK);
     a.m_tiles = (uint32_t)mt; a.n_tiles = (uint32_t)nt; a.tiles = (uint32_t)(mt * nt);
     uint32_t clusters = a.tiles;
     if (a.splits == 1u) {
@@ -712,33 +735,33 @@ mc_status_t launch_tile(const void* w, const uint16_t* x, uint32_t x_pitch, uint
 
 }  // namespace
 
-// The plan with the least estimated time.  The terms were fitted to 2200 timings on B200 (90 shapes, M 66 .. 8192, N 65 ..
-// 23000, K 256 .. 8100, both weight types, every plan); over them the choice is on average 0.4 % and at most 17 % slower than
+// The plan with the least estimated time.  The terms were fitted to 2400 timings on B200 (100 shapes, M 66 .. 8192, N 65 ..
+// 23000, K 256 .. 8100, both weight types, every plan); over them the choice is on average 0.5 % and at most 19 % slower than
 // the best plan, where 2 CTAs x 256 features for every call would be 30 % slower on average.  In us:
-//   a K block     0.21 - 0.30, not in proportion to the tile's width (what one SM draws from L2 bounds the narrow ones, the
-//                 MMA the widest); e4m3 0.27 - 0.40 (widening)
-//   an epilogue   0.8 for 64 columns, e4m3 1.5 times that (fewer registers)
-//   a K slice     4.0 for barriers and a cluster's start, 1.3 per 32 columns sent away
+//   a K block     0.19 - 0.30, not in proportion to the tile's width (what one SM draws from L2 bounds the narrow ones, the
+//                 MMA the widest); e4m3 0.29 - 0.41 (widening)
+//   an epilogue   1.0 for 64 columns, e4m3 1.2 times that (fewer registers)
+//   a K slice     2.4 for barriers and a cluster's start, 3.4 with pairs, 1.2 per 32 columns sent away
 TilePlan tile_plan(int wb, uint32_t M, uint32_t N, uint32_t K, uint32_t sms) {
     struct Form { uint32_t cg, bn, splits; double block[2]; };
-    static const Form forms[] = {{1, 64, 1, {0.22, 0.27}}, {1, 64, 2, {0.22, 0.27}}, {1, 128, 1, {0.24, 0.40}}, {1, 128, 2, {0.24, 0.40}},
-                                 {1, 128, 4, {0.24, 0.40}}, {2, 128, 1, {0.21, 0.31}}, {2, 128, 2, {0.21, 0.31}}, {2, 128, 4, {0.21, 0.31}},
-                                 {2, 256, 1, {0.30, 0.37}}, {2, 256, 2, {0.30, 0.37}}, {2, 256, 4, {0.30, 0.37}}};
-    const uint32_t blocks = (K + kBK - 1) / kBK;
+    static const Form forms[] = {{1, 64, 1, {0.19, 0.29}}, {1, 64, 2, {0.19, 0.29}}, {1, 64, 4, {0.19, 0.29}}, {1, 128, 1, {0.24, 0.41}},
+                                 {1, 128, 2, {0.24, 0.41}}, {1, 128, 4, {0.24, 0.41}}, {2, 128, 1, {0.245, 0.30}}, {2, 128, 2, {0.245, 0.30}},
+                                 {2, 128, 4, {0.245, 0.30}}, {2, 256, 1, {0.295, 0.36}}, {2, 256, 2, {0.295, 0.36}}, {2, 256, 4, {0.295, 0.36}}};
     TilePlan best{2, 256, 1};
     double least = 1e30;
     for (const Form& f : forms) {
-        if (f.splits > blocks) continue;
+        const uint32_t per = stage_blocks(wb, (int)f.bn), stages = (K + per * kBK - 1u) / (per * kBK);
+        if (f.splits > stages) continue;
         const double tiles = (double)((M + 128ull * f.cg - 1) / (128ull * f.cg)) * (double)((N + f.bn - 1ull) / f.bn);
         // clusters that run at once: all SMs as pairs, fewer of the larger ones (whole GPCs do not divide evenly)
         const uint32_t size = f.cg * f.splits;
         double room = size == 1u ? sms : size == 2u ? sms / 2u : size == 4u ? sms * 32u / 148u : sms * 14u / 148u;
         if (room < 1.0) room = 1.0;
         const double rounds = (double)(uint64_t)((tiles + room - 1.0) / room);
-        const double block = f.block[wb == 1 ? 1 : 0], epi = 0.8 * f.bn / 64.0 * (wb == 1 ? 1.5 : 1.0);
-        const double slice = (double)((blocks + f.splits - 1u) / f.splits);
+        const double block = f.block[wb == 1 ? 1 : 0], epi = 1.0 * f.bn / 64.0 * (wb == 1 ? 1.2 : 1.0);
+        const double slice = (double)((stages + f.splits - 1u) / f.splits * per);
         const double t = f.splits == 1u ? rounds * (slice * block + epi)
-                                        : rounds * (4.0 + slice * block + 1.3 * (f.splits - 1.0) / f.splits * f.bn / 32.0) + epi / f.splits;
+                                        : rounds * ((f.cg == 1u ? 2.4 : 3.4) + slice * block + 1.2 * (f.splits - 1.0) / f.splits * f.bn / 32.0) + epi / f.splits;
         if (t < least) { least = t; best = {f.cg, f.bn, f.splits}; }
     }
     return best;
@@ -753,10 +776,10 @@ mc_status_t linear_tile(int wb, const void* w, const uint16_t* x, uint32_t x_pit
                         const EpiArgs& ep, cudaStream_t stream, bool pdl) {
     TilePlan p = tile_plan(wb, M, N, K, (uint32_t)sm_count());
     if (const uint32_t f = g_forced.load(); f != 0u) p = {f >> 24, f & 0xFFFFu, (f >> 16) & 0xFFu};
-    const uint32_t blocks = (K + kBK - 1) / kBK;
-    while (p.splits > 1u && (p.splits > blocks || p.bn / p.splits < 32u || p.cg * p.splits > 8u)) p.splits >>= 1;   // a slice is never empty
+    const uint32_t per = kBK * stage_blocks(wb, (int)p.bn), stages = (K + per - 1u) / per;
+    while (p.splits > 1u && (p.splits > stages || (p.cg == 2u && p.bn / p.splits < 32u) || p.cg * p.splits > 8u)) p.splits >>= 1;   // a slice is never empty
     TileArgs a{};
-    a.ep = ep; a.M = M; a.N = N; a.nkb = blocks; a.n_out = ep.gated ? N / 2u : N; a.splits = p.splits;
+    a.ep = ep; a.M = M; a.N = N; a.n_out = ep.gated ? N / 2u : N; a.splits = p.splits;
     a.y_vec = aligned16(ep.y) && (ep.y_stride & 7u) == 0u;
     a.res_vec = aligned16(ep.res) && (ep.res_stride & 7u) == 0u;
     a.status = wait_status_sink();

@@ -21,8 +21,8 @@ struct LogitsArgs {
 // is 4 bytes a token; seen bits and masks are 1/16 of that, and counts are gathered for seen tokens only.  At full batches the
 // instructions bound it, not the bytes: most tokens are neither seen nor listed and stay the bits that they are, a mask is a
 // select on the packed words (64 rows of 122753 with every rule: 36 us with every token through the fp32 path, 24.5 us with
-// every piece that holds a touched token, 29.5 us with touched tokens always one a lane; the rule below 23 us, bound by latency
-// and instructions alike).
+// every piece that holds a touched token, 29.5 us with touched tokens always one a lane; the rule below 19.3 us, bound by
+// instructions, 37 a token, and latency alike).
 // Biases: the entries that fall into the span are kept in list order in shared memory; the thread of a token's first entry
 // adds up the others behind it: a fixed order, no floating-point atomics, any list length (512 entries at a time).
 constexpr uint32_t kOwn = 16, kSpan = kLogitsThreads * kOwn, kBiasBatch = 2 * kLogitsThreads, kFew = 64;
@@ -393,8 +393,8 @@ mc_status_t mc_sm100_token_history(const mc_sm100_token_history_t* call, void* s
     }
     const HistoryArgs a{d.d_counts, d.d_seen, d.n_slots, table_vocab, d.d_tokens, d.n_tokens, d.d_offsets, d.d_prompt_len, d.d_slots, d.d_status};
     if (d.rebuild != 0u) {
-        // One round of CTAs, four to an SM (512 threads, 56 KB each) where the batch allows it: spans of 2048 to 13664 tokens.
-        // 64 slots of 122753: 9 spans, 576 CTAs in one round; with spans of 16384 (three CTAs to an SM, two rounds) 13.5 us.
+        // One round of CTAs, four to an SM (56 KB each) where the batch allows it: spans of 2048 to 13664 tokens.
+        // 64 slots of 122753: 9 spans, 576 CTAs in one round: 10.9 us; with spans of 16384 (three CTAs to an SM, two rounds) 13.5 us.
         const uint64_t spans = 4ull * (uint32_t)sm_count() / n_seqs;
         uint64_t span = spans == 0 ? table_vocab : ((uint64_t)table_vocab + spans - 1u) / spans;
         span = span < 2048u ? 2048u : (span > 13664u ? 13664u : (span + 31u) & ~(uint64_t)31u);

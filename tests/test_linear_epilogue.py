@@ -65,7 +65,7 @@ def test_tile_plan(pkg):
             for N in (1, 63, 2304, 122753):
                 for K in (8, 64, 65, 2304, 30000):
                     cg, bn, s = pkg.debug_tile_plan(wb, M, N, K)
-                    assert (cg, bn) in ((1, 64), (1, 128), (2, 128), (2, 256)) and s in (1, 2, 4) and s <= -(-K // 64) and bn // s >= 32 and cg * s <= 8
+                    assert (cg, bn) in ((1, 64), (1, 128), (2, 128), (2, 256)) and s in (1, 2, 4) and s <= -(-K // 64) and bn // s >= (32 if cg == 2 else 16) and cg * s <= 8
         assert pkg.debug_tile_plan(wb, 300, 300, 300, 1)[0] in (1, 2)
 
 
@@ -122,7 +122,7 @@ SHAPES = [(1, 1, 1), (1, 2, 7), (2, 31, 16), (3, 130, 24), (5, 96, 72), (1, 2304
           (129, 514, 136), (200, 1026, 1040), (255, 30, 48), (256, 512, 512), (301, 770, 2304), (513, 258, 72), (1030, 130, 80)]
 
 
-PLANS = [(1, 64, 1), (1, 64, 2), (1, 128, 1), (1, 128, 2), (1, 128, 4), (2, 128, 1), (2, 128, 2), (2, 128, 4), (2, 256, 1), (2, 256, 2), (2, 256, 4)]
+PLANS = [(1, 64, 1), (1, 64, 2), (1, 64, 4), (1, 128, 1), (1, 128, 2), (1, 128, 4), (2, 128, 1), (2, 128, 2), (2, 128, 4), (2, 256, 1), (2, 256, 2), (2, 256, 4)]
 
 
 @pytest.mark.gpu
@@ -165,6 +165,8 @@ def test_activations(pkg, M, act, gated):
     for e4m3 in (False, True):
         _run(pkg, M, 196, 208, e4m3, bias=True, act=act, gated=gated, seed=M)
         _run(pkg, M, 196, 208, e4m3, residual=True, act=act, gated=gated, seed=M + 5)
+        if M == 20:
+            _run(pkg, 40, 196, 1200, e4m3, bias=True, residual=True, act=act, gated=gated, seed=M + 6)
 
 
 @pytest.mark.gpu

@@ -49,6 +49,18 @@ def test_logits_refusals(pkg):
     assert "struct_size=40" in pkg.last_error()
 
 
+def test_tables_take_what_every_tensor_holds(pkg):
+    """The binding counts rows that all tensors of a table have; a table that misses one is refused."""
+    import torch
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32)   # noqa: E731
+    f = pkg.LOGITS_TABLES.unpack(pkg.logits_tables(100, counts=i32(300), seen=i32(8), masks=i32(12), bias_token=i32(5), bias_value=torch.zeros(3)))
+    assert f[:6] == (72, 100, 2, 3, 3, 0)
+    for kw in (dict(counts=i32(300)), dict(seen=i32(8)), dict(bias_token=i32(5)), dict(bias_value=torch.zeros(3))):
+        with pytest.raises(pkg.McError) as e:
+            pkg.logits_process(16, 16, 1, 100, 100, 100, 16, pkg.logits_tables(100, **kw), stream=16)
+        assert e.value.status == pkg.MC_E_INVALID_ARGUMENT and "invalid tables" in e.value.message
+
+
 def test_history_refusals(pkg):
     base = dict(counts=16, seen=16, tokens=16, n_seqs=2, table_vocab=10, n_tokens=2, n_slots=2)
     for kw in (dict(counts=None), dict(seen=None), dict(tokens=None), dict(n_seqs=0), dict(table_vocab=0), dict(n_tokens=1), dict(n_slots=0),
