@@ -479,8 +479,8 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     asm volatile("bar.sync 1, %0;" ::"n"(EPI * 32u) : "memory");
                 }
                 // This CTA finishes columns [c_lo, c_hi), this warp every GROUPS-th chunk of them.  More slices than chunks: a
-                // chunk's rows are dealt out too, in `parts` of rows.
-                const uint32_t per = max(BN / S, 32u), parts = per * S / BN, rows = 128u / parts, part_of_warp = q * parts / 4u;
+                // chunk's rows are dealt out too, in `parts` of rows (pairs: never).
+                const uint32_t per = CG == 2 ? BN / S : max(BN / S, 32u), parts = CG == 2 ? 1u : per * S / BN, rows = 128u / parts, part_of_warp = q * parts / 4u;
                 const uint32_t c_lo = split / parts * per;
                 uint32_t c_hi = n0 + c_lo + per <= a.N ? c_lo + per : (a.N - n0 > c_lo ? a.N - n0 : c_lo);
                 if (part_of_warp != split % parts) c_hi = c_lo;
