@@ -1,6 +1,8 @@
 // linear_epilogue.cu -- mc_sm100_linear_epilogue: checks, choice of a kernel, and the kernel that takes every shape.
 #include "linear_epilogue.cuh"
 
+#include <type_traits>
+
 #include "fast_dispatch.cuh"
 #include "linear_rows.cuh"
 #include "linear_tile.cuh"
@@ -11,9 +13,10 @@ namespace mcl {
 namespace {
 
 // ---- any shape, any stride, any alignment ------------------------------------------------------
-// 64 x 64 tiles of y, K in steps of 32, mma.sync m16n8k16 with fp32 accumulators, plain element loads with bounds.
+// 64 x 64 tiles of y, K in steps of 64, mma.sync m16n8k16 with fp32 accumulators, plain element loads with bounds, a step's
+// loads in registers before the step in front of it is multiplied (610 x 5192 e4m3, M = 20: 192 us; element by element 772).
 // e4m3 codes are widened to bf16 (exact).  Each warp owns a 32 x 32 quarter.
-constexpr uint32_t kAnyTile = 64, kAnyK = 32, kAnyPitch = kAnyK + 8, kAnyThreads = 128;
+constexpr uint32_t kAnyTile = 64, kAnyK = 64, kAnyPitch = kAnyK + 8, kAnyThreads = 128;
 
 __device__ __forceinline__ void any_mma(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -33,17 +36,31 @@ linear_any_kernel(const void* __restrict__ w, const uint16_t* __restrict__ x, ui
     pdl_trigger();
     pdl_wait();
     float acc[2][4][4] = {};
-    for (uint32_t k0 = 0; k0 < K; k0 += kAnyK) {
-        for (uint32_t i = tid; i < kAnyTile * kAnyK; i += kAnyThreads) {
-            const uint32_t r = i / kAnyK, c = i % kAnyK, k = k0 + c;
-            sx[r][c] = (m0 + r < M && k < K) ? x[(size_t)(m0 + r) * x_stride + k] : (uint16_t)0;
-            uint16_t v = 0;
-            if (n0 + r < N && k < K) {
-                if constexpr (WB == 2) v = static_cast<const uint16_t*>(w)[(size_t)(n0 + r) * K + k];
-                else v = f32_to_bf16_bits(e4m3_to_f32(static_cast<const uint8_t*>(w)[(size_t)(n0 + r) * K + k]));
-            }
-            sw[r][c] = v;
+    constexpr uint32_t kEach = kAnyTile * kAnyK / kAnyThreads;               // elements of x, and of W, that a thread loads a step
+    using W = std::conditional_t<WB == 2, uint16_t, uint8_t>;
+    const uint32_t c = tid % kAnyK, r0 = tid / kAnyK;                        // one column, every second row
+    const W* wt = static_cast<const W*>(w);
+    uint16_t vx[kEach];
+    W vw[kEach];
+    auto fetch = [&](uint32_t k0) {
+        const bool in = k0 + c < K;
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const uint32_t r = r0 + i * (kAnyThreads / kAnyK);
+            vx[i] = in && m0 + r < M ? x[(size_t)(m0 + r) * x_stride + k0 + c] : (uint16_t)0;
+            vw[i] = in && n0 + r < N ? wt[(size_t)(n0 + r) * K + k0 + c] : (W)0;
         }
+    };
+    fetch(0);
+    for (uint32_t k0 = 0; k0 < K; k0 += kAnyK) {
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const uint32_t r = r0 + i * (kAnyThreads / kAnyK);
+            sx[r][c] = vx[i];
+            if constexpr (WB == 2) sw[r][c] = vw[i];
+            else sw[r][c] = f32_to_bf16_bits(e4m3_to_f32(vw[i]));
+        }
+        if (K - k0 > kAnyK) fetch(k0 + kAnyK);
         __syncthreads();
 #pragma unroll
         for (uint32_t kk = 0; kk < kAnyK; kk += 16) {
@@ -153,11 +170,11 @@ extern "C" mc_status_t mc_sm100_linear_epilogue(const mc_sm100_linear_epilogue_t
     }
     const bool tma = unit && (xs & 7u) == 0u;
     // Up to 64 rows the skinny kernel, which splits K eight ways and pads M to 16, 32 or 64.  From 17 rows on the tiled kernel
-    // is faster where K is short for the padded M (M = 32, 4096 x 448: 5.0 against 6.4 us; M = 64, 2304 x 1024: 6.8 against 9.1)
-    // or the weights have many rows (M = 33, lm_head 122753 x 2304: 95 against 115; M = 64, 11520 x 3008: 17.4 against 22.1);
-    // elsewhere it is slower (M = 32, 2304 x 1024 level; M = 64, 2304 x 5760: 16.7 against 12.9; M = 33, 20000 x 5760: 59 against
-    // 51).  Over 560 shapes the rule is within 0.5 % of the better one on average, 18 % in the worst case (M = 33, 480 x 1024).
-    const bool short_k = M > 16u && K <= (M <= 32u ? 512u : 1024u), tall = M > 24u && N >= 5000u && K <= 72u * M;
+    // is faster where K is short for the padded M (M = 32, 4096 x 448: 5.0 against 6.4 us; M = 64, 2304 x 1024: 6.0 against 9.1)
+    // or, from 33 on, the weights have many rows (M = 33, lm_head 122753 x 2304: 95 against 115; M = 64, 11520 x 3008: 17.4 against
+    // 22.1); elsewhere it is slower (M = 32, 11520 x 1536: a third; M = 64, 2304 x 5760: 16.7 against 13.8).  Over 1900 timings
+    // (M 17 .. 64, N 480 .. 122753, K 256 .. 5760) the rule is within 1 % of the better one on average, 32 % in the worst case.
+    const bool short_k = M > 16u && K <= (M <= 32u ? 640u : 1280u), tall = M > 32u && N >= 4096u && K <= 80u * M;
     const bool tiled = M > 64u || tile_forced() || short_k || tall;
     if (wb == 1 && M <= 16u && tma && !tile_forced() && linear_rows_ok(M, K, xs))
         return linear_rows(static_cast<const uint8_t*>(d_w), d_x, xs, M, N, K, e, st, true);

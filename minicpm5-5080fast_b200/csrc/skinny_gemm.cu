@@ -111,6 +111,9 @@ template <int MODE, int NPAD> struct Ring {
     __host__ __device__ static constexpr uint32_t bytes(uint32_t ops, uint32_t raws) { return ops * (A_OP + B_OP) + raws * A_RAW; }
 };
 
+// Features that each CTA of a cluster of S finishes: pairs stay together, all eight of them (S a power of two) even shares.
+__host__ __device__ constexpr uint32_t slice_rows(uint32_t S) { return 2u * ((kTileN / 2u + S - 1u) / S); }
+
 }  // namespace
 
 // MODE: SKINNY_W_BF16 / SKINNY_W_E4M3 / SKINNY_W8A8.  NPAD: MMA N (16, 32 or 64).  EXT: fused epilogue.
@@ -305,12 +308,13 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     // (3) each owner sums its S partials from its own shared memory in rank order, scales, stores.
     // Nothing remote is touched after the barrier, so no CTA waits for its peers before it exits.
     const uint32_t S = a.splits, rank = split;
-    const uint32_t per_n = kTileN / S;                               // features per owner (S divides 128)
+    const uint32_t per_n = slice_rows(S);                            // features per owner (the last one may have fewer)
     constexpr uint32_t PITCH = NPAD + 4;                             // fp32 per feature row: 16-byte aligned pushes, spread banks
     const uint32_t part_s = base + G::bytes(OPS, E4 ? RAWS : 0);     // part[S][per_n][PITCH] fp32
-    // fused epilogue: this thread's outputs (the slice is a power of two wide), and its first residuals under the products
-    const uint32_t e_gate = EXT ? a.ep.gated : 0u, e_outs = per_n >> e_gate, e_shift = 31u - (uint32_t)__clz((int)e_outs);
-    const uint32_t e_base = ((uint32_t)n0 + rank * per_n) >> e_gate, e_limit = a.N >> e_gate;
+    // fused epilogue: this thread's outputs (counted over a power of two of columns), and its first residuals under the products
+    const uint32_t e_gate = EXT ? a.ep.gated : 0u, e_own = min(per_n, kTileN - min(rank * per_n, (uint32_t)kTileN)) >> e_gate;
+    const uint32_t e_shift = 32u - (uint32_t)__clz((int)((per_n >> e_gate) - 1u)), e_outs = 1u << e_shift;
+    const uint32_t e_base = ((uint32_t)n0 + rank * per_n) >> e_gate, e_limit = min(a.N >> e_gate, e_base + e_own);
     auto res_of = [&](uint32_t idx) {
         const uint32_t m = idx >> e_shift, j = e_base + (idx & (e_outs - 1u));
         return a.ep.res != nullptr && m < a.M && j < e_limit ? a.ep.res[(size_t)m * a.ep.res_stride + j] : (uint16_t)0x8000u;   // -0 changes no sum
@@ -462,13 +466,28 @@ struct Plan { uint32_t tiles, splits; };
 
 // Cluster size along K: the largest of 8/4/2/1 that keeps the grid within two CTAs per SM
 // and leaves every CTA at least two K blocks.
-Plan make_plan(uint32_t N, uint32_t K, uint32_t bk) {
+Plan make_plan(uint32_t N, uint32_t K, uint32_t bk, bool ext) {
     Plan p;
     p.tiles = (N + kTileN - 1) / kTileN;
-    const uint32_t nkb = (K + bk - 1) / bk;
-    const uint32_t room = 2u * (uint32_t)sm_count();
+    const uint32_t nkb = (K + bk - 1) / bk, sms = (uint32_t)sm_count();
+    const uint32_t room = 2u * sms;
     uint32_t s = 8;
-    while (s > 1 && (p.tiles * s > room || nkb / s < 2)) s >>= 1;
+    if (!ext) {
+        while (s > 1 && (p.tiles * s > room || nkb / s < 2)) s >>= 1;
+    } else {
+        // Any number of slices whose clusters run at once, two CTAs to an SM (packed into TPCs and GPCs; an eighth more would
+        // start when the first have left: 6000 x 2304, M = 33, in clusters of six 20.9 us, of four 13.0): the one with the least
+        // K blocks in a row, a second CTA on an SM counted half (the two hide each other's waits).  Against the largest power of
+        // two, M = 20: 11520 x 2304 in three slices instead of two 14.5 -> 13.6 us, e4m3 18.8 -> 15.5; 5720 x 7232 in five instead
+        // of four 19.4 -> 17.8, e4m3 26.4 -> 22.7.
+        static const uint32_t at_once[9] = {0, 296, 148, 90, 74, 52, 44, 30, 33};        // of 148 SMs
+        uint64_t least = ~0ull;
+        for (uint32_t c = 8; c >= 1; --c) {
+            if (c > 1 && ((uint64_t)p.tiles * 148u > (uint64_t)at_once[c] * sms || nkb / c < 2)) continue;
+            const uint64_t ctas = (uint64_t)p.tiles * c, load = (nkb + c - 1u) / c * (ctas > sms ? sms + ctas : 2ull * sms);
+            if (load < least) { least = load; s = c; }
+        }
+    }
     p.splits = s;
     return p;
 }
@@ -484,7 +503,7 @@ mc_status_t launch_one(const void* w, const void* x, uint32_t x_pitch, const Ski
         set_error("skinny_gemm: cannot raise shared memory to %zu: %s", smem_max, cudaGetErrorString(ae));
         return MC_E_CUDA;
     }
-    const size_t smem = (size_t)G::bytes(a.op_stages, MODE == SKINNY_W_E4M3 ? a.raw_stages : 0) + (size_t)(NPAD + 4) * kTileN * 4 + 2048;
+    const size_t smem = (size_t)G::bytes(a.op_stages, MODE == SKINNY_W_E4M3 ? a.raw_stages : 0) + (size_t)(NPAD + 4) * a.splits * slice_rows(a.splits) * 4 + 2048;
     CUtensorMap map_w, map_x;
     mc_status_t s;
     if (EXT) {      // nothing is kept from call to call
@@ -539,8 +558,8 @@ bool skinny_shape_ok(uint32_t N, uint32_t K, int wb) {
 size_t skinny_workspace_bytes(uint32_t, uint32_t, uint32_t) { return 0; }
 
 // What a call needs besides its operands: K slices, ring depths, the hints of this thread.
-static uint32_t plan_args(int mode, uint32_t M, uint32_t N, uint32_t K, SkinnyArgs& a) {
-    const Plan p = make_plan(N, K, mode == SKINNY_W8A8 ? 128u : 64u);
+static uint32_t plan_args(int mode, uint32_t M, uint32_t N, uint32_t K, SkinnyArgs& a, bool ext) {
+    const Plan p = make_plan(N, K, mode == SKINNY_W8A8 ? 128u : 64u, ext);
     a.M = M; a.N = N; a.K = K; a.splits = p.splits;
     const uint32_t grid = p.tiles * p.splits;
     a.pf = make_prefetch_args(take_next_weights(), grid);
@@ -551,7 +570,7 @@ static uint32_t plan_args(int mode, uint32_t M, uint32_t N, uint32_t K, SkinnyAr
     // no longer become resident (and prefetch its weights) while this one drains.
     const uint32_t npad = M <= 16 ? 16u : (M <= 32 ? 32u : 64u);
     const uint32_t op_stage = (uint32_t)(kTileN + npad) * kRowBytes;
-    const uint32_t budget = 108u * 1024u - (npad + 4u) * kTileN * 4u - 1024u;  // minus the split-K exchange region
+    const uint32_t budget = 108u * 1024u - (npad + 4u) * p.splits * slice_rows(p.splits) * 4u - 1024u;  // minus the split-K exchange region
     if (mode == SKINNY_W_E4M3) {
         // operand ring of 3 (2 when the raw ring would otherwise drop below 2 stages)
         a.op_stages = (budget >= 3u * op_stage + 2u * kTileN * 64u) ? 3u : 2u;
@@ -579,7 +598,7 @@ mc_status_t skinny_gemm(int mode, const void* w, const float* w_scale, const uin
     SkinnyArgs a{};
     a.w_scale = w_scale; a.x_scale = x_scale; a.y = y; a.swiglu = swiglu ? 1u : 0u;
     if (out != nullptr) a.out = *out;
-    const uint32_t grid = plan_args(mode, M, N, K, a);
+    const uint32_t grid = plan_args(mode, M, N, K, a, false);
     if (mode == SKINNY_W_BF16) return launch_mode<SKINNY_W_BF16, false>(w, x, x_pitch, a, grid, stream, pdl);
     if (mode == SKINNY_W_E4M3) return launch_mode<SKINNY_W_E4M3, false>(w, x, x_pitch, a, grid, stream, pdl);
     return launch_mode<SKINNY_W8A8, false>(w, x, x_pitch, a, grid, stream, pdl);
@@ -589,7 +608,7 @@ mc_status_t skinny_gemm_fused(int mode, const void* w, const uint16_t* x, uint32
                               const EpiArgs& ep, cudaStream_t stream, bool pdl) {
     SkinnyArgs a{};
     a.w_scale = ep.scale; a.y = ep.y; a.ep = ep;
-    const uint32_t grid = plan_args(mode, M, N, K, a);
+    const uint32_t grid = plan_args(mode, M, N, K, a, true);
     if (mode == SKINNY_W_BF16) return launch_mode<SKINNY_W_BF16, true>(w, x, x_pitch, a, grid, stream, pdl);
     return launch_mode<SKINNY_W_E4M3, true>(w, x, x_pitch, a, grid, stream, pdl);
 }
