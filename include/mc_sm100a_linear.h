@@ -448,7 +448,7 @@ MC_SM100_API mc_status_t mc_sm100_logits_process(const mc_sm100_logits_process_t
 
 typedef struct mc_sm100_token_history_t {
     uint32_t struct_size;            /* caller sets sizeof(mc_sm100_token_history_t) */
-    uint32_t n_slots, table_vocab, n_tokens, n_seqs;
+    uint32_t n_slots, table_vocab, n_tokens, n_seqs;   /* each < 2^31, table_vocab <= 2^28 */
     uint32_t rebuild;                /* 0 or 1 */
     int32_t*  d_counts;              /* [n_slots, table_vocab] */
     uint32_t* d_seen;                /* [n_slots, ceil(table_vocab / 32)] */

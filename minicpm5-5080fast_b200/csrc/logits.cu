@@ -337,6 +337,9 @@ __global__ void __launch_bounds__(kLogitsThreads) history_add_kernel(const Histo
     }
 }
 
+// Tables are words: misaligned ones are refused, not read.
+template <typename... P> bool words_aligned(const P*... p) { return ((reinterpret_cast<uintptr_t>(p) | ...) & 3u) == 0u; }
+
 }  // namespace
 
 }  // namespace mcl
@@ -365,7 +368,8 @@ mc_status_t mc_sm100_logits_process(const mc_sm100_logits_process_t* call, const
     const mc_sm100_logits_tables_t& t = *tables;
     if (t.struct_size != sizeof(mc_sm100_logits_tables_t) || t.reserved != 0u || t.table_vocab > 0x10000000u ||
         (uint64_t)index_base + vocab > t.table_vocab || (t.n_slots != 0u && (t.d_counts == nullptr || t.d_seen == nullptr)) ||
-        (t.n_masks != 0u && t.d_mask == nullptr) || (t.n_bias != 0u && (t.d_bias_token == nullptr || t.d_bias_value == nullptr))) {
+        (t.n_masks != 0u && t.d_mask == nullptr) || (t.n_bias != 0u && (t.d_bias_token == nullptr || t.d_bias_value == nullptr)) ||
+        !words_aligned(call->d_cfg, t.d_counts, t.d_seen, t.d_mask, t.d_bias_token, t.d_bias_value, t.d_status)) {
         set_error("%s: invalid tables (struct_size=%u table_vocab=%u slots=%u masks=%u biases=%u) for columns %d..%llu", who, t.struct_size,
                   t.table_vocab, t.n_slots, t.n_masks, t.n_bias, index_base, (unsigned long long)((uint64_t)index_base + vocab));
         return MC_E_INVALID_ARGUMENT;
@@ -387,7 +391,8 @@ mc_status_t mc_sm100_token_history(const mc_sm100_token_history_t* call, void* s
     const uint32_t n_seqs = d.n_seqs, table_vocab = d.table_vocab;
     if (d.d_counts == nullptr || d.d_seen == nullptr || d.n_slots == 0 || d.n_slots > 0x7FFFFFFFu || table_vocab == 0 || table_vocab > 0x10000000u ||
         (d.d_tokens == nullptr && d.n_tokens != 0u) || n_seqs == 0 || n_seqs > 0x7FFFFFFFu || (d.d_offsets == nullptr && d.n_tokens < n_seqs) ||
-        (d.d_slots == nullptr && n_seqs > d.n_slots)) {
+        (d.d_slots == nullptr && n_seqs > d.n_slots) || d.n_tokens > 0x7FFFFFFFu ||
+        !words_aligned(d.d_counts, d.d_seen, d.d_tokens, d.d_offsets, d.d_prompt_len, d.d_slots, d.d_status)) {
         set_error("mc_sm100_token_history: invalid args (slots=%u vocab=%u tokens=%u sequences=%u)", d.n_slots, table_vocab, d.n_tokens, n_seqs);
         return MC_E_INVALID_ARGUMENT;
     }

@@ -61,6 +61,22 @@ def test_tables_take_what_every_tensor_holds(pkg):
         assert e.value.status == pkg.MC_E_INVALID_ARGUMENT and "invalid tables" in e.value.message
 
 
+def test_misaligned_tables_are_refused(pkg):
+    for i in range(6, 12):
+        t = [72, 100, 1, 1, 1, 0, 16, 16, 16, 16, 16, 16]
+        t[i] = 18
+        with pytest.raises(pkg.McError) as e:
+            pkg.logits_process(16, 16, 1, 100, 100, 100, 16, pkg.LOGITS_TABLES.pack(*t), stream=16)
+        assert e.value.status == pkg.MC_E_INVALID_ARGUMENT and "invalid tables" in e.value.message
+    ok = dict(counts=16, seen=16, tokens=16, offsets=16, prompt_len=16, slots=16, status=16)
+    for bad in [{k: 18} for k in ok] + [dict(n_tokens=2 ** 31)]:
+        kw = dict(ok, n_seqs=1, table_vocab=100, n_slots=1, n_tokens=4, stream=16)
+        kw.update(bad)
+        with pytest.raises(pkg.McError) as e:
+            pkg.token_history(**kw)
+        assert e.value.status == pkg.MC_E_INVALID_ARGUMENT and "invalid args" in e.value.message
+
+
 def test_history_refusals(pkg):
     base = dict(counts=16, seen=16, tokens=16, n_seqs=2, table_vocab=10, n_tokens=2, n_slots=2)
     for kw in (dict(counts=None), dict(seen=None), dict(tokens=None), dict(n_seqs=0), dict(table_vocab=0), dict(n_tokens=1), dict(n_slots=0),
