@@ -9,9 +9,9 @@
 // Blocks of 16 weight rows are dealt to the CTAs as contiguous near-equal ranges; a CTA works on R blocks at a time, KW = 16 / R
 // warps to a block, which take its 64-element K steps round-robin; their partial tiles meet in shared memory and are added in
 // warp order.  Bound by latency where N is small, by the bit placement and mma.sync where it is large (lm_head M = 2: 3.4 TB/s).
-// Measured (us, this kernel / skinny): 2304 x 5760 M = 8 8.8 / 12.6, M = 16 12.8 / 12.8; 11520 x 2304 M = 8 12.5 / 17.2, M = 16
-// 15.3 / 18.0; 20000 x 4096 M = 8 31.5 / 49, M = 16 39 / 50; 122753 x 2304 M = 8 89 / 106, M = 16 114 / 112.  Four column blocks
-// (M <= 32) lost: 11520 x 2304 23.8 / 19.8.
+// Measured (us, this kernel / skinny): 2304 x 5760 M = 8 8.9 / 12.6, M = 16 12.7 / 12.4; 11520 x 2304 M = 8 12.7 / 13.9, M = 16
+// 15.3 / 14.6; 20000 x 4096 M = 8 31.4 / 49, M = 16 39 / 50; 122753 x 2304 M = 8 89 / 107, M = 16 114 / 112.  Four column blocks
+// (M <= 32) lost: 11520 x 2304 23.8 / 16.4.
 #include "linear_rows.cuh"
 
 #include "gemv_fast.cuh"

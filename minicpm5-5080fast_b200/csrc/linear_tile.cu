@@ -1,10 +1,10 @@
-// linear_tile.cu -- y = epilogue(x W^T) for M > 64 on the 5th-generation tensor cores.
+// linear_tile.cu -- y = epilogue(x W^T) for M > 64 (from 17 rows on in places) on the 5th-generation tensor cores.
 //
 // The MMA's A operand is a tile of 128 activation rows per CTA, B a tile of BN weight rows, D [128 x BN] fp32 in TMEM (lane =
 // activation row, column = feature).  With CG = 2 two CTAs of a cluster work on one 256 x BN tile (cta_group::2): each loads
 // its own 128 activation rows and HALF of the weight rows, so a weight row enters shared memory once per 256 activation rows.
 //   first EPI warps: epilogue (warp w reads TMEM lanes 32 (w % 4) .. + 31; groups of four take alternate column chunks)
-//   next            : TMA producer of the ring of (A, B) stages, 64 K elements = one 128-byte swizzled row each
+//   next            : TMA producer of the ring of (A, B) stages, one or two K blocks each (64 K elements = a 128-byte swizzled row)
 //   next            : MMA issuer (of the pair's first CTA)
 //   e4m3 only, next : TMA producer of raw weight tiles; one warp idle; then eight warps that widen raw tiles to bf16 (exact)
 //                     into the B stages, two groups of four on alternate K blocks
