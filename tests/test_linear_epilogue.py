@@ -383,3 +383,79 @@ def test_waits_for_the_kernel_before(pkg, M):
         pkg.launch_linear_epilogue(dst[0], None, dst[1], y, M, N, K, bias=dst[2], residual=dst[3])
         pkg.launch_linear_epilogue(dst[0], None, dst[1], y, M, N, K, bias=dst[2], residual=dst[3])
         assert torch.equal(y, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 12, 40, 300])
+def test_waits_for_both_streams_it_joins(pkg, M):
+    """x comes from this stream's short kernel, the residual from another stream's long one, joined by an event; eager and replayed."""
+    import torch
+    N, K, L = 512, 256, 8192
+    g = torch.Generator(device="cuda")
+    g.manual_seed(M)
+    w1, w2 = [(torch.randn(*s, generator=g, device="cuda") * 0.05).bfloat16() for s in ((K, 64), (N, K))]
+    wl = (torch.randn(L, 2048, generator=g, device="cuda") * 0.02).bfloat16()
+    x0 = torch.randn(M, 64, generator=g, device="cuda").bfloat16()
+    xl = torch.randn(1024, 2048, generator=g, device="cuda").bfloat16()
+    x1, long, y = [torch.full(s, float("nan"), dtype=torch.bfloat16, device="cuda") for s in ((M, K), (1024, L), (M, N))]
+    side = torch.cuda.Stream()
+
+    def run(apart):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side if apart else torch.cuda.current_stream()):
+            for _ in range(3):
+                pkg.launch_linear_epilogue(wl, None, xl, long, 1024, L, 2048)
+        pkg.launch_linear_epilogue(w1, None, x0, x1, M, K, 64, activation="silu")
+        torch.cuda.current_stream().wait_stream(side)
+        # the last rows that the long kernel writes
+        pkg.launch_linear_epilogue(w2, None, x1, y, M, N, K, residual=long[1024 - M:, L - N:], residual_stride=L)
+    run(False)
+    torch.cuda.synchronize()
+    want = y.clone()
+    assert torch.isfinite(want.float()).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(True)
+    for replay in (False, True, True):
+        for t in (x1, long, y):
+            t.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graph.replay() if replay else run(True)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want), replay
+
+
+@pytest.mark.gpu
+def test_several_threads(pkg):
+    """Four host threads, each with its own stream, shapes and types; every call gives the bits it gives alone."""
+    import threading
+    import torch
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    jobs = []
+    for M, N, K, e4m3 in ((1, 700, 512, False), (9, 700, 512, True), (40, 1500, 2048, False), (300, 640, 512, True)):
+        w = torch.randint(0, 0x70, (N, K), dtype=torch.uint8, generator=g, device="cuda") if e4m3 else torch.randn(N, K, generator=g, device="cuda").bfloat16()
+        sc = torch.rand(N, generator=g, device="cuda") if e4m3 else None
+        x = torch.randn(M, K, generator=g, device="cuda").bfloat16()
+        ys = [torch.empty(M, N, dtype=torch.bfloat16, device="cuda") for _ in range(25)]
+        pkg.launch_linear_epilogue(w, sc, x, ys[0], M, N, K, activation="gelu")
+        jobs.append((M, N, K, w, sc, x, ys, ys[0].clone(), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(M, N, K, w, sc, x, ys, _, stream):
+        try:
+            with torch.cuda.stream(stream):
+                for y in ys:
+                    pkg.launch_linear_epilogue(w, sc, x, y, M, N, K, activation="gelu")
+        except Exception as e:      # reported by the main thread
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for j in jobs:
+        assert all(torch.equal(y, j[7]) for y in j[6])
