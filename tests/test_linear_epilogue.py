@@ -119,7 +119,8 @@ def _run(pkg, M, N, K, e4m3=False, bias=False, residual=False, act="none", gated
 
 SHAPES = [(1, 1, 1), (1, 2, 7), (2, 31, 16), (3, 130, 24), (5, 96, 72), (1, 2304, 2304), (1, 257, 5760), (4, 514, 256), (7, 65, 777), (8, 1000, 512),
           (16, 3456, 256), (17, 258, 1040), (33, 300, 2304), (64, 128, 64), (65, 128, 64), (100, 66, 96), (127, 384, 320), (128, 256, 128),
-          (129, 514, 136), (200, 1026, 1040), (255, 30, 48), (256, 512, 512), (301, 770, 2304), (513, 258, 72), (1030, 130, 80)]
+          (129, 514, 136), (200, 1026, 1040), (255, 30, 48), (256, 512, 512), (301, 770, 2304), (513, 258, 72), (1030, 130, 80),
+          (70, 1, 64), (2000, 2, 16), (17, 1, 16), (33, 7, 32), (20, 1411, 3600), (24, 5720, 720), (12, 2310, 1600)]
 
 
 PLANS = [(1, 64, 1), (1, 64, 2), (1, 64, 4), (1, 128, 1), (1, 128, 2), (1, 128, 4), (2, 128, 1), (2, 128, 2), (2, 128, 4), (2, 256, 1), (2, 256, 2), (2, 256, 4)]
