@@ -21,9 +21,12 @@ struct LogitsArgs {
 // is 4 bytes a token; seen bits and masks are 1/16 of that, and counts are gathered for seen tokens only.  At full batches the
 // instructions bound it, not the bytes: most tokens are neither seen nor listed and stay the bits that they are, a mask is a
 // select on the packed words (64 rows of 122753 with every rule: 36 us with every token through the fp32 path, 24.5 us with
-// every piece that holds a touched token, 29.5 us with touched tokens always one a lane; the rule below 19.3 us, bound by
-// instructions, 37 a token, and latency alike).
-// Biases: the entries that fall into the span are kept in list order in shared memory; the thread of a token's first entry
+// every piece that holds a touched token, 29.5 us with touched tokens always one a lane; the rule below 16.3 us, 11.4 in a chain, bound by
+// instructions and latency alike).
+// The rows' first spans go first: the most frequent tokens, seen or listed (twice, too), are a vocabulary's first, and the CTAs
+// that hold them take longest (64 rows with 300 biases each, in a chain: 11.4 us; a row's spans one after another 13.8).
+// Biases: a token that the list holds once takes its value straight away.  If one of a span's is listed twice, the entries
+// that fall into the span are kept in list order in shared memory; the thread of a token's first entry
 // adds up the others behind it: a fixed order, no floating-point atomics, any list length (512 entries at a time).
 constexpr uint32_t kOwn = 16, kSpan = kLogitsThreads * kOwn, kBiasBatch = 2 * kLogitsThreads, kFew = 64;
 
@@ -33,15 +36,16 @@ __global__ void __launch_bounds__(kLogitsThreads, 5) logits_process_kernel(const
     __shared__ float s_value[kBiasBatch];
     __shared__ uint2 s_touched[kLogitsThreads / 32][kFew];
     __shared__ uint32_t s_listed[kSpan / 32], s_once[kSpan / 32], s_again[kSpan / 32], s_warp[kBiasBatch / 32];
-    const uint32_t row = blockIdx.y, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    const uint32_t row = blockIdx.x, block = blockIdx.z * gridDim.y + blockIdx.y, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     pdl_trigger();
+    for (uint32_t w = tid; w < kSpan / 32; w += kLogitsThreads) s_once[w] = 0u;
     pdl_wait();
     const mc_sm100_logits_config_t c = a.cfg[row];
     const uint16_t* in = a.in + (size_t)row * a.row_stride;
     uint16_t* out = a.out + (size_t)row * a.out_stride;
     // this thread's columns first .. + 15; those below 0 or beyond the row are not there
     const int32_t head = (int32_t)((reinterpret_cast<uintptr_t>(out) & 31u) >> 1), vocab = (int32_t)a.vocab;
-    const int32_t span0 = (int32_t)(blockIdx.x * kSpan) - head, first = span0 + (int32_t)(tid * kOwn);
+    const int32_t span0 = (int32_t)(block * kSpan) - head, first = span0 + (int32_t)(tid * kOwn);
     const bool together = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 31u) == 0u;
     const bool whole = first >= 0 && first + (int32_t)kOwn <= vocab;
     uint32_t raw[8];
@@ -59,7 +63,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 5) logits_process_kernel(const
     const bool history = c.history_slot >= 0 && (uint32_t)c.history_slot < a.t.n_slots;
     const bool masked = c.mask_row >= 0 && (uint32_t)c.mask_row < a.t.n_masks;
     const uint64_t end64 = (uint64_t)c.bias_begin + c.bias_count;
-    if (a.t.d_status != nullptr && blockIdx.x == 0u && tid == 0u &&
+    if (a.t.d_status != nullptr && block == 0u && tid == 0u &&
         ((c.history_slot >= 0 && !history) || (c.mask_row >= 0 && !masked) || (c.bias_count != 0u && end64 > a.t.n_bias)))
         *a.t.d_status = 1;
     // the bits of a table row that belong to the columns, bit e = column first + e, 0 where there is none
@@ -77,11 +81,9 @@ __global__ void __launch_bounds__(kLogitsThreads, 5) logits_process_kernel(const
     if (begin < end) {                                                               // the same for every thread
         const int32_t lo = span0 < 0 ? 0 : span0, hi = span0 + (int32_t)kSpan < vocab ? span0 + (int32_t)kSpan : vocab;
         const bool one = end - begin <= kBiasBatch;
-        if (!one)
-            for (uint32_t w = tid; w < kSpan / 32; w += kLogitsThreads) s_listed[w] = 0u;
-        for (uint32_t j0 = begin; j0 < end; j0 = end - j0 > kBiasBatch ? j0 + kBiasBatch : end) {
-            uint32_t col[2], hits[2];
-            float value[2];
+        uint32_t col[2];
+        float value[2];
+        auto load = [&](uint32_t j0) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const uint32_t d = (uint32_t)h * kLogitsThreads + tid;
@@ -91,6 +93,27 @@ __global__ void __launch_bounds__(kLogitsThreads, 5) logits_process_kernel(const
                 if (d < end - j0) { const int32_t tok = a.t.d_bias_token[j0 + d]; column = tok < 0 ? -1 : tok - a.index_base; value[h] = a.t.d_bias_value[j0 + d]; }
                 col[h] = column >= lo && column < hi ? (uint32_t)(column - span0) : 0xFFFFFFFFu;
             }
+        };
+        bool several = !one;
+        if (one) {
+            // no token of the span listed twice, as nearly always: its one entry is its sum
+            load(begin);
+            __syncthreads();                                                         // s_once is zero
+            int twice = 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (col[h] != 0xFFFFFFFFu) {
+                    const uint32_t bit = 1u << (col[h] & 31u);
+                    if (atomicOr(&s_once[col[h] >> 5], bit) & bit) twice = 1;
+                    else s_sum[col[h]] = __fadd_rn(0.f, value[h]);
+                }
+            several = __syncthreads_or(twice) != 0;
+        } else {
+            for (uint32_t w = tid; w < kSpan / 32; w += kLogitsThreads) s_listed[w] = 0u;
+        }
+        for (uint32_t j0 = begin; several && j0 < end; j0 = end - j0 > kBiasBatch ? j0 + kBiasBatch : end) {
+            uint32_t hits[2];
+            if (!one) load(j0);
             for (uint32_t w = tid; w < kSpan / 32; w += kLogitsThreads) s_once[w] = s_again[w] = 0u;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -375,7 +398,8 @@ mc_status_t mc_sm100_logits_process(const mc_sm100_logits_process_t* call, const
         return MC_E_INVALID_ARGUMENT;
     }
     const LogitsArgs a{call->d_logits, call->d_out, vocab, row_stride, out_stride, index_base, call->d_cfg, t};
-    (void)launch(logits_process_kernel, dim3((vocab + kOwn - 1u + kSpan - 1u) / kSpan, n_rows), dim3(kLogitsThreads), 0,
+    const uint32_t spans = (vocab + kOwn - 1u + kSpan - 1u) / kSpan, deep = (spans + 65534u) / 65535u;
+    (void)launch(logits_process_kernel, dim3(n_rows, (spans + deep - 1u) / deep, deep), dim3(kLogitsThreads), 0,
                  (cudaStream_t)stream, true, a);
     MCL_CHECK_LAUNCH("logits_process");
     return MC_OK;
