@@ -734,7 +734,8 @@ MC_SM100_API void mc_sm100_debug_mma_rows_plan(uint32_t N, uint32_t sms, uint32_
 MC_SM100_API void mc_sm100_debug_chain_plan(int32_t fp8, uint32_t hidden, uint32_t inter, uint32_t* slot_bytes, uint32_t* rows_hidden,
                                             uint32_t* rows_gate_up, uint32_t* rows_down);
 
-/* How mc_sm100_linear_epilogue cuts a call of more than 64 rows that takes the tiled tensor-core kernel (host logic alone):
+/* How mc_sm100_linear_epilogue cuts a call that takes the tiled tensor-core kernel (more than 64 rows; from 17 on where K is short
+ * or the weights have many rows; host logic alone):
  * CTAs per tile (1 or 2, 128 rows each), features per tile, K slices.  set_tile_plan: A/B and test hook (process-wide),
  * every such call takes this plan (cg = 0: the rule again; as many K slices as fit the shape).  No plan changes a result
  * beyond the order of its sums. */

@@ -431,7 +431,7 @@ def debug_tile_plan(bytes_per_weight: int, M: int, N: int, K: int, sms: int = 14
 
 
 def debug_set_tile_plan(cg: int = 0, bn: int = 0, splits: int = 1) -> None:
-    """Fused linears of more than 64 rows take this plan (cg = 0: the library's rule)."""
+    """Fused linears whose rows TMA can read take the tiled kernel with this plan (cg = 0: the library's rule)."""
     lib().mc_sm100_debug_set_tile_plan(cg, bn, splits)
 
 
