@@ -460,3 +460,28 @@ def test_several_threads(pkg):
     assert not errors
     for j in jobs:
         assert all(torch.equal(y, j[7]) for y in j[6])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ACTS)
+def test_activations_over_every_bf16(pkg, act):
+    """z runs through every bf16 value: the activation's own error, tails, infinities and NaN included."""
+    import gpu_util as g
+    bits = np.arange(65536, dtype=np.uint16)
+    x = np.zeros((65536, 8), np.uint16)
+    x[:, 0] = bits
+    w = np.zeros((8, 8), np.uint16)
+    w[:, 0] = 0x3F80                                            # 1.0
+    y = g.empty_u16(65536, 8)
+    pkg.launch_linear_epilogue(g.dev(w), None, g.dev(x), y, 65536, 8, 8, activation=act)
+    g.sync()
+    z = onp.bf16_to_f32(bits).astype(np.float64)
+    got = onp.bf16_to_f32(g.host_u16(y).reshape(65536, 8)).astype(np.float64)
+    assert np.array_equal(got, np.repeat(got[:, :1], 8, axis=1), equal_nan=True)
+    ok = np.isfinite(z)
+    with np.errstate(over="ignore"):
+        want, bound = onp.linear_epilogue_f64(np.ones((1, 1)), z[ok][:, None], act=act)
+    d = np.abs(got[ok, 0] - want[:, 0])
+    assert np.all(d <= bound[:, 0]), (act, z[ok][np.argmax(d / bound[:, 0])], float(np.max(d / bound[:, 0])))
+    assert np.isnan(got[np.isnan(z), 0]).all()
+    assert got[np.isposinf(z), 0][0] == np.inf
