@@ -23,26 +23,36 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // no synchronisation; cudaDeviceGetAttribute is a host-side query).
 int sm_count();
 
-// Dynamic shared memory above 48 KB has to be opted into per kernel AND per device
-// (cudaFuncSetAttribute acts on the current device).  One SmemOptIn per kernel instantiation
-// remembers what each device was raised to; host threads may race through it.
+// Without an opt-in a launch may take 48 KB of shared memory, the kernel's own static part included; what goes beyond has to
+// be opted into per kernel AND per device (cudaFuncSetAttribute acts on the current device).  One SmemOptIn per kernel
+// instantiation remembers the static part and what each device was raised to; host threads may race through it.
 constexpr int kMaxDevices = 64;
+constexpr size_t kSharedWithoutOptIn = 48u * 1024u;
 struct SmemOptIn {
     std::atomic<uint32_t> set[kMaxDevices];
+    std::atomic<uint32_t> known_static;        // bytes of static shared memory + 1; 0 = not asked yet
     std::mutex mu;
     // true when `bytes` of dynamic shared memory are usable by `kern` on the current device
     template <typename Kern>
     cudaError_t ensure(Kern kern, size_t bytes) {
-        if (bytes <= 48u * 1024u) return cudaSuccess;
+        uint32_t known = known_static.load(std::memory_order_relaxed);
+        if (known == 0u) {
+            cudaFuncAttributes at{};
+            const cudaError_t e = cudaFuncGetAttributes(&at, kern);
+            if (e != cudaSuccess) return e;
+            known = (uint32_t)at.sharedSizeBytes + 1u;
+            known_static.store(known, std::memory_order_relaxed);
+        }
+        if (bytes + (known - 1u) <= kSharedWithoutOptIn) return cudaSuccess;
         int dev = 0;
         const cudaError_t e = cudaGetDevice(&dev);
         if (e != cudaSuccess) return e;
-        return ensure_on(dev, bytes, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes); });
+        return ensure_on(dev, bytes, known - 1u, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes); });
     }
     // the bookkeeping alone: `raise` performs the opt-in on device `dev` (a fake in the host-side self-test)
     template <typename Raise>
-    cudaError_t ensure_on(int dev, size_t bytes, Raise raise) {
-        if (bytes <= 48u * 1024u) return cudaSuccess;
+    cudaError_t ensure_on(int dev, size_t bytes, size_t fixed, Raise raise) {
+        if (bytes + fixed <= kSharedWithoutOptIn) return cudaSuccess;
         if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
         if (set[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
         std::lock_guard<std::mutex> lock(mu);

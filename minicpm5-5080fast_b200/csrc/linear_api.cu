@@ -486,8 +486,8 @@ int32_t mc_sm100_debug_optin_selftest(void) {
     static SmemOptIn o;                       // zero-initialised
     std::atomic<int> raised[kMaxDevices];
     for (auto& r : raised) r.store(0);
-    auto on = [&](int dev, size_t bytes, cudaError_t result = cudaSuccess) {
-        return o.ensure_on(dev, bytes, [&] { raised[dev].fetch_add(1); return result; });
+    auto on = [&](int dev, size_t bytes, cudaError_t result = cudaSuccess, size_t fixed = 0) {
+        return o.ensure_on(dev, bytes, fixed, [&] { raised[dev].fetch_add(1); return result; });
     };
     if (on(0, 40u * 1024u) != cudaSuccess || raised[0] != 0) return 1;          // below 48 KB: nothing to raise
     if (on(0, 100u * 1024u) != cudaSuccess || raised[0] != 1) return 2;         // first use on device 0
@@ -499,6 +499,10 @@ int32_t mc_sm100_debug_optin_selftest(void) {
     if (on(64, 100u * 1024u) != cudaErrorInvalidDevice || on(-1, 100u * 1024u) != cudaErrorInvalidDevice) return 8;
     if (on(2, 100u * 1024u, cudaErrorInvalidValue) != cudaErrorInvalidValue || o.recorded(2) != 0u) return 9;   // a failed raise is not remembered
     if (on(2, 100u * 1024u) != cudaSuccess || raised[2] != 2) return 10;
+    // static shared memory counts: 48 KB hold both parts or are raised by the dynamic one
+    if (on(3, 48u * 1024u - 32u, cudaSuccess, 32u) != cudaSuccess || raised[3] != 0) return 12;
+    if (on(3, 48u * 1024u - 16u, cudaSuccess, 32u) != cudaSuccess || raised[3] != 1 || o.recorded(3) != 48u * 1024u - 16u) return 13;
+    if (on(3, 48u * 1024u, cudaSuccess, 32u) != cudaSuccess || raised[3] != 2) return 14;
     // host threads racing for one device: exactly one raise
     std::thread th[8];
     for (auto& t : th) t = std::thread([&] { for (int i = 0; i < 1000; ++i) (void)on(5, 150u * 1024u); });

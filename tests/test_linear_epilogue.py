@@ -485,3 +485,14 @@ def test_activations_over_every_bf16(pkg, act):
     assert np.all(d <= bound[:, 0]), (act, z[ok][np.argmax(d / bound[:, 0])], float(np.max(d / bound[:, 0])))
     assert np.isnan(got[np.isnan(z), 0]).all()
     assert got[np.isposinf(z), 0][0] == np.inf
+
+
+@pytest.mark.gpu
+def test_one_row_that_needs_48_kb_is_a_process_s_first_call():
+    """The activation alone fits the 48 KB that a launch may take unasked, with the kernel's static shared memory it does not."""
+    import subprocess
+    import sys
+    code = ("import sys; sys.path[:0] = %r\nimport importlib, test_linear_epilogue as t\npkg = importlib.import_module('minicpm5-5080fast_b200')\n"
+            "for K, e4m3 in ((24560, False), (12272, True)):\n    for gated in (False, True):\n        t._run(pkg, 1, 8, K, e4m3, gated=gated)") % [p for p in sys.path if p]
+    p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0, p.stderr[-2000:]

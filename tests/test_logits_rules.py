@@ -438,3 +438,41 @@ def test_prompt_then_steps_eager_and_replayed(pkg):
         again2.append(again["token"].tolist())
     assert again2 == drawn
     assert torch.equal(again["counts"], s["counts"]) and torch.equal(again["seen"], s["seen"])
+
+
+def _many_slots(pkg, slots, vocab, seed):
+    """As many sequences as slots, in turned order, a few tokens each: every entry of the rebuilt tables."""
+    import gpu_util as g
+    import torch
+    r = np.random.default_rng(seed)
+    tokens = r.integers(0, vocab, (slots, 50)).astype(np.int32)
+    tokens[:, 0], tokens[:, 1], tokens[:, 2] = 0, vocab - 1, -1
+    counts = torch.full((slots, vocab), 9, dtype=torch.int32, device="cuda")
+    seen = torch.full((slots, (vocab + 31) // 32), -1, dtype=torch.int32, device="cuda")
+    order = r.permutation(slots).astype(np.int32)
+    pkg.token_history(counts, seen, g.dev(tokens.reshape(-1)), slots, vocab, offsets=g.dev(np.arange(slots + 1, dtype=np.uint32) * 50),
+                      prompt_len=g.dev(np.full(slots, 20, np.uint32)), slots=g.dev(order), rebuild=True)
+    g.sync()
+    want, known = np.zeros((slots, vocab), np.int32), np.zeros((slots, vocab), bool)
+    onp.token_history(want, known, [(int(order[i]), tokens[i].tolist(), 20) for i in range(slots)], True)
+    assert np.array_equal(counts.cpu().numpy(), want)
+    assert np.array_equal(seen.cpu().numpy().view(np.uint32), onp.pack_bits(known))
+
+
+# A CTA of the rebuild takes ceil(vocab / floor(4 * 148 / slots)) tokens, a multiple of 32 between 2048 and 13664: sizes in front of, inside
+# and behind the spans (11904 .. 11936) whose counters and bits pass 48 KB only together with the kernel's static shared memory.
+@pytest.mark.gpu
+@pytest.mark.parametrize("slots,vocab", [(64, 106800), (64, 107000), (64, 107136), (64, 107200), (52, 130800), (33, 202048), (64, 122753), (64, 20000), (148, 54657), (300, 30001)])
+def test_history_of_many_slots(pkg, slots, vocab):
+    _many_slots(pkg, slots, vocab, slots + vocab)
+
+
+@pytest.mark.gpu
+def test_history_of_many_slots_is_a_process_s_first_call():
+    """No earlier call has raised the kernel's shared memory."""
+    import subprocess
+    import sys
+    code = ("import sys; sys.path[:0] = %r\nimport importlib, test_logits_rules as t\n"
+            "t._many_slots(importlib.import_module('minicpm5-5080fast_b200'), 64, 107000, 1)") % [p for p in sys.path if p]
+    p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0, p.stderr[-2000:]
