@@ -496,3 +496,24 @@ def test_one_row_that_needs_48_kb_is_a_process_s_first_call():
             "for K, e4m3 in ((24560, False), (12272, True)):\n    for gated in (False, True):\n        t._run(pkg, 1, 8, K, e4m3, gated=gated)") % [p for p in sys.path if p]
     p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert p.returncode == 0, p.stderr[-2000:]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(4096, 11520, 2304, True, False), (2048, 2304, 5760, False, True), (301, 2304, 2304, False, False), (33, 122753, 2304, False, False)])
+def test_same_bits_between_other_calls(pkg, shape):
+    """Calls one behind the other without a wait, another call's inputs between them: every output of the first inputs has the same bits."""
+    import torch
+    M, N, K, gated, e4m3 = shape
+    g = torch.Generator(device="cuda")
+    g.manual_seed(M)
+    n_out = N // 2 if gated else N
+    w = torch.randint(0, 0x70, (N, K), dtype=torch.uint8, generator=g, device="cuda") if e4m3 else (torch.randn(N, K, generator=g, device="cuda") * 0.02).bfloat16()
+    sc = torch.rand(N, generator=g, device="cuda") * 1e-3 if e4m3 else None
+    xs = [torch.randn(M, K, generator=g, device="cuda").bfloat16() for _ in range(2)]
+    ys = [torch.full((M, n_out), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(9)]
+    for i, y in enumerate(ys):
+        pkg.launch_linear_epilogue(w, sc, xs[1 if i % 3 == 1 else 0], y, M, N, K, activation="silu" if gated else "none", gated=gated)
+    torch.cuda.synchronize()
+    for i, y in enumerate(ys):
+        assert torch.equal(y, ys[1 if i % 3 == 1 else 0]), i
+    assert bool(torch.isfinite(ys[0]).all()) and not torch.equal(ys[0], ys[1])
