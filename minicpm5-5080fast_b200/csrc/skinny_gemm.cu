@@ -68,6 +68,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     return false;
 }
 
+// The same for a whole warp.  Every lane polls for itself, and when a wait runs out elsewhere while the phase turns, some may
+// see the phase and others the flag: what stands behind (elect.sync, tcgen05.ld, __syncwarp) wants all of them on one path.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status)) != 0;
+}
+
 template <int KIND_F8>
 __device__ __forceinline__ void mma_issue(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
     if constexpr (KIND_F8) {
@@ -235,13 +241,14 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         // ---------------------------------------------------------------- MMA issuer: the warp together, one lane elected to issue
         bool ok = true;
         uint32_t s = 0, par = 0;
-        for (uint32_t it = 0; it < nloc && ok; ++it) {
-            ok = mbar_wait(op_full(s), par, abortp, a.status);
+        // A lane whose wait ran out stays in the loop and issues nothing: elect.sync and __syncwarp want all 32.  The elected lane
+        // is the same every time.
+        for (uint32_t it = 0; it < nloc; ++it) {
+            if (ok) ok = mbar_wait(op_full(s), par, abortp, a.status);
             if (ok && E4) ok = mbar_wait(conv_done(s), par, abortp, a.status);
-            if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint64_t da = make_desc(sA + s * G::A_OP), db = make_desc(sB + s * G::B_OP);
-            if (elect_lane()) {
+            if (elect_lane() && ok) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)   // 4 x (K = 32 bytes) per 128-byte row
                     mma_issue<MODE == SKINNY_W8A8>(tmem_base, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), IDESC,
@@ -251,7 +258,7 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             __syncwarp();
             if (++s == OPS) { s = 0; par ^= 1u; }
         }
-        if (ok && nloc > 0 && elect_lane()) mma_commit(accum_bar);
+        if (elect_lane() && ok && nloc > 0) mma_commit(accum_bar);
         __syncwarp();
     } else if constexpr (E4) {
         // ---------------------------------------------------------------- e4m3 -> bf16 widening
@@ -328,7 +335,7 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     asm volatile("barrier.cluster.wait;" ::: "memory");              // completes the arrive of the prologue
     if (warp >= 2 && warp < 6) {
         const uint32_t q = warp & 3u;       // the TMEM lane quarter this warp may read
-        const bool ok = nloc > 0 && mbar_wait(accum_bar, 0u, abortp, a.status);
+        const bool ok = nloc > 0 && mbar_wait_warp(accum_bar, 0u, abortp, a.status);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t nl = q * 32u + lane, owner = nl / per_n;
         uint32_t remote;
