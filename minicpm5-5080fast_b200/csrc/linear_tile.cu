@@ -501,6 +501,10 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 if (S > 1u) {
                     // the cluster's rings are idle: they become the exchange [source split][row of the part][per] of fp32
                     cluster_sync();
+                    // A CTA whose wait ran out pushes sums that are not finished: whoever adds them up stores nothing either.
+                    if (!ok || *abortp != 0)
+                        for (uint32_t p = 0; p < csize; ++p)
+                            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to_rank(smem_u32(&abort_flag), p)), "r"(1u) : "memory");
                     uint32_t turn = 0;
                     for (uint32_t o = 0; o < S; ++o) {
                         if (o == split) continue;

@@ -337,6 +337,13 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         const uint32_t q = warp & 3u;       // the TMEM lane quarter this warp may read
         const bool ok = nloc > 0 && mbar_wait_warp(accum_bar, 0u, abortp, a.status);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        // a CTA whose wait ran out pushes sums that are not finished: whoever adds them up stores nothing either
+        if (!ok || *abortp != 0)
+            for (uint32_t p = 0; p < S; ++p) {
+                uint32_t flag;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(flag) : "r"(smem_u32(&abort_flag)), "r"(p));
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(flag), "r"(1u) : "memory");
+            }
         const uint32_t nl = q * 32u + lane, owner = nl / per_n;
         uint32_t remote;
         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote)
