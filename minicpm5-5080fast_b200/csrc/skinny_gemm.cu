@@ -467,6 +467,10 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         }
     }
     __syncthreads();
+    if (*abortp != 0) {                                              // a wait ran out: let this CTA's copies in flight land before it leaves
+        const unsigned long long t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    }
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
