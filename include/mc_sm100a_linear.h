@@ -303,6 +303,8 @@ typedef struct mc_sm100_linear_epilogue_t {
  * aligned d_w and d_x, K * (bytes per weight) and x_stride * 2 multiples of 16 take the kernels that stream; anything else a
  * slower one with plain loads.  y overlaps neither x nor, but for the whole, the residual.  Results do not depend on the
  * launch: no atomics, a fixed order of every sum.
+ * The waits inside the tensor-core kernels are bounded, 200 ms without progress each: where one runs out, y or a part of it stays
+ * as it was, after the call has returned MC_OK, and mc_sm100_debug_take_error alone says so.
  * The arguments come in one struct (copied before the call returns).  The kernel's launch and set-up may run under the end
  * of the previous kernel in the stream, but with pdl == 0 it reads nothing, and with pdl != 0 only the weights and what
  * belongs to them (scale), before that end. */

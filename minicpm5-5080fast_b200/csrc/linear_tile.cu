@@ -27,6 +27,7 @@ constexpr uint32_t kResBuf = 2048;                             // an epilogue wa
 constexpr uint32_t kWarpBuf = 4096;
 constexpr uint32_t kTileNapNs = 1000000u;                      // a poll may sleep this long; spinning warps take issue slots from working ones
 constexpr unsigned long long kTileWaitNs = 200ull * 1000ull * 1000ull;
+constexpr uint32_t kProgress = 16;                             // stages between two marks of the producer
 
 __device__ int g_tile_error;
 
@@ -72,8 +73,11 @@ __device__ __forceinline__ void tile_of(const TileArgs& a, uint32_t t, uint32_t&
 // acquire at cluster scope: arrivals come from both CTAs of a pair.  Every lane polls for itself: where a wait runs out while
 // the phase turns, some lanes of a warp may see the phase and others the flag.  What stands behind (elect.sync, tcgen05.ld,
 // __syncwarp) wants all 32, so no lane leaves a warp's loop alone.
-__device__ __forceinline__ bool tile_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
+// The limit is a stage's; who waits for a whole slice of K hands over the count that this CTA's producer keeps (kProgress), and the
+// clock starts anew whenever it has moved: a slice of 2^22 K blocks takes a second and more.
+__device__ __forceinline__ bool tile_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status, const volatile uint32_t* progress = nullptr) {
     unsigned long long t0 = 0;
+    uint32_t seen = 0;
     for (uint32_t spin = 0;; ++spin) {
         uint32_t done;
         asm volatile(
@@ -85,8 +89,13 @@ __device__ __forceinline__ bool tile_wait(uint32_t bar, uint32_t parity, volatil
         if (*abort_flag) return false;
         if ((spin & 15u) == 15u) {
             const unsigned long long now = global_timer_ns();
-            if (t0 == 0) t0 = now;
-            else if (now - t0 > kTileWaitNs) break;
+            if (t0 == 0) {
+                t0 = now;
+                if (progress != nullptr) seen = *progress;
+            } else if (now - t0 > kTileWaitNs) {
+                if (progress == nullptr || *progress == seen) break;
+                t0 = now; seen = *progress;
+            }
         }
     }
     *abort_flag = 1;
@@ -369,6 +378,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     __shared__ __align__(8) uint64_t bars[36];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
+    __shared__ uint32_t progress;
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -397,7 +407,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint32_t early = CG == 1 ? min(nloc, EARLY) : 0u;
     static_assert(STAGES >= EARLY && (WB == 2 || RAWS >= EARLY), "the early stages are all the ring's");
     if (tid == EPI * 32u) {
-        abort_flag = 0;
+        abort_flag = 0; progress = 0u;
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
         for (uint32_t s = 0; s < STAGES; ++s) { mbar_init(full(s), 1u + (WB == 1 ? CONV_WARPS * CG : 0u)); mbar_init(empty(s), 1); }
@@ -440,6 +450,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_slot;
     volatile int* abortp = &abort_flag;
+    volatile uint32_t* progressp = &progress;
     pdl_wait();
 
     if (warp < EPI) {
@@ -488,7 +499,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 if (part_of_warp != split % parts) c_hi = c_lo;
                 const uint32_t c_first = c_lo + group * 32u;
                 if (a.ep.res != nullptr && c_first < c_hi) io.fetch_res((n0 + c_first) >> a.ep.gated);
-                if (ok) ok = tile_wait(acc_full(b), (i / bufs) & 1u, abortp, a.status);
+                if (ok) ok = tile_wait(acc_full(b), (i / bufs) & 1u, abortp, a.status, progressp);
                 __syncwarp();
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t taddr = tmem + b * G::COLS + ((q * 32u) << 16);
@@ -563,6 +574,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                             if (it < early) continue;
                             if (it >= STAGES) ok = tile_wait(empty(s), ((it / STAGES) - 1u) & 1u, abortp, a.status);
                             if (!ok) break;
+                            if (it % kProgress == 0u) *progressp = it;
                             if (leader) mbar_expect_tx(full(s), CG * (G::A + (WB == 2 ? G::B : 0u)));
                             const uint32_t bar = CG == 2 ? map_to_rank(full(s), lead) : full(s);
 #pragma unroll

@@ -37,13 +37,17 @@ constexpr int kConvThreads = 256;  // warps 2..9
 constexpr uint32_t kConvGroup = 128;  // converter threads that share one K block (two groups)
 constexpr uint32_t kNapNs = 1000000u;   // a poll may sleep this long; spinning warps take issue slots from working ones
 constexpr unsigned long long kWaitLimitNs = 200ull * 1000ull * 1000ull;   // a wait gives up after 200 ms
+constexpr uint32_t kProgress = 16;      // stages between two marks of the producer
 
 __device__ int g_skinny_error;     // set when a bounded wait ran out (read back by tests)
 
 // Bounded wait on a phase parity.  Returns false when the limit ran out or
 // another role already gave up (abort flag in shared memory).
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
+// The limit is a stage's; who waits for a whole slice of K hands over the count that this CTA's producer keeps (kProgress), and the
+// clock starts anew whenever it has moved: a slice of 2^21 K blocks takes 0.3 s and more.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status, const volatile uint32_t* progress = nullptr) {
     unsigned long long t0 = 0;
+    uint32_t seen = 0;
     for (uint32_t spin = 0;; ++spin) {
         uint32_t done;
         asm volatile(
@@ -58,8 +62,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
         if ((spin & 15u) == 15u) {            // look at the clock now and then; bound the wait in TIME
             unsigned long long now;
             asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
-            if (t0 == 0) t0 = now;
-            else if (now - t0 > kWaitLimitNs) break;
+            if (t0 == 0) {
+                t0 = now;
+                if (progress != nullptr) seen = *progress;
+            } else if (now - t0 > kWaitLimitNs) {
+                if (progress == nullptr || *progress == seen) break;
+                t0 = now; seen = *progress;
+            }
         }
     }
     *abort_flag = 1;
@@ -70,8 +79,8 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 
 // The same for a whole warp.  Every lane polls for itself, and when a wait runs out elsewhere while the phase turns, some may
 // see the phase and others the flag: what stands behind (elect.sync, tcgen05.ld, __syncwarp) wants all of them on one path.
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
-    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status)) != 0;
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status, const volatile uint32_t* progress) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status, progress)) != 0;
 }
 
 template <int KIND_F8>
@@ -140,6 +149,7 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     __shared__ __align__(8) uint64_t bars[41];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
+    __shared__ uint32_t progress;
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -166,7 +176,7 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     const uint32_t pre = nloc < WS ? nloc : WS;
     if (tid == 0) {
         if constexpr (EXT) { if (a.ep.wait_first) pdl_wait(); }
-        abort_flag = 0;
+        abort_flag = 0; progress = 0u;
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
         for (uint32_t s = 0; s < OPS; ++s) { mbar_init(op_full(s), 1); mbar_init(op_empty(s), 1); }
         if (E4) {
@@ -196,6 +206,7 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
     const uint32_t tmem_base = tmem_slot;
     volatile int* abortp = &abort_flag;
+    volatile uint32_t* progressp = &progress;
     // warps 2..9 have nothing to do yet: they ask for the next kernel's weights (HBM -> L2)
     if (tid >= 64u) prefetch_next_weights(a.pf, blockIdx.x, tid - 64u, kThreads - 64u);
 
@@ -218,6 +229,7 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     const uint32_t s = it % OPS;
                     ok = mbar_wait(op_empty(s), ((it / OPS) - 1u) & 1u, abortp, a.status);
                     if (!ok) break;
+                    if (it % kProgress == 0u) *progressp = it;
                     mbar_expect_tx(op_full(s), G::A_OP + G::B_OP);
                     tma_load_2d(sA + s * G::A_OP, &map_w, op_full(s), (int32_t)((kb0 + it) * BK), n0);
                     tma_load_2d(sB + s * G::B_OP, &map_x, op_full(s), (int32_t)((kb0 + it) * BK), 0);
@@ -335,7 +347,8 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     asm volatile("barrier.cluster.wait;" ::: "memory");              // completes the arrive of the prologue
     if (warp >= 2 && warp < 6) {
         const uint32_t q = warp & 3u;       // the TMEM lane quarter this warp may read
-        const bool ok = nloc > 0 && mbar_wait_warp(accum_bar, 0u, abortp, a.status);
+        // e4m3: these warps have widened the slice themselves, so that little of it is left
+        const bool ok = nloc > 0 && mbar_wait_warp(accum_bar, 0u, abortp, a.status, E4 ? nullptr : progressp);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         // a CTA whose wait ran out pushes sums that are not finished: whoever adds them up stores nothing either
         if (!ok || *abortp != 0)

@@ -517,3 +517,49 @@ def test_same_bits_between_other_calls(pkg, shape):
     for i, y in enumerate(ys):
         assert torch.equal(y, ys[1 if i % 3 == 1 else 0]), i
     assert bool(torch.isfinite(ys[0]).all()) and not torch.equal(ys[0], ys[1])
+
+
+def _long_k(pkg, M, K, e4m3):
+    """One feature, zeros but for some places around every cut of K: sums of small whole numbers, exact in every order."""
+    import gpu_util as g
+    import torch
+    r = np.random.default_rng(M)
+    cuts = np.arange(9, dtype=np.int64) * (K // 8)
+    at = np.unique(np.clip(np.concatenate([cuts - 65, cuts - 64, cuts - 1, cuts, cuts + 63, cuts + 64, r.integers(0, K, 40)]), 0, K - 1))
+    wv, xv = r.integers(1, 3, at.size), r.integers(-2, 3, (M, at.size))
+    w = torch.zeros(K, dtype=torch.uint8 if e4m3 else torch.bfloat16, device="cuda")
+    w[g.dev(at)] = g.dev(np.where(wv == 2, 0x40, 0x38).astype(np.uint8)) if e4m3 else g.dev(wv.astype(np.float32)).bfloat16()
+    x = torch.zeros((M, K), dtype=torch.bfloat16, device="cuda")
+    for m in range(M):
+        x[m, g.dev(at)] = g.dev(xv[m].astype(np.float32)).bfloat16()
+    sc = torch.ones(1, device="cuda") if e4m3 else None
+    y = torch.full((M, 1), float("nan"), dtype=torch.bfloat16, device="cuda")
+    begin, end = torch.cuda.Event(True), torch.cuda.Event(True)
+    begin.record()
+    pkg.launch_linear_epilogue(w, sc, x, y, M, 1, K)
+    end.record()
+    torch.cuda.synchronize()
+    assert pkg.debug_take_error() == 0, "a wait ran out"
+    want = xv @ wv
+    assert np.abs(want).max() <= 256                                # whole numbers that bf16 holds
+    assert y[:, 0].float().tolist() == want.tolist()
+    return begin.elapsed_time(end)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_the_longest_sums(pkg, e4m3):
+    """K = 2^30: a CTA's slice takes longer than the limit of a single wait."""
+    for M in (1, 2):
+        assert _long_k(pkg, M, 2 ** 30, e4m3) > 200.0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("plan", [(1, 64, 1), (2, 128, 1), (1, 128, 2), (2, 256, 2)])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_the_longest_sums_of_a_tile(pkg, plan, e4m3):
+    pkg.debug_set_tile_plan(*plan)
+    try:
+        assert _long_k(pkg, 1, 2 ** 28 * plan[2], e4m3) > 200.0
+    finally:
+        pkg.debug_set_tile_plan()
