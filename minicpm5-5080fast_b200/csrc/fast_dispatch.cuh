@@ -10,17 +10,35 @@
 
 namespace mcl {
 
+// CTAs of a launch, one a group of `rows` weight rows at most.
+inline uint32_t fast_grid(int epi, uint32_t rows, uint32_t N) {
+    const uint32_t groups = (N + rows - 1u) / rows;
+    uint32_t gx = (uint32_t)sm_count();
+    if (groups < gx) gx = groups;
+    if (epi == EPI_ARGMAX && gx > kArgmaxCands) gx = kArgmaxCands;
+    return gx;
+}
+
+// Dynamic shared memory of a launch: the activation, with the fused epilogue the biases and residuals of a CTA's groups behind it.
+constexpr size_t kFastMostShared = 200u * 1024u;
+inline size_t fast_shared_bytes(int wb, int pro, int epi, uint32_t rows, uint32_t N, uint32_t K) {
+    const uint32_t groups = (N + rows - 1u) / rows, gx = fast_grid(epi, rows, N);
+    const size_t fused = epi == EPI_FUSED || epi == EPI_FUSED_GATED ? (size_t)((groups + gx - 1u) / gx) * (rows + (epi == EPI_FUSED ? rows : 1u)) * 2u : 0u;
+    return (size_t)K * (wb == 1 ? 4u : 2u) + (pro == PRO_RESNORM ? (size_t)K * 4u : 0u) + fused;
+}
+
+// Whether the M = 1 kernel with the fused epilogue takes a call, whichever of its tile shapes (one or two rows a group) that gets.
+inline bool fast_fused_fits(int wb, bool gated, uint32_t N, uint32_t K) {
+    const int epi = gated ? EPI_FUSED_GATED : EPI_FUSED;
+    return fast_shared_bytes(wb, PRO_NONE, epi, 2u, N, K) <= kFastMostShared && (gated || fast_shared_bytes(wb, PRO_NONE, epi, 1u, N, K) <= kFastMostShared);
+}
+
 template <int WB, int R, int U, bool PRE, bool DB, int PRO, int EPI, int T, int MINB = 1>
 inline mc_status_t launch_fast_one(const RowsArgs& a, cudaStream_t stream, bool pdl) {
     auto kern = gemv_fast_kernel<WB, R, U, PRE, DB, PRO, EPI, T, MINB>;
-    const uint32_t groups = (a.N + R - 1) / R;
-    uint32_t gx = (uint32_t)sm_count();
-    if (groups < gx) gx = groups;
-    if (EPI == EPI_ARGMAX && gx > kArgmaxCands) gx = kArgmaxCands;
-    // fused epilogue: bias and residual entries of a CTA's groups
-    const size_t fused = EPI == EPI_FUSED || EPI == EPI_FUSED_GATED ? (size_t)((groups + gx - 1u) / gx) * (R + (EPI == EPI_FUSED ? R : 1)) * 2u : 0u;
-    const size_t smem = (size_t)a.K * (WB == 1 ? 4u : 2u) + (PRO == PRO_RESNORM ? (size_t)a.K * 4u : 0u) + fused;
-    if (smem > 200u * 1024u) {
+    const uint32_t gx = fast_grid(EPI, R, a.N);
+    const size_t smem = fast_shared_bytes(WB, PRO, EPI, R, a.N, a.K);
+    if (smem > kFastMostShared) {
         set_error("gemv: activation of %zu bytes does not fit in shared memory", smem);
         return MC_E_UNSUPPORTED;
     }

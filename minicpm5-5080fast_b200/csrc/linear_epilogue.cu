@@ -161,7 +161,7 @@ extern "C" mc_status_t mc_sm100_linear_epilogue(const mc_sm100_linear_epilogue_t
     // previous kernel; what it reads before that end is nothing (e.wait_first), or with `pdl` the weights.
     // rows that a 16-byte unit divides, at aligned addresses: the kernels that stream
     const bool unit = aligned16(d_w) && aligned16(d_x) && ((uint64_t)K * (uint32_t)wb) % 16u == 0u;
-    if (M == 1u && unit && (uint64_t)K * (wb == 1 ? 4u : 2u) + (uint64_t)N / 16u <= 200u * 1024u) {       // the activation in shared memory
+    if (M == 1u && unit && fast_fused_fits(wb, d.gated != 0u, N, K)) {       // the activation in shared memory
         RowsArgs a{};
         a.w = d_w; a.scale = d_scale; a.x = d_x; a.y = d_y; a.N = N; a.K = K; a.y_stride = ys; a.kseg = K; a.ep = e;
         const NextWeights nw = take_next_weights();

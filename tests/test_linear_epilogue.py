@@ -563,3 +563,25 @@ def test_the_longest_sums_of_a_tile(pkg, plan, e4m3):
         assert _long_k(pkg, 1, 2 ** 28 * plan[2], e4m3) > 200.0
     finally:
         pkg.debug_set_tile_plan()
+
+
+# The activation of one row stands in shared memory where 200 KB hold it with the biases and residuals of a CTA's outputs: 102400 bf16
+# or, behind e4m3 weights, 51200 are exactly 200 KB.
+@pytest.mark.gpu
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("N", [1, 8, 15, 66, 300])
+@pytest.mark.parametrize("around", [-32, -16, 0, 16])
+def test_one_row_with_the_longest_activations(pkg, N, around, e4m3):
+    K = (51200 if e4m3 else 102400) + around
+    _run(pkg, 1, N, K, e4m3, seed=N)
+    _run(pkg, 1, N, K, e4m3, bias=True, residual=True, act="silu", seed=N + 1)
+    if N % 2 == 0:
+        _run(pkg, 1, N, K, e4m3, bias=True, residual=True, act="gelu", gated=True, seed=N + 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(2304, 11520), (500, 30000), (5000, 9216)])
+def test_one_row_with_long_activations(pkg, shape):
+    for e4m3 in (False, True):
+        _run(pkg, 1, *shape, e4m3, bias=True, residual=True, act="relu", seed=3)
+        _run(pkg, 1, *shape, e4m3, bias=True, in_place=True, act="silu", gated=True, seed=4)
