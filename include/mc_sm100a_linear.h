@@ -739,11 +739,11 @@ MC_SM100_API void mc_sm100_debug_chain_plan(int32_t fp8, uint32_t hidden, uint32
 /* How mc_sm100_linear_epilogue cuts a call that takes the tiled tensor-core kernel (more than 64 rows; from 17 on where K is short
  * or the weights have many rows; host logic alone):
  * CTAs per tile (1 or 2, 128 rows each), features per tile, K slices.  set_tile_plan: A/B and test hook (process-wide),
- * every such call takes this plan (cg = 0: the rule again; as many K slices as fit the shape).  No plan changes a result
- * beyond the order of its sums. */
+ * every such call takes this plan (cg = 0: the rule again; as many K slices as fit the shape): 1 CTA with 64 or 128 features, 2 with
+ * 128 or 256, 1, 2 or 4 slices; others are refused and change nothing.  No plan changes a result beyond the order of its sums. */
 MC_SM100_API void mc_sm100_debug_tile_plan(int32_t bytes_per_weight, uint32_t M, uint32_t N, uint32_t K, uint32_t sms, uint32_t* cg,
                                            uint32_t* bn, uint32_t* splits);
-MC_SM100_API void mc_sm100_debug_set_tile_plan(uint32_t cg, uint32_t bn, uint32_t splits);
+MC_SM100_API mc_status_t mc_sm100_debug_set_tile_plan(uint32_t cg, uint32_t bn, uint32_t splits);
 
 /* Host-only self-test of the per-device bookkeeping behind the kernels' shared-memory opt-in (one entry per
  * device, raised once per device and size, safe under racing host threads); makes no CUDA call.  0 = passed. */

@@ -123,7 +123,7 @@ SIGNATURES = {
     "mc_sm100_debug_set_mma_rows": (None, [_i32]),
     "mc_sm100_debug_mma_rows_plan": (None, [_u32, _u32, _vp, _vp, _vp]),
     "mc_sm100_debug_tile_plan": (None, [_i32, _u32, _u32, _u32, _u32, _vp, _vp, _vp]),
-    "mc_sm100_debug_set_tile_plan": (None, [_u32, _u32, _u32]),
+    "mc_sm100_debug_set_tile_plan": (_i32, [_u32, _u32, _u32]),
     "mc_sm100_debug_chain_plan": (None, [_i32, _u32, _u32, _vp, _vp, _vp, _vp]),
     "mc_sm100_debug_set_math": (None, [_i32, _i32]),
     "mc_sm100_debug_take_error": (_i32, []),
@@ -432,7 +432,7 @@ def debug_tile_plan(bytes_per_weight: int, M: int, N: int, K: int, sms: int = 14
 
 def debug_set_tile_plan(cg: int = 0, bn: int = 0, splits: int = 1) -> None:
     """Fused linears whose rows TMA can read take the tiled kernel with this plan (cg = 0: the library's rule)."""
-    lib().mc_sm100_debug_set_tile_plan(cg, bn, splits)
+    _check(lib().mc_sm100_debug_set_tile_plan(cg, bn, splits))
 
 
 def debug_chain_plan(fp8: bool, hidden: int, inter: int):

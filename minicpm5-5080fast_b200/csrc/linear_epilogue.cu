@@ -184,7 +184,10 @@ extern "C" mc_status_t mc_sm100_linear_epilogue(const mc_sm100_linear_epilogue_t
     return linear_any(wb, d_w, d_x, xs, M, N, K, e, st, true);
 }
 
-extern "C" void mc_sm100_debug_set_tile_plan(uint32_t cg, uint32_t bn, uint32_t splits) { tile_force(cg, bn, splits); }
+extern "C" mc_status_t mc_sm100_debug_set_tile_plan(uint32_t cg, uint32_t bn, uint32_t splits) {
+    clear_error();
+    return tile_force(cg, bn, splits);
+}
 
 extern "C" void mc_sm100_debug_tile_plan(int32_t bytes_per_weight, uint32_t M, uint32_t N, uint32_t K, uint32_t sms, uint32_t* cg,
                                          uint32_t* bn, uint32_t* splits) {

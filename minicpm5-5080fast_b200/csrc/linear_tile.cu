@@ -763,14 +763,14 @@ mc_status_t launch_tile(const void* w, const uint16_t* x, uint32_t x_pitch, uint
 //                 MMA the widest); e4m3 0.29 - 0.41 (widening)
 //   an epilogue   1.0 for 64 columns, e4m3 1.2 times that (fewer registers)
 //   a K slice     2.4 for barriers and a cluster's start, 3.4 with pairs, 1.2 per 32 columns sent away
+struct TileForm { uint32_t cg, bn, splits; double block[2]; };
+static constexpr TileForm kForms[] = {{1, 64, 1, {0.19, 0.29}}, {1, 64, 2, {0.19, 0.29}}, {1, 64, 4, {0.19, 0.29}}, {1, 128, 1, {0.24, 0.41}},
+                                      {1, 128, 2, {0.24, 0.41}}, {1, 128, 4, {0.24, 0.41}}, {2, 128, 1, {0.245, 0.30}}, {2, 128, 2, {0.245, 0.30}},
+                                      {2, 128, 4, {0.245, 0.30}}, {2, 256, 1, {0.295, 0.36}}, {2, 256, 2, {0.295, 0.36}}, {2, 256, 4, {0.295, 0.36}}};
 TilePlan tile_plan(int wb, uint32_t M, uint32_t N, uint32_t K, uint32_t sms) {
-    struct Form { uint32_t cg, bn, splits; double block[2]; };
-    static const Form forms[] = {{1, 64, 1, {0.19, 0.29}}, {1, 64, 2, {0.19, 0.29}}, {1, 64, 4, {0.19, 0.29}}, {1, 128, 1, {0.24, 0.41}},
-                                 {1, 128, 2, {0.24, 0.41}}, {1, 128, 4, {0.24, 0.41}}, {2, 128, 1, {0.245, 0.30}}, {2, 128, 2, {0.245, 0.30}},
-                                 {2, 128, 4, {0.245, 0.30}}, {2, 256, 1, {0.295, 0.36}}, {2, 256, 2, {0.295, 0.36}}, {2, 256, 4, {0.295, 0.36}}};
     TilePlan best{2, 256, 1};
     double least = 1e30;
-    for (const Form& f : forms) {
+    for (const TileForm& f : kForms) {
         const uint32_t per = stage_blocks(wb, (int)f.bn), stages = (K + per * kBK - 1u) / (per * kBK);
         if (f.splits > stages) continue;
         const double tiles = (double)((M + 128ull * f.cg - 1) / (128ull * f.cg)) * (double)((N + f.bn - 1ull) / f.bn);
@@ -788,10 +788,20 @@ TilePlan tile_plan(int wb, uint32_t M, uint32_t N, uint32_t K, uint32_t sms) {
     return best;
 }
 
-// benchmark and test hook: every call takes this plan (cg = 0: the rule above)
+// benchmark and test hook: every call takes this plan (cg = 0: the rule above).  Only the plans that the rule chooses from: a slice
+// of the exchange is a whole number of 32 columns, or of rows.
 static std::atomic<uint32_t> g_forced{0};
 bool tile_forced() { return g_forced.load() != 0u; }
-void tile_force(uint32_t cg, uint32_t bn, uint32_t splits) { g_forced.store(cg == 0u ? 0u : (cg << 24) | (splits << 16) | bn); }
+mc_status_t tile_force(uint32_t cg, uint32_t bn, uint32_t splits) {
+    bool known = cg == 0u;
+    for (const TileForm& f : kForms) known = known || (f.cg == cg && f.bn == bn && f.splits == splits);
+    if (!known) {
+        set_error("mc_sm100_debug_set_tile_plan: no plan of %u CTAs, %u features, %u slices", cg, bn, splits);
+        return MC_E_INVALID_ARGUMENT;
+    }
+    g_forced.store(cg == 0u ? 0u : (cg << 24) | (splits << 16) | bn);
+    return MC_OK;
+}
 
 mc_status_t linear_tile(int wb, const void* w, const uint16_t* x, uint32_t x_pitch, uint32_t M, uint32_t N, uint32_t K,
                         const EpiArgs& ep, cudaStream_t stream, bool pdl) {

@@ -15,7 +15,8 @@ struct TilePlan { uint32_t cg, bn, splits; };
 TilePlan tile_plan(int wb, uint32_t M, uint32_t N, uint32_t K, uint32_t sms);
 
 bool tile_forced();                                           // such a plan is set
-void tile_force(uint32_t cg, uint32_t bn, uint32_t splits);   // every call takes this plan; cg = 0: tile_plan
+// Every call takes this plan; cg = 0: tile_plan's.  A plan that tile_plan does not choose from is refused and changes nothing.
+mc_status_t tile_force(uint32_t cg, uint32_t bn, uint32_t splits);
 
 // 1 when a bounded wait inside the kernel ran out since the last query (clears it), -1 on a CUDA error.
 int linear_tile_take_error();

@@ -69,6 +69,18 @@ def test_tile_plan(pkg):
         assert pkg.debug_tile_plan(wb, 300, 300, 300, 1)[0] in (1, 2)
 
 
+def test_plans_that_the_tiled_kernel_does_not_have_are_refused(pkg):
+    """The hook takes the plans of the rule; anything else leaves what was set."""
+    for plan in ((1, 64, 3), (1, 128, 3), (2, 128, 3), (1, 64, 0), (1, 64, 8), (2, 256, 8), (1, 64, 256), (1, 256, 1), (2, 64, 1), (3, 128, 1), (1, 0, 1),
+                 (1, 64 + 65536, 1), (257, 64, 1)):
+        with pytest.raises(pkg.McError) as e:
+            pkg.debug_set_tile_plan(*plan)
+        assert e.value.status == pkg.MC_E_INVALID_ARGUMENT and "no plan" in e.value.message, plan
+    for plan in PLANS:
+        pkg.debug_set_tile_plan(*plan)
+    pkg.debug_set_tile_plan()
+
+
 # ---- GPU -------------------------------------------------------------------------------------------------------------
 def _make(M, N, K, e4m3, bias, residual, gated, seed):
     n_out = N // 2 if gated else N
