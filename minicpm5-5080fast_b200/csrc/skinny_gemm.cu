@@ -601,7 +601,11 @@ static uint32_t plan_args(int mode, uint32_t M, uint32_t N, uint32_t K, SkinnyAr
     // no longer become resident (and prefetch its weights) while this one drains.
     const uint32_t npad = M <= 16 ? 16u : (M <= 32 ? 32u : 64u);
     const uint32_t op_stage = (uint32_t)(kTileN + npad) * kRowBytes;
-    const uint32_t budget = 108u * 1024u - (npad + 4u) * p.splits * slice_rows(p.splits) * 4u - 1024u;  // minus the split-K exchange region
+    const uint32_t exchange = (npad + 4u) * p.splits * slice_rows(p.splits) * 4u;     // the split-K exchange region
+    // Fused, 33 to 64 rows: all of the 112 KB that the launch opts in for, less its 2 KB.  The exchange of 3, 6 or 7 slices is a little
+    // larger than that of the powers of two and cost a stage (M = 48: 10000 x 8192 40.3 -> 34.8 us, 5000 x 5760 20.2 -> 18.4,
+    // e4m3 41.3 -> 40.3 and 20.6 -> 20.3); fewer rows keep their stages either way.
+    const uint32_t budget = (ext && npad == 64u ? 112u * 1024u - 2048u : 107u * 1024u) - exchange;
     if (mode == SKINNY_W_E4M3) {
         // operand ring of 3 (2 when the raw ring would otherwise drop below 2 stages)
         a.op_stages = (budget >= 3u * op_stage + 2u * kTileN * 64u) ? 3u : 2u;

@@ -597,3 +597,13 @@ def test_one_row_with_long_activations(pkg, shape):
     for e4m3 in (False, True):
         _run(pkg, 1, *shape, e4m3, bias=True, residual=True, act="relu", seed=3)
         _run(pkg, 1, *shape, e4m3, bias=True, in_place=True, act="silu", gated=True, seed=4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("shape", [(40, 10000, 3584), (64, 5000, 5312), (48, 9600, 4112), (33, 5632, 2816)])
+def test_three_and_six_slices_of_many_rows(pkg, shape, e4m3):
+    """33 to 64 rows, K cut in three (74 to 90 row tiles) or six (38 to 44): the rings that stand beside the larger exchange."""
+    _run(pkg, *shape, e4m3, bias=True, residual=True, act="silu", seed=shape[0])
+    _run(pkg, *shape, e4m3, bias=True, residual=True, act="gelu", gated=True, seed=shape[0] + 1)
+    assert pkg.debug_take_error() == 0
