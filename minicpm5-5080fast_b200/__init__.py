@@ -346,10 +346,21 @@ def _a(t) -> int:
     return t if t.__class__ is int else t.data_ptr()
 
 
+def _width(call: str, what: str):
+    raise McError(MC_E_INVALID_ARGUMENT, f"{call}: {what}")
+
+
+# Where the three calls are given tensors, their element widths are looked at (a | b is 4 only where both are: widths are powers
+# of two): a table of bytes, 64-bit tokens or codes without their scales would be read beyond the tensor's end or as something else.
 def launch_linear_epilogue(w, scale, x, y, M, N, K, bias=None, residual=None, activation="none", gated=False, x_stride=0,
                            y_stride=0, residual_stride=0, stream=None, pdl=False):
-    """y = act(x W^T * scale + bias) [* up] + residual for any M; activation: a key of ACTIVATIONS."""
+    """y = act(x W^T * scale + bias) [* up] + residual for any M; activation: a key of ACTIVATIONS.  w holds 16-bit elements (bf16),
+    or with fp32 scales 8-bit ones (e4m3 codes); everything else 16-bit ones."""
     try:                                          # tensors, without a call of _a for each
+        if (w.itemsize != 2 if scale is None else w.itemsize != 1 or scale.itemsize != 4):
+            _width("launch_linear_epilogue", "bf16 weights without scales, or 8-bit codes with fp32 scales")
+        if x.itemsize | y.itemsize | (2 if bias is None else bias.itemsize) | (2 if residual is None else residual.itemsize) != 2:
+            _width("launch_linear_epilogue", "x, y, bias and residual hold 16-bit elements (bf16)")
         call = _pack_linear(88, M, N, K, ACTIVATIONS[activation], gated, x_stride, y_stride, residual_stride, 0, w.data_ptr(),
                             0 if scale is None else scale.data_ptr(), x.data_ptr(), y.data_ptr(), 0 if bias is None else bias.data_ptr(),
                             0 if residual is None else residual.data_ptr())
@@ -362,39 +373,63 @@ def launch_linear_epilogue(w, scale, x, y, M, N, K, bias=None, residual=None, ac
 
 
 def logits_tables(table_vocab, counts=None, seen=None, masks=None, bias_token=None, bias_value=None, status=None) -> bytes:
-    """Tables of logits_process out of device tensors (their sizes give the numbers of rows); the caller keeps the tensors."""
-    words = (table_vocab + 31) // 32
-    slots = 0 if counts is None else counts.numel() // table_vocab                          # one without the other is refused
-    if seen is not None:
-        n = seen.numel() // words
+    """Tables of logits_process out of contiguous device tensors of 32-bit words (their bytes give the numbers of rows); the caller
+    keeps the tensors."""
+    words, width = (table_vocab + 31) // 32, 4
+    slots = masked = biases = d_counts = d_seen = d_mask = d_token = d_value = 0
+    if counts is not None:
+        width |= counts.itemsize
+        slots, d_counts = counts.nbytes // (4 * table_vocab), counts.data_ptr()
+    if seen is not None:                                                                    # one without the other is refused
+        width |= seen.itemsize
+        n, d_seen = seen.nbytes // (4 * words), seen.data_ptr()
         slots = n if counts is None or n < slots else slots
-    biases = 0 if bias_token is None else bias_token.numel()
+    if masks is not None:
+        width |= masks.itemsize
+        masked, d_mask = masks.nbytes // (4 * words), masks.data_ptr()
+    if bias_token is not None:
+        width |= bias_token.itemsize
+        biases, d_token = bias_token.nbytes >> 2, bias_token.data_ptr()
     if bias_value is not None:
-        n = bias_value.numel()
+        width |= bias_value.itemsize
+        n, d_value = bias_value.nbytes >> 2, bias_value.data_ptr()
         biases = n if bias_token is None or n < biases else biases
-    return _pack_tables(72, table_vocab, slots, 0 if masks is None else masks.numel() // words, biases, 0,
-                        0 if counts is None else counts.data_ptr(), 0 if seen is None else seen.data_ptr(), 0 if masks is None else masks.data_ptr(),
-                        0 if bias_token is None else bias_token.data_ptr(), 0 if bias_value is None else bias_value.data_ptr(),
-                        0 if status is None else status.data_ptr())
+    if width != 4:
+        _width("logits_tables", "tables hold 32-bit words")
+    return _pack_tables(72, table_vocab, slots, masked, biases, 0, d_counts, d_seen, d_mask, d_token, d_value, 0 if status is None else status.data_ptr())
 
 
 def logits_process(logits, out, n_rows, vocab, row_stride, out_stride, cfg, tables, index_base=0, stream=None, pdl=False):
     """cfg: device tensor of n_rows x 8 words (rep, freq, pres penalty as f32 bits, history slot, mask row, bias begin, bias count, 0)."""
-    rc = (_lib or lib()).mc_sm100_logits_process(_pack_logits(48, n_rows, vocab, row_stride, out_stride, index_base, _a(logits), _a(out), _a(cfg)),
-                                                 tables, (_current_stream or _stream)() if stream is None else _stream(stream), pdl)
+    try:
+        if logits.itemsize | out.itemsize != 2 or cfg.itemsize != 4:
+            _width("logits_process", "logits and out hold 16-bit elements (bf16), cfg 32-bit words")
+        call = _pack_logits(48, n_rows, vocab, row_stride, out_stride, index_base, logits.data_ptr(), out.data_ptr(), cfg.data_ptr())
+    except AttributeError:
+        call = _pack_logits(48, n_rows, vocab, row_stride, out_stride, index_base, _a(logits), _a(out), _a(cfg))
+    rc = (_lib or lib()).mc_sm100_logits_process(call, tables, (_current_stream or _stream)() if stream is None else _stream(stream), pdl)
     if rc:
         _check(rc)
 
 
 def token_history(counts, seen, tokens, n_seqs, table_vocab, offsets=None, prompt_len=None, slots=None, n_tokens=None, n_slots=None,
                   rebuild=False, status=None, stream=None, pdl=False):
+    """Token lists into the counts and seen bits of their slots; every tensor holds 32-bit words."""
     if n_tokens is None:
         n_tokens = tokens.numel()
     if n_slots is None:
         n_slots = counts.numel() // table_vocab
-    rc = (_lib or lib()).mc_sm100_token_history(_pack_history(80, n_slots, table_vocab, n_tokens, n_seqs, rebuild, _a(counts), _a(seen), _a(tokens),
-                                                              _a(offsets), _a(prompt_len), _a(slots), _a(status)),
-                                                (_current_stream or _stream)() if stream is None else _stream(stream), pdl)
+    try:
+        if (counts.itemsize | seen.itemsize | tokens.itemsize | (4 if offsets is None else offsets.itemsize) | (4 if prompt_len is None else prompt_len.itemsize)
+                | (4 if slots is None else slots.itemsize)) != 4:
+            _width("token_history", "counts, seen, tokens, offsets, prompt_len and slots hold 32-bit words")
+        call = _pack_history(80, n_slots, table_vocab, n_tokens, n_seqs, rebuild, counts.data_ptr(), seen.data_ptr(), tokens.data_ptr(),
+                             0 if offsets is None else offsets.data_ptr(), 0 if prompt_len is None else prompt_len.data_ptr(),
+                             0 if slots is None else slots.data_ptr(), 0 if status is None else status.data_ptr())
+    except AttributeError:
+        call = _pack_history(80, n_slots, table_vocab, n_tokens, n_seqs, rebuild, _a(counts), _a(seen), _a(tokens), _a(offsets), _a(prompt_len),
+                             _a(slots), _a(status))
+    rc = (_lib or lib()).mc_sm100_token_history(call, (_current_stream or _stream)() if stream is None else _stream(stream), pdl)
     if rc:
         _check(rc)
 

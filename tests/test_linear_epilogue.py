@@ -81,6 +81,20 @@ def test_plans_that_the_tiled_kernel_does_not_have_are_refused(pkg):
     pkg.debug_set_tile_plan()
 
 
+def test_tensors_of_other_widths_are_refused(pkg):
+    """The binding decides between bf16 and e4m3 by the scales: codes without them, and anything else that is not as wide as what it
+    stands for, is refused before the call (nothing is launched: the tensors are the host's)."""
+    import torch
+    t = lambda dtype, *s: torch.zeros(s, dtype=dtype)  # noqa: E731
+    bf, u8, f32, f64 = torch.bfloat16, torch.uint8, torch.float32, torch.float64
+    ok = dict(w=t(bf, 8, 16), scale=None, x=t(bf, 1, 16), y=t(bf, 1, 8))
+    for bad in (dict(w=t(u8, 8, 16)), dict(w=t(f32, 8, 16)), dict(scale=t(f32, 8)), dict(w=t(u8, 8, 16), scale=t(bf, 8)), dict(w=t(u8, 8, 16), scale=t(f64, 8)),
+                dict(x=t(f32, 1, 16)), dict(x=t(u8, 1, 16)), dict(y=t(f32, 1, 8)), dict(y=t(u8, 1, 8)), dict(bias=t(f32, 8)), dict(residual=t(f32, 1, 8))):
+        with pytest.raises(pkg.McError) as e:
+            pkg.launch_linear_epilogue(**{**ok, **bad}, M=1, N=8, K=16, stream=16)
+        assert e.value.status == pkg.MC_E_INVALID_ARGUMENT and "launch_linear_epilogue: " in e.value.message, list(bad)
+
+
 # ---- GPU -------------------------------------------------------------------------------------------------------------
 def _make(M, N, K, e4m3, bias, residual, gated, seed):
     n_out = N // 2 if gated else N

@@ -90,6 +90,30 @@ def test_history_refusals(pkg):
     assert pkg.lib().mc_sm100_token_history(None, None, 0) == pkg.MC_E_INVALID_ARGUMENT
 
 
+def test_tensors_of_other_widths_are_refused(pkg):
+    """Truth values for bits, 64-bit tokens or offsets, fp32 logits: refused by the binding before the call (nothing is launched: the
+    tensors are the host's)."""
+    import torch
+    t = lambda dtype, *s: torch.zeros(s, dtype=dtype)  # noqa: E731
+    i32, i64, bf, f32, f64, yes = torch.int32, torch.int64, torch.bfloat16, torch.float32, torch.float64, torch.bool
+    for bad in (dict(counts=t(i64, 2, 100)), dict(counts=t(torch.int16, 2, 100)), dict(seen=t(yes, 2, 100)), dict(seen=t(i64, 2, 4)), dict(masks=t(yes, 2, 100)),
+                dict(bias_token=t(i64, 3)), dict(bias_value=t(bf, 3)), dict(bias_value=t(f64, 3))):
+        kw = {**dict(counts=t(i32, 2, 100), seen=t(i32, 2, 4), masks=t(i32, 2, 4), bias_token=t(i32, 3), bias_value=t(f32, 3)), **bad}
+        with pytest.raises(pkg.McError) as e:
+            pkg.logits_tables(100, **kw)
+        assert e.value.status == pkg.MC_E_INVALID_ARGUMENT and "logits_tables: " in e.value.message, list(bad)
+    for bad in (dict(logits=t(f32, 1, 100)), dict(out=t(f32, 1, 100)), dict(cfg=t(i64, 1, 8)), dict(cfg=t(bf, 1, 8))):
+        kw = {**dict(logits=t(bf, 1, 100), out=t(bf, 1, 100), cfg=t(i32, 1, 8)), **bad}
+        with pytest.raises(pkg.McError) as e:
+            pkg.logits_process(**kw, n_rows=1, vocab=100, row_stride=100, out_stride=100, tables=_tables(pkg), stream=16)
+        assert e.value.status == pkg.MC_E_INVALID_ARGUMENT and "logits_process: " in e.value.message, list(bad)
+    for bad in [{k: t(i64, 8)} for k in ("counts", "seen", "tokens", "offsets", "prompt_len", "slots")] + [dict(seen=t(yes, 8)), dict(tokens=t(torch.int16, 8))]:
+        kw = {**{k: t(i32, 8) for k in ("counts", "seen", "tokens", "offsets", "prompt_len", "slots")}, **bad}
+        with pytest.raises(pkg.McError) as e:
+            pkg.token_history(**kw, n_seqs=1, table_vocab=4, n_slots=1, n_tokens=4, stream=16)
+        assert e.value.status == pkg.MC_E_INVALID_ARGUMENT and "token_history: " in e.value.message, list(bad)
+
+
 # ---- GPU: logits -----------------------------------------------------------------------------------------------------
 def _config(rows):
     a = np.zeros((len(rows), 8), np.uint32)
