@@ -512,8 +512,9 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 if (S > 1u) {
                     // the cluster's rings are idle: they become the exchange [source split][row of the part][per] of fp32
                     cluster_sync();
-                    // A CTA whose wait ran out pushes sums that are not finished: whoever adds them up stores nothing either.
-                    if (!ok || *abortp != 0)
+                    // Sums that did not come are pushed all the same: whoever adds them up stores nothing either.  (Where they came
+                    // they are whole: the lane that commits them has seen every stage.)
+                    if (!ok)
                         for (uint32_t p = 0; p < csize; ++p)
                             asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to_rank(smem_u32(&abort_flag), p)), "r"(1u) : "memory");
                     uint32_t turn = 0;
@@ -647,10 +648,9 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 constexpr uint32_t R = RAWS;
                 const uint32_t group = (warp - (EPI + 4u)) / CONV_WARPS, ct = tid & (CONV_WARPS * 32u - 1u);
                 const uint32_t my_tiles = cid < a.tiles ? (a.tiles - cid + clusters - 1u) / clusters : 0u, total = my_tiles * (kb1 - kb0);
-                // A lane whose wait ran out stays with its warp, whose barriers want all 32, and widens what there is: the flag that it
-                // has raised stands in front of every arrival behind it, and this CTA's epilogue stores nothing.  A pair's other CTA
-                // does not see the flag; there the whole warp leaves without the arrival.  (Leaving by a vote in single CTAs too:
-                // M = 301, 2304 x 2304 13.6 -> 14.4 us.)
+                // A lane whose wait ran out stays with its warp, whose barriers want all 32, up to the vote behind the second wait:
+                // the whole warp leaves there, without the arrival on a stage that would miss a part.  The arrival in front of it
+                // hands back a raw stage that the lane has not read, which nobody misses.
                 for (uint32_t it = group; it < total; it += 2u) {
                     const uint32_t r = it % R, s = it % STAGES;
                     bool ok = tile_wait(raw_full(r), (it / R) & 1u, abortp, a.status);
@@ -669,7 +669,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     __syncwarp();
                     if (lane == 0) mbar_arrive(raw_empty(r));
                     if (it >= STAGES) ok = tile_wait(empty(s), ((it / STAGES) - 1u) & 1u, abortp, a.status) && ok;
-                    if constexpr (CG == 2) { if (!__all_sync(0xFFFFFFFFu, ok)) break; }
+                    if (!__all_sync(0xFFFFFFFFu, ok)) break;
 #pragma unroll
                     for (uint32_t i = 0; i < PER; ++i) {
                         sts16(sB + s * G::B + swz(row0 + 32u * i, 2u * cc), wide[i][0]);

@@ -42,7 +42,8 @@ constexpr uint32_t kProgress = 16;      // stages between two marks of the produ
 __device__ int g_skinny_error;     // set when a bounded wait ran out (read back by tests)
 
 // Bounded wait on a phase parity.  Returns false when the limit ran out or
-// another role already gave up (abort flag in shared memory).
+// another role already gave up (abort flag in shared memory).  Every lane polls for itself: when a wait runs out elsewhere while
+// the phase turns, some lanes of a warp may see the phase and others the flag, so none leaves the loop of a warp that works together.
 // The limit is a stage's; who waits for a whole slice of K hands over the count that this CTA's producer keeps (kProgress), and the
 // clock starts anew whenever it has moved: a slice of 2^21 K blocks takes 0.3 s and more.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status, const volatile uint32_t* progress = nullptr) {
@@ -75,12 +76,6 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     g_skinny_error = 1;
     if (status != nullptr) *reinterpret_cast<volatile int32_t*>(status) = 1;
     return false;
-}
-
-// The same for a whole warp.  Every lane polls for itself, and when a wait runs out elsewhere while the phase turns, some may
-// see the phase and others the flag: what stands behind (elect.sync, tcgen05.ld, __syncwarp) wants all of them on one path.
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status, const volatile uint32_t* progress) {
-    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status, progress)) != 0;
 }
 
 template <int KIND_F8>
@@ -348,10 +343,12 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     if (warp >= 2 && warp < 6) {
         const uint32_t q = warp & 3u;       // the TMEM lane quarter this warp may read
         // e4m3: these warps have widened the slice themselves, so that little of it is left
-        const bool ok = nloc > 0 && mbar_wait_warp(accum_bar, 0u, abortp, a.status, E4 ? nullptr : progressp);
+        const bool ok = mbar_wait(accum_bar, 0u, abortp, a.status, E4 ? nullptr : progressp);
+        __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        // a CTA whose wait ran out pushes sums that are not finished: whoever adds them up stores nothing either
-        if (!ok || *abortp != 0)
+        // Sums that did not come are pushed all the same: whoever adds them up stores nothing either.  (Where they came they are whole:
+        // the lane that commits them has seen every stage.)
+        if (!ok)
             for (uint32_t p = 0; p < S; ++p) {
                 uint32_t flag;
                 asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(flag) : "r"(smem_u32(&abort_flag)), "r"(p));
@@ -364,18 +361,14 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 #pragma unroll
         for (int c0 = 0; c0 < NPAD; c0 += 16) {
             uint32_t r[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) r[j] = 0u;
-            if (ok) {
-                const uint32_t taddr = tmem_base + ((q * 32u) << 16) + (uint32_t)c0;
-                asm volatile(
-                    "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                    : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                      "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                    : "r"(taddr)
-                    : "memory");
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            }
+            const uint32_t taddr = tmem_base + ((q * 32u) << 16) + (uint32_t)c0;
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                  "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                : "r"(taddr)
+                : "memory");
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
             for (int j = 0; j < 16; j += 4)
                 asm volatile("st.shared::cluster.v4.u32 [%0], {%1,%2,%3,%4};"
