@@ -272,7 +272,8 @@ MC_SM100_API mc_status_t mc_sm100_residual_rmsnorm_rows(uint16_t* d_res, const u
 
 /* Activations of mc_sm100_linear_epilogue, in fp32:
  * relu max(z, 0) (a NaN stays one), gelu z / 2 * (1 + erf(z / sqrt 2)), gelu_tanh
- * z / 2 * (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))), silu z / (1 + e^-z). */
+ * z / 2 * (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))), silu z / (1 + e^-z).  Of -infinity the last three give a NaN, as their
+ * formulas do, relu 0; silu and gelu_tanh of less than 1e-36 in size may come out as 0. */
 typedef enum mc_sm100_activation_t {
     MC_SM100_ACT_NONE = 0, MC_SM100_ACT_RELU = 1, MC_SM100_ACT_GELU = 2, MC_SM100_ACT_GELU_TANH = 3, MC_SM100_ACT_SILU = 4
 } mc_sm100_activation_t;

@@ -18,12 +18,14 @@ struct EpiArgs {
 
 #if defined(__CUDACC__)
 
-// __expf and __fdividef are off by a few units of 2^-23; the result is rounded to bf16 (2^-9) right after.
+// __expf and __fdividef are off by a few units of 2^-23 (e^-a by a * 2^-24 more); the result is rounded to bf16 (2^-9) right after.
+// __fdividef gives 0 for divisors above 2^126: from a = -87.4 on, where the value is below 1e-36.
 __device__ __forceinline__ float epi_sigmoid_mul(float z, float a) { return __fdividef(z, 1.0f + __expf(-a)); }   // z / (1 + e^-a)
 
 // z Phi(z), Phi(-a) = erfc(a / sqrt 2) / 2 = t Q(t) e^(-a^2 / 2) with t = 1 / (1 + 0.36 a), the form of Hastings' approximations; Q is
-// our own fit (weighted least squares against erfcx over 0 <= a <= 14: 9e-7 of the value, with fp32 rounding 7e-6), so that the
-// negative tail keeps its digits.  erfcf, exact to a few units, is most of an epilogue: M 3563, 22400 x 368, 242 us; this 151.
+// our own fit (weighted least squares against erfcx over 0 <= a <= 14: 9e-7 of the value), so that the negative tail keeps its
+// digits: the exponent, up to 120, is rounded twice, which adds up to 2 * 120 * 2^-24 * ln 2 = 1e-5 of the value at z = -13 and
+// 2e-6 at z = -6 (where z has the few digits of a bf16, z * z is exact and half of that goes).  erfcf, exact to a few units, is most of an epilogue: M 3563, 22400 x 368, 242 us; this 151.
 __device__ __forceinline__ float epi_gelu(float z) {
     const float t = __fdividef(1.0f, fmaf(0.36f, fabsf(z), 1.0f));
     float q = fmaf(0.04705774784f, t, -0.17976957560f);

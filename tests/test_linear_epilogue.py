@@ -621,3 +621,22 @@ def test_three_and_six_slices_of_many_rows(pkg, shape, e4m3):
     _run(pkg, *shape, e4m3, bias=True, residual=True, act="silu", seed=shape[0])
     _run(pkg, *shape, e4m3, bias=True, residual=True, act="gelu", gated=True, seed=shape[0] + 1)
     assert pkg.debug_take_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,want", [("none", -np.inf), ("relu", 0.0), ("gelu", np.nan), ("gelu_tanh", np.nan), ("silu", np.nan)])
+def test_activations_of_minus_infinity(pkg, act, want):
+    """z is -infinity through the bias of every third feature: each kernel gives what the formula's own operations give; its neighbours
+    stay finite."""
+    import gpu_util as g
+    for M, N, K in ((1, 96, 64), (6, 96, 64), (40, 96, 2048), (140, 96, 64), (9, 96, 63)):
+        for e4m3 in (False, True):
+            w, q, sc, x, b, _ = _make(M, N, K, e4m3, True, False, False, M)
+            b = b.copy()
+            b[::3] = 0xFF80
+            y = g.empty_u16(M, N)
+            pkg.launch_linear_epilogue(g.dev(q if e4m3 else w), g.dev(sc) if e4m3 else None, g.dev(x), y, M, N, K, bias=g.dev(b), activation=act)
+            g.sync()
+            got = onp.bf16_to_f32(g.host_u16(y))
+            assert np.array_equal(got[:, ::3], np.full_like(got[:, ::3], want), equal_nan=True), (M, e4m3)
+            assert np.isfinite(np.delete(got, np.s_[::3], axis=1)).all()
