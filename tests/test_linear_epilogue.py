@@ -640,3 +640,58 @@ def test_activations_of_minus_infinity(pkg, act, want):
             got = onp.bf16_to_f32(g.host_u16(y))
             assert np.array_equal(got[:, ::3], np.full_like(got[:, ::3], want), equal_nan=True), (M, e4m3)
             assert np.isfinite(np.delete(got, np.s_[::3], axis=1)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(2, 40, 12272), (8, 40, 12288), (5, 33, 12272), (9, 40, 5872), (16, 40, 5888), (16, 33, 5872)])
+def test_few_rows_around_the_longest_staged_activation(pkg, shape):
+    """e4m3, up to 16 rows: the whole activation stands in shared memory up to K = 12280 (from nine rows on 5880)."""
+    _run(pkg, *shape, True, bias=True, residual=True, act="silu", seed=shape[0])
+
+
+def _captured_first():
+    """A process's first calls, recorded into a graph and replayed: what a call asks of its kernel once happens under capture."""
+    import importlib
+    import gpu_util as g
+    import torch
+    pkg = importlib.import_module("minicpm5-5080fast_b200")
+    f, jobs = onp.bf16_to_f32, []
+    for M, N, K, e4m3 in ((1, 40, 512, False), (1, 40, 24560, False), (1, 40, 512, True), (5, 40, 512, True), (20, 40, 2048, False), (40, 136, 2048, True),
+                          (130, 136, 512, False), (130, 136, 512, True), (3, 40, 77, False)):
+        w, q, sc, x, b, r = _make(M, N, K, e4m3, True, True, False, M)
+        dev = [g.dev(q if e4m3 else w), g.dev(sc) if e4m3 else None, g.dev(x), g.empty_u16(M, N), g.dev(b), g.dev(r)]
+        jobs.append((M, N, K, dev, onp.linear_epilogue_f64(onp.e4m3_to_f32(q) if e4m3 else f(w), f(x), sc, f(b), f(r), "silu")))
+    V = 107000
+    counts, seen = torch.full((64, V), 9, dtype=torch.int32, device="cuda"), torch.full((64, (V + 31) // 32), -1, dtype=torch.int32, device="cuda")
+    tokens = np.random.default_rng(1).integers(0, V, (64, 9)).astype(np.int32)
+    d_tokens, d_offsets = g.dev(tokens.reshape(-1)), g.dev(np.arange(65, dtype=np.uint32) * 9)
+    lg, out = onp.seeded_bf16(3, (64, V), 2.0), g.empty_u16(64, V)
+    cfg = np.zeros((64, 8), np.uint32)
+    cfg[:, :3] = np.float32([1.5, 0.5, 0.25]).view(np.uint32)
+    cfg[:, 3], cfg[:, 4] = np.arange(64), 0xFFFFFFFF
+    d_lg, d_cfg = g.dev(lg), g.dev(cfg)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for M, N, K, (w, sc, x, y, b, r), _ in jobs:
+            pkg.launch_linear_epilogue(w, sc, x, y, M, N, K, bias=b, residual=r, activation="silu")
+        pkg.token_history(counts, seen, d_tokens, 64, V, offsets=d_offsets, rebuild=True)
+        pkg.logits_process(d_lg, out, 64, V, V, V, d_cfg, pkg.logits_tables(V, counts=counts, seen=seen))
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for M, N, K, dev, (want, bound) in jobs:
+        assert np.all(np.abs(f(g.host_u16(dev[3])) - want) <= bound), (M, N, K)
+    c, s = np.zeros((64, V), np.int32), np.zeros((64, V), bool)
+    onp.token_history(c, s, [(i, tokens[i].tolist(), 0) for i in range(64)], True)
+    assert np.array_equal(counts.cpu().numpy(), c) and np.array_equal(seen.cpu().numpy().view(np.uint32), onp.pack_bits(s))
+    assert np.array_equal(g.host_u16(out), np.stack([onp.logits_process_f32(lg[i], (1.5, 0.5, 0.25), c[i], s[i], None, [], []) for i in range(64)]))
+
+
+@pytest.mark.gpu
+def test_a_process_s_first_calls_are_captured():
+    import subprocess
+    import sys
+    code = "import sys; sys.path[:0] = %r\nimport test_linear_epilogue as t\nt._captured_first()" % [p for p in sys.path if p]
+    p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0, p.stderr[-2000:]
