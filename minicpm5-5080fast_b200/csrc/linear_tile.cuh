@@ -1,4 +1,5 @@
-// linear_tile.cuh -- interface of the tiled tcgen05 GEMM with the fused epilogue (prompt chunks, M > 64).
+// linear_tile.cuh -- interface of the tiled tcgen05 GEMM with the fused epilogue (prompt chunks, M > 64; from 17 rows on where K is
+// short, from 33 where the weights have many rows).
 #pragma once
 
 #include "linear_epilogue.cuh"
