@@ -504,10 +504,10 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t taddr = tmem + b * G::COLS + ((q * 32u) << 16);
                 const uint32_t row = q * 32u + lane - part_of_warp * rows;          // in its part
-                auto release = [&]() {                                               // this warp has read its part of the accumulator
+                auto release = [&]() {       // this warp has read its part of the accumulator; one that did not come is not given back
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) { if (CG == 2) arrive_remote(map_to_rank(acc_empty(b), lead)); else mbar_arrive(acc_empty(b)); }
+                    if (lane == 0 && ok) { if (CG == 2) arrive_remote(map_to_rank(acc_empty(b), lead)); else mbar_arrive(acc_empty(b)); }
                 };
                 if (S > 1u) {
                     // the cluster's rings are idle: they become the exchange [source split][row of the part][per] of fp32
@@ -649,8 +649,8 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 const uint32_t group = (warp - (EPI + 4u)) / CONV_WARPS, ct = tid & (CONV_WARPS * 32u - 1u);
                 const uint32_t my_tiles = cid < a.tiles ? (a.tiles - cid + clusters - 1u) / clusters : 0u, total = my_tiles * (kb1 - kb0);
                 // A lane whose wait ran out stays with its warp, whose barriers want all 32, up to the vote behind the second wait:
-                // the whole warp leaves there, without the arrival on a stage that would miss a part.  The arrival in front of it
-                // hands back a raw stage that the lane has not read, which nobody misses.
+                // the whole warp leaves there, without the arrival on a stage that would miss a part.  A raw stage goes back only where
+                // the lane that returns it has seen it land: nobody arms a barrier whose copy is still pending.
                 for (uint32_t it = group; it < total; it += 2u) {
                     const uint32_t r = it % R, s = it % STAGES;
                     bool ok = tile_wait(raw_full(r), (it / R) & 1u, abortp, a.status);
@@ -667,7 +667,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                         widen4(v.z, wide[i][1].x, wide[i][1].y); widen4(v.w, wide[i][1].z, wide[i][1].w);
                     }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(raw_empty(r));
+                    if (lane == 0 && ok) mbar_arrive(raw_empty(r));
                     if (it >= STAGES) ok = tile_wait(empty(s), ((it / STAGES) - 1u) & 1u, abortp, a.status) && ok;
                     if (!__all_sync(0xFFFFFFFFu, ok)) break;
 #pragma unroll
